@@ -199,12 +199,13 @@ def prepare(case, seed):
         seq = torch.repeat_interleave(torch.arange(c["nseq"], device="cuda"), torch.tensor(counts, device="cuda"))
         drafted = torch.ones(rows, dtype=torch.bool, device="cuda")
         drafted[s["row_start"][1:].long() - 1] = False  # the last row of a sequence has no draft behind it
-        near = target[drafted] + normal(rows - c["nseq"], vocab) * 0.7
+        near = target + normal(rows, vocab) * 0.7
         heat = max(c["temperature"], 0.3) if c["draft"] else 0.4
         noise = -torch.log(-torch.log(torch.rand(near.shape, generator=g, device="cuda").clamp(1e-20, 1 - 1e-7)))
         draft = near.to(DTYPES[c["dtype"]])
         tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")  # the pending token, then the drafted ones
-        tokens[torch.nonzero(drafted)[:, 0] + 1] = (draft.float() / heat + noise * (1.0 if c["temperature"] else 0.3)).argmax(1).to(torch.int32)
+        guess = (draft.float() / heat + noise * (1.0 if c["temperature"] else 0.3)).argmax(1).to(torch.int32)
+        tokens[torch.nonzero(drafted)[:, 0] + 1] = guess[drafted]
         s.update(target=target.to(DTYPES[c["dtype"]]), draft=draft if c["draft"] else None, tokens=tokens, seq=seq)
         s.update(uniforms=torch.rand(rows, generator=g, device="cuda"), draws=torch.rand(c["nseq"], generator=g, device="cuda"))
         return s
@@ -395,7 +396,7 @@ def _verify(s, c):
         px = p[row, following]
         if s["draft"] is not None:
             q = probabilities(s["draft"])
-            qx = q[(row - seq).clamp(max=rows - nseq - 1), following] if rows > nseq else torch.ones_like(px)
+            qx = q[row, following]
         else:
             qx = torch.ones_like(px)
         good = s["uniforms"].double() * qx < px
@@ -412,10 +413,8 @@ def _verify(s, c):
         if s["draft"] is None:
             left = pe.clone()
             left[torch.arange(nseq, device="cuda"), following[end]] = 0.0
-        elif rows > nseq:
-            left = (pe - q[(end - torch.arange(nseq, device="cuda")).clamp(max=rows - nseq - 1)]).clamp(min=0.0)
         else:
-            left = pe
+            left = (pe - q[end]).clamp(min=0.0)
         left = torch.where(last[end][:, None], pe, left)
         sums = torch.cumsum(left, 1)
         drawn = (sums <= s["draws"].double()[:, None] * sums[:, -1:]).sum(1).clamp(max=vocab - 1)
@@ -536,7 +535,7 @@ def _exact_verify(s, c):
                     q = torch.zeros_like(p)
                     q[x] = 1.0
                 else:
-                    q = torch.softmax(s["draft"][r0 - b + j].double() / heat, 0)
+                    q = torch.softmax(s["draft"][r0 + j].double() / heat, 0)
                 stays = bool(uniforms[r0 + j] * q[x] < p[x])
             if not stays:
                 left = torch.clamp(p - q, min=0)
