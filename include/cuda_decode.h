@@ -347,6 +347,102 @@ int cd_flash_decode_static(int dtype, int heads, int kv_heads, int hd, size_t at
                            int page_tokens, const float* d_q, const void* d_kv_pages,
                            const int* d_page_table, float* d_out, void* stream);
 
+/* ---------------------------------------------------------------- additive: operators of a serving step
+ * No counterpart in the reference, which decodes one sequence.  A batch of sequences over paged K and V on the caller's
+ * own device memory: write rotated K and V into the pages, attend, drop the least used entries, check drafted tokens.
+ *
+ * All pointers are DEVICE pointers the caller owns; the work is enqueued on `stream` (a cudaStream_t, NULL = default
+ * stream) and not synchronised; nothing is allocated.  A call may be captured into a CUDA graph.  `device` is the CUDA
+ * ordinal the pointers and the stream belong to (-1: the current device); the caller's current device is left as it was.
+ * Workspaces carry nothing from one call to the next and need no initialisation; calls that may overlap on the GPU need
+ * workspaces of their own.  A workspace starts on a 256-byte boundary.  Arguments that can be checked on the host are,
+ * first (CD_ERR_INVALID / CD_ERR_UNSUPPORTED / CD_ERR_CAPACITY, text in cd_last_error(NULL)); lengths, rows and page ids live
+ * on the device and are checked there: what does not fit is left out, as each call says, and OR-ed into *status.
+ *
+ * A batch: sequence b has the new rows row_start[b] .. row_start[b+1] - 1 of q, k, v and out (any number, none included;
+ * at most max_rows where a call asks for that) and lens[b] entries in the cache, those of its new rows being the last.
+ * Row j of n is entry lens[b] - n + j.  Rows from row_start[nseq] on are not touched. */
+enum { CD_STATUS_BATCH = 1,   /* row_start not ascending, past nrows or max_rows, or lens outside the page table: the sequence is left out */
+       CD_STATUS_PAGE = 2,    /* a page id outside the pool: its entries are not written, or count as masked */
+       CD_STATUS_LOGITS = 4 };/* a logit row that was needed holds NaN or has no finite maximum */
+
+typedef struct cd_paged_cache {
+    int32_t dtype;        /* of the pool: CD_DTYPE_F32 / F16 / BF16 */
+    int32_t kv_heads, hd; /* hd: 64 or 128 */
+    int32_t page_tokens;  /* 1 .. 65536 */
+    int32_t npages;       /* pages in the pool */
+    int32_t nseq;         /* sequences: rows of page_table, entries of lens; at most 4096 */
+    int32_t max_pages;    /* entries of a page_table row; max_pages * page_tokens < 2^31 */
+    int32_t device;
+    int64_t table_stride; /* elements from one page_table row to the next */
+    void* pool;           /* [npages][2 (k,v)][kv_heads][page_tokens][hd], 16-byte aligned */
+    const int32_t* page_table;
+    const int32_t* lens;
+    /* Bookkeeping for eviction, [nseq][kv_heads][max_pages * page_tokens] each, or NULL both: what an entry has been worth so
+     * far, and the position it was written for. */
+    float* weight;
+    int32_t* position;
+    int32_t* status;      /* one word the caller zeroes and reads when it likes, or NULL */
+} cd_paged_cache;
+
+/* Rotary positions.  The first rot_dim elements of a head turn (even, 2 .. hd), the rest pass: pair i is elements
+ * (2i, 2i+1) of an interleaved head or (i, i + rot_dim/2) of one in halves;  a' = (a cos - b sin) magnitude,
+ * b' = (a sin + b cos) magnitude at angle position * 2 pi turns[i] / 2^64.  Angles are exact to 2^-32 of a turn at any
+ * position: position * turns[i] is taken modulo 2^64. */
+enum { CD_ROPE_INTERLEAVED = 0, CD_ROPE_HALF = 1 };
+enum { CD_ROPE_PLAIN = 0, CD_ROPE_LINEAR = 1, CD_ROPE_NTK = 2, CD_ROPE_YARN = 3 };
+typedef struct cd_rope {
+    int32_t rot_dim, layout;
+    float magnitude;
+    int32_t reserved;
+    const uint64_t* turns; /* [rot_dim / 2], device */
+} cd_rope;
+/* Host: the table and the magnitude for pairs of base^(-2i/rot_dim) radians a position.  LINEAR divides every frequency by
+ * `factor`; NTK raises the base to base * factor^(rot_dim / (rot_dim - 2)); YARN keeps the pairs that turn over 32 times in
+ * `original` positions, divides those that turn less than once, blends in between, and has magnitude 0.1 ln(factor) + 1. */
+int cd_rope_frequencies(int rot_dim, double base, int scaling, double factor, int original, uint64_t* turns, float* magnitude);
+
+/* Rotate q and k (row r at positions[r]), leave q in q_out, and write k and v to their entries in the pages.  q [nrows][heads][hd], k and
+ * v [nrows][kv_heads][hd] of `dtype` (F32, or the pool's type), rows *_stride elements apart (0: packed); q_out packed, of `dtype`;
+ * it may be q itself where q is packed.  With bookkeeping the entry's weight becomes 0 and its position the row's. */
+int cd_rope_append(const cd_paged_cache* cache, const cd_rope* rope, int dtype, int heads, int nrows, const void* q, int64_t q_stride, const void* k,
+                   int64_t k_stride, const void* v, int64_t v_stride, const int32_t* positions, const int32_t* row_start, void* q_out, void* stream);
+
+/* Softmax attention of every new row over the entries up to its own (with window > 0: over the last `window` of them).
+ * q, out [nrows][heads][hd] of `dtype` (F32, or the pool's type), q rows q_stride elements apart (0: packed), out packed; heads is
+ * a multiple of kv_heads, q head h reads kv head h / (heads / kv_heads).  scale <= 0: 1/sqrt(hd).  lse [nrows][heads]: natural
+ * log of the sum of exp(score), or NULL.  A row that sees nothing gets zeros and -inf.  What a row does not see cannot
+ * reach it, NaN and infinities included.  collect != 0: the probabilities an entry got, summed over the rows and q heads of
+ * its kv head, are added to its weight.  Results do not depend on the run: nothing is summed by atomics. */
+int cd_paged_attention_workspace(const cd_paged_cache* cache, int heads, int nrows, int max_rows, int collect, size_t* bytes);
+int cd_paged_attention(const cd_paged_cache* cache, int dtype, int heads, int nrows, int max_rows, const void* q, int64_t q_stride,
+                       const int32_t* row_start, float scale, int window, int collect, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Bring every sequence with more than `keep` entries down to `keep`, for each kv head on its own.  Entries at positions below
+ * `sinks` or above the head's newest position - `recent` come first (sinks + recent <= keep), then the heaviest; of equals
+ * the one in the lower place; NaN counts as the lightest.  Kept entries that lie in places from `keep` on move into the places that
+ * fell free below, in order; the others stay where they are.  K and V move in the pool, so its pages must not be shared between
+ * sequences; lens_out [nseq], weight_out and position_out (shaped as the cache's, and may be those) receive the bookkeeping, places
+ * from the new length on as they were.  lens_out must not be lens.  Entries of a page outside the pool do not move (CD_STATUS_PAGE). */
+int cd_cache_evict_workspace(const cd_paged_cache* cache, int keep, size_t* bytes);
+int cd_cache_evict(const cd_paged_cache* cache, int keep, int sinks, int recent, int32_t* lens_out, float* weight_out, int32_t* position_out,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which drafted tokens stay.  Sequence b fed the rows row_start[b] .. : a pending token, then its drafts (tokens[r], r past the first).
+ * target [nrows][vocab] of `dtype` holds the logits behind each row, p = softmax(target / temperature); draft [nrows][vocab], where
+ * given, the logits the token drafted behind each row was drawn from (a sequence's last row of it is not read), q = softmax(draft /
+ * temperature); without it q is 1 at the drafted token.  Rows are *_stride elements apart (0: vocab).  The draft x behind row r stays while uniforms[r] q(x) < p(x); behind the first that does not, a token is drawn from
+ * max(p - q, 0), or from the last row's p where all stay: the first one whose running sum exceeds draws[b] times the whole.
+ * temperature (0, or 1e-6 .. 1e6) 0: a draft stays where it is the row's largest logit (of equals the lowest token), which is also what is drawn.
+ * accepted [nseq]: drafts that stay; out_tokens [nrows]: per sequence those, the drawn one, then -1.  A sequence without rows
+ * has accepted 0.  Where a row that is reached holds NaN or has no finite maximum the drawn token is -1 (CD_STATUS_LOGITS). */
+int cd_verify_drafts_workspace(int nrows, int nseq, int vocab, size_t* bytes);
+int cd_verify_drafts(int device, int dtype, int nseq, int nrows, int max_rows, int vocab, const void* target, int64_t target_stride,
+                     const void* draft, int64_t draft_stride, const int32_t* tokens, const int32_t* row_start, const float* uniforms,
+                     const float* draws, double temperature, int32_t* accepted, int32_t* out_tokens, int32_t* status, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- additive: host policy / samplers
  * (no device work; usable without a GPU) */
 

@@ -45,6 +45,15 @@ class CdOptions(C.Structure):
                 ("test_flags", C.c_int32), ("test_ring_kb", C.c_int32)]
 
 
+class CdPagedCache(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "kv_heads", "hd", "page_tokens", "npages", "nseq", "max_pages", "device")] + \
+               [("table_stride", C.c_int64)] + [(n, C.c_void_p) for n in ("pool", "page_table", "lens", "weight", "position", "status")]
+
+
+class CdRope(C.Structure):
+    _fields_ = [("rot_dim", C.c_int32), ("layout", C.c_int32), ("magnitude", C.c_float), ("reserved", C.c_int32), ("turns", C.c_void_p)]
+
+
 class CdRequest(C.Structure):
     _fields_ = [("decode_backend", C.c_int32), ("steps", C.c_int32), ("temperature", C.c_float),
                 ("top_k", C.c_int32), ("samples", C.c_int32), ("seed", C.c_uint64)]
@@ -125,6 +134,17 @@ SIGNATURES = {
     "cd_flash_decode": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_int, _f32p, _vp, _vp, _f32p]),
     "cd_flash_decode_static": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_int, C.c_int, _f32p, _vp,
                                          _P(C.c_int32), _f32p, _vp]),
+    "cd_rope_frequencies": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_int, _u64p, _f32p]),
+    "cd_rope_append": (C.c_int, [_P(CdPagedCache), _P(CdRope), C.c_int, C.c_int, C.c_int, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp,
+                                 _vp, _vp]),
+    "cd_paged_attention_workspace": (C.c_int, [_P(CdPagedCache), C.c_int, C.c_int, C.c_int, C.c_int, _szp]),
+    "cd_paged_attention": (C.c_int, [_P(CdPagedCache), C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_int64, _vp, C.c_float, C.c_int, C.c_int, _vp, _vp,
+                                     _vp, C.c_size_t, _vp]),
+    "cd_cache_evict_workspace": (C.c_int, [_P(CdPagedCache), C.c_int, _szp]),
+    "cd_cache_evict": (C.c_int, [_P(CdPagedCache), C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "cd_verify_drafts_workspace": (C.c_int, [C.c_int, C.c_int, C.c_int, _szp]),
+    "cd_verify_drafts": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp, _vp, _vp, C.c_double,
+                                   _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "cd_param_count": (C.c_size_t, [_P(CdConfig)]),
     "cd_select_decode_mode": (C.c_int, [_P(CdConfig), C.c_int, C.c_size_t, C.c_size_t, _P(CdSelection)]),
     "cd_backend_name": (C.c_char_p, [C.c_int]),

@@ -1,0 +1,354 @@
+// Attention of a batch's new rows over paged K and V (cd_paged_attention).
+//
+// o = sum_t p_t v_t, p = softmax(scale q k_t) over the entries a row sees.  A unit is (sequence, kv head, block of RU rows): its
+// rows are the q heads of the kv head times the sequence's new rows, so K and V are read once for all of them.  A unit's entries are cut into tiles of 64 and
+// all units' tiles lie on one line, which the CTAs share evenly: CTA i of G = min(grid, T) takes tiles [i T / G, (i + 1) T / G), whatever the lengths
+// are (they are known on the device only; every CTA adds them up for itself).  A unit that one CTA has whole is finished there;
+// the others leave (max, sum, sum of p v) per CTA in slot CTA + unit (both only ever grow along the line, so no two meet),
+// and join_kernel puts them together in the line's order.  Inside a CTA four warps share a unit: `row_warps` of them have different rows of
+// the same entries, the rest other entries.  Statistics are fp32 in the log2 domain.
+#pragma once
+#include "serve.cuh"
+
+namespace cd {
+
+constexpr int PA_THREADS = 128, PA_WARPS = 4, PA_TILE = 64, PA_MAX_CTAS = 640;
+
+struct AttnArgs {
+    PagedView c;
+    const int* row_start;
+    const void* q;
+    void* out;
+    float* lse;       // natural log, or nullptr
+    float* part_o;    // [ctas + units][ru][hd]
+    float2* part_ml;  // [ctas + units][ru] (max, sum)
+    int2* unit_info;  // [units] first CTA, CTAs
+    float* lse2;      // [nrows][heads] log2; with scores only
+    float* scores;    // [nrows][heads][score_stride] log2 domain, or nullptr
+    long long q_stride, score_stride;
+    float scale_log2;
+    int heads, group, nrows, max_rows, window, ru, row_warps, blocks;  // blocks: row blocks a sequence may have
+};
+
+struct SeqWork {
+    BatchSeq s;
+    int start, tiles, blocks;
+};
+__device__ inline SeqWork seq_work(const AttnArgs& p, int b) {
+    SeqWork w;
+    w.s = batch_seq(p.c, p.row_start, b, p.nrows, p.max_rows);
+    w.start = 0;
+    if (p.window > 0) {
+        const int first = w.s.len - w.s.n + 1 - p.window;  // of the first row
+        w.start = first > 0 ? first & ~(PA_TILE - 1) : 0;
+    }
+    w.tiles = w.s.n > 0 && w.s.len > 0 ? (w.s.len - w.start + PA_TILE - 1) / PA_TILE : 0;
+    w.blocks = (w.s.n * p.group + p.ru - 1) / p.ru;
+    return w;
+}
+
+// pre[b] = tiles of the sequences before b (all threads; ends with a barrier); returns the total
+__device__ inline long long line_up(const AttnArgs& p, long long* pre, long long* sums) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    long long carry = 0;
+    if (tid == 0) pre[0] = 0;
+    for (int base = 0; base < p.c.nseq; base += PA_THREADS) {
+        const int b = base + tid;
+        long long v = 0;
+        if (b < p.c.nseq) {
+            const SeqWork w = seq_work(p, b);
+            v = (long long)w.tiles * w.blocks * p.c.kv_heads;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += x;
+        }
+        if (lane == 31) sums[warp] = v;
+        __syncthreads();
+        long long before = carry;
+        for (int i = 0; i < PA_WARPS; ++i) {
+            if (i < warp) before += sums[i];
+            carry += sums[i];
+        }
+        if (b < p.c.nseq) pre[b + 1] = before + v;
+        __syncthreads();
+    }
+    return carry;
+}
+
+template <typename T> __device__ inline T from_float(float v);
+template <> __device__ inline float from_float<float>(float v) { return v; }
+template <> __device__ inline __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <typename T> __device__ inline float as_float(T v);
+template <> __device__ inline float as_float<float>(float v) { return v; }
+template <> __device__ inline float as_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ inline float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+constexpr float LN2 = 0.69314718055994530942f;
+
+// One row's end: o relative to 2^m with sum l.  l is 0 where nothing was seen.
+template <typename QT> __device__ inline void store_out(const AttnArgs& p, size_t row_head, int hd, int col, float o, float l) {
+    static_cast<QT*>(p.out)[row_head * hd + col] = from_float<QT>(l > 0.f || l != l ? o / l : 0.f);
+}
+__device__ inline void store_lse(const AttnArgs& p, size_t row_head, float m, float l) {
+    const float lse2 = l > 0.f || l != l ? m + log2f(l) : -INFINITY;
+    if (p.lse) p.lse[row_head] = lse2 * LN2;
+    if (p.scores) p.lse2[row_head] = lse2;
+}
+
+// What the warps of a CTA leave of a unit: o[w][rows][HD + PAD], (m, l)[w][rows], warp w = entry group * row_warps + row group.
+template <int HD, int PAD> struct UnitParts {
+    float* o;
+    float2* ml;
+};
+// Merge the entry groups and store: the result where the unit is this CTA's alone, else this CTA's slot.  All threads.
+template <typename QT, int HD, int PAD>
+__device__ inline void finish_unit(const AttnArgs& p, const UnitParts<HD, PAD>& u, int rows_per_warp, const SeqWork& w, int kvh, int block, bool whole, size_t slot) {
+    const int groups = PA_WARPS / p.row_warps, rows = min(p.ru, w.s.n * p.group - block * p.ru);
+    for (int at = threadIdx.x; at < rows * HD; at += PA_THREADS) {
+        const int r = at / HD, col = at % HD, rw = r / rows_per_warp, rr = r % rows_per_warp;
+        float m = -INFINITY;
+        for (int t = 0; t < groups; ++t) m = fmaxf(m, u.ml[(t * p.row_warps + rw) * rows_per_warp + rr].x);
+        const float base = m == -INFINITY ? 0.f : m;
+        float l = 0.f, o = 0.f;
+        for (int t = 0; t < groups; ++t) {
+            const int at_w = (t * p.row_warps + rw) * rows_per_warp + rr;
+            const float2 ml = u.ml[at_w];
+            const float f = exp2f(ml.x - base);
+            l += ml.y * f;
+            o += u.o[(size_t)at_w * (HD + PAD) + col] * f;
+        }
+        if (whole) {
+            const int rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
+            const size_t row_head = (size_t)(w.s.r0 + j) * p.heads + head;
+            store_out<QT>(p, row_head, HD, col, o, l);
+            if (col == 0) store_lse(p, row_head, m, l);
+        } else {
+            p.part_o[(slot * p.ru + r) * HD + col] = o;
+            if (col == 0) p.part_ml[slot * p.ru + r] = make_float2(m, l);
+        }
+    }
+}
+
+// Walk this CTA's share of the line; work(w, b, kvh, block, first tile, tiles, whole, slot) handles a run of one unit's tiles.
+template <typename F> __device__ inline void walk_line(const AttnArgs& p, long long* pre, long long* sums, F&& work) {
+    const long long total = line_up(p, pre, sums), ctas = min((long long)gridDim.x, total);  // no share is empty
+    if (blockIdx.x >= ctas) return;
+    long long t = total * blockIdx.x / ctas;
+    const long long end = total * (blockIdx.x + 1) / ctas;
+    while (t < end) {
+        int lo = 0, hi = p.c.nseq - 1;  // the last sequence whose tiles begin at t or before
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (pre[mid] <= t) lo = mid; else hi = mid - 1;
+        }
+        const SeqWork w = seq_work(p, lo);
+        const long long in_seq = t - pre[lo];
+        const int unit = (int)(in_seq / w.tiles), tile = (int)(in_seq % w.tiles), kvh = unit / w.blocks, block = unit % w.blocks;
+        const long long u0 = t - tile, u1 = u0 + w.tiles;  // the unit's tiles on the line
+        const int n = (int)(min(u1, end) - t);
+        const size_t slot_unit = ((size_t)lo * p.c.kv_heads + kvh) * p.blocks + block;
+        const int c0 = (int)(((u0 + 1) * ctas - 1) / total), c1 = (int)((u1 * ctas - 1) / total);  // the CTAs of its first and last tile
+        if (tile == 0 && threadIdx.x == 0) p.unit_info[slot_unit] = make_int2(c0, c1 - c0 + 1);
+        work(w, lo, kvh, block, tile, n, c0 == c1, slot_unit + blockIdx.x);
+        t += n;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ fp32 FMAs
+// Eight lanes hold one entry's K (and V) row, a warp four entries side by side; each eight lanes keep (m, l, o) of their entries
+// for four rows.
+template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS, 2) attn_fma_kernel(const __grid_constant__ AttnArgs p) {
+    constexpr int VEC = 16 / sizeof(KT), NC = HD / 8 / VEC, RW = 4, PAD = 4;  // elements of a load, loads of a lane and row
+    extern __shared__ long long pre[];
+    __shared__ long long sums[PA_WARPS];
+    __shared__ __align__(16) float so[PA_WARPS * RW * (HD + PAD)];
+    __shared__ float2 sml[PA_WARPS * RW];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l8 = lane & 7, side = lane >> 3;
+    const int rw = warp % p.row_warps, tg = warp / p.row_warps, groups = PA_WARPS / p.row_warps;
+    const KT* pool = static_cast<const KT*>(p.c.pool);
+
+    walk_line(p, pre, sums, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
+        float q[RW][NC * VEC], o[RW][NC * VEC], m[RW], l[RW];
+        int last[RW];        // the last entry a row sees, -1: none
+        float* srow[RW];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            const int rho = block * p.ru + rw * RW + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
+            const bool valid = rho < w.s.n * p.group;
+            last[r] = valid ? w.s.len - w.s.n + j : -1;
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+            srow[r] = p.scores && valid ? p.scores + ((size_t)(w.s.r0 + j) * p.heads + head) * p.score_stride : nullptr;
+            const QT* src = static_cast<const QT*>(p.q) + (size_t)(valid ? w.s.r0 + j : 0) * p.q_stride + (size_t)(valid ? head : 0) * HD;
+#pragma unroll
+            for (int i = 0; i < NC * VEC; ++i) {
+                q[r][i] = valid ? as_float(src[(i / VEC * 8 + l8) * VEC + i % VEC]) * p.scale_log2 : 0.f;
+                o[r][i] = 0.f;
+            }
+        }
+        const int first = w.start + tile * PA_TILE, end = min(w.s.len, first + tiles * PA_TILE);
+        for (int t0 = first + tg * 4 + side; __any_sync(0xffffffffu, t0 < end); t0 += groups * 4) {
+            const int page = t0 < end ? page_at(p.c, b, t0) : -1;
+            float k[NC * VEC], v[NC * VEC];
+            if (page >= 0) {
+                const KT *kr = pool + row_at(p.c, page, 0, kvh, t0, HD), *vr = pool + row_at(p.c, page, 1, kvh, t0, HD);
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    const uint4 a = __ldg(reinterpret_cast<const uint4*>(kr) + i * 8 + l8), c = __ldg(reinterpret_cast<const uint4*>(vr) + i * 8 + l8);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        k[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&a)[e]);
+                        v[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&c)[e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NC * VEC; ++i) k[i] = v[i] = 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < RW; ++r) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < NC * VEC; ++i) s = fmaf(q[r][i], k[i], s);
+#pragma unroll
+                for (int x = 1; x < 8; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+                const bool seen = page >= 0 && t0 <= last[r] && (p.window == 0 || t0 > last[r] - p.window);
+                if (!seen) s = -INFINITY;
+                if (srow[r] && l8 == r && t0 < end) srow[r][t0] = s;
+                if (!seen) continue;  // what is masked does not reach the sums, whatever its V holds
+                if (s > m[r] || s != s) {
+                    const float f = exp2f(m[r] - s);
+                    m[r] = s;
+                    l[r] *= f;
+#pragma unroll
+                    for (int i = 0; i < NC * VEC; ++i) o[r][i] *= f;
+                }
+                const float e = exp2f(s - (m[r] == -INFINITY ? 0.f : m[r]));
+                l[r] += e;
+#pragma unroll
+                for (int i = 0; i < NC * VEC; ++i) o[r][i] = fmaf(e, v[i], o[r][i]);
+            }
+        }
+        __syncthreads();  // the unit before has been read
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            float top = m[r];
+#pragma unroll
+            for (int x = 8; x < 32; x <<= 1) {
+                const float other = __shfl_xor_sync(0xffffffffu, top, x);
+                top = other > top || other != other ? other : top;
+            }
+            const float f = exp2f(m[r] - (top == -INFINITY ? 0.f : top));
+            float sum = l[r] * f;
+#pragma unroll
+            for (int x = 8; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (lane == 0) sml[warp * RW + r] = make_float2(top, sum);
+#pragma unroll
+            for (int i = 0; i < NC * VEC; ++i) {
+                float x = o[r][i] * f;
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (side == 0) so[(warp * RW + r) * (HD + PAD) + (i / VEC * 8 + l8) * VEC + i % VEC] = x;
+            }
+        }
+        __syncthreads();
+        finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sml}, RW, w, kvh, block, whole, slot);
+    });
+}
+
+// ------------------------------------------------------------------------------------------------ the joint
+// One row and q head of a unit that several CTAs shared: sum their parts in order.  Rows that see nothing get zeros here.
+template <typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS) attn_join_kernel(const __grid_constant__ AttnArgs p) {
+    __shared__ float factor[PA_MAX_CTAS], red[32];
+    __shared__ float4 acc[PA_WARPS][HD / 4];
+    const int b = blockIdx.x / p.blocks / p.c.kv_heads, kvh = blockIdx.x / p.blocks % p.c.kv_heads, block = blockIdx.x % p.blocks, r = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const SeqWork w = seq_work(p, b);
+    const int rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
+    const size_t row_head = (size_t)(w.s.r0 + j) * p.heads + head;
+    pdl_wait();  // (ahead of every return: a grid that ends early would let the next one start before the kernel ahead has ended)
+    if (rho >= w.s.n * p.group) return;
+    if (w.tiles == 0) {
+        for (int col = tid; col < HD; col += PA_THREADS) store_out<QT>(p, row_head, HD, col, 0.f, 0.f);
+        if (tid == 0) store_lse(p, row_head, 0.f, 0.f);
+        return;
+    }
+    const int2 info = __ldcg(p.unit_info + blockIdx.x);
+    const int n = info.y;
+    if (n <= 1) return;
+    const size_t slot0 = (size_t)blockIdx.x + info.x;
+    float m = -INFINITY;
+    bool nan = false;
+    for (int i = tid; i < n; i += PA_THREADS) {
+        const float x = __ldcg(p.part_ml + (slot0 + i) * p.ru + r).x;
+        m = fmaxf(m, x);
+        nan |= x != x;
+    }
+    m = block_max(m, red);
+    if (__syncthreads_or(nan)) m = NAN;
+    float l = 0.f;
+    for (int i = tid; i < n; i += PA_THREADS) {
+        const float2 ml = __ldcg(p.part_ml + (slot0 + i) * p.ru + r);
+        const float f = exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+        factor[i] = f;
+        l += ml.y * f;
+    }
+    l = block_sum(l, red);  // (its barriers: factor is complete)
+    constexpr int PER = 128 / HD;  // parts a warp reads side by side: a part's row is HD / 4 lanes
+    const int c4 = lane % (HD / 4), side = lane / (HD / 4);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = warp * PER + side; i < n; i += PA_WARPS * PER) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((slot0 + i) * p.ru + r) * HD) + c4);
+        const float f = factor[i];
+        a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
+    }
+    if (PER == 2) {
+        a.x += __shfl_xor_sync(0xffffffffu, a.x, 16); a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
+        a.z += __shfl_xor_sync(0xffffffffu, a.z, 16); a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
+    }
+    if (side == 0) acc[warp][c4] = a;
+    __syncthreads();
+    for (int col = tid; col < HD; col += PA_THREADS) {
+        float o = 0.f;
+        for (int i = 0; i < PA_WARPS; ++i) o += reinterpret_cast<const float*>(acc[i])[col];
+        store_out<QT>(p, row_head, HD, col, o, l);
+    }
+    if (tid == 0) store_lse(p, row_head, m, l);
+}
+
+// weight[entry] += sum over the kv head's rows of 2^(score - lse): one thread per entry, rows in order
+constexpr int PA_COLLECT = 512;
+__global__ void __launch_bounds__(PA_THREADS) attn_collect_kernel(const __grid_constant__ AttnArgs p) {
+    const int b = blockIdx.z, kvh = blockIdx.y;
+    const SeqWork w = seq_work(p, b);
+    const int first = blockIdx.x * PA_COLLECT, end = min(w.s.len, first + PA_COLLECT);
+    pdl_wait();
+    if (w.s.n == 0 || end <= max(first, w.start)) return;
+    float sum[PA_COLLECT / PA_THREADS];
+#pragma unroll
+    for (int i = 0; i < PA_COLLECT / PA_THREADS; ++i) sum[i] = 0.f;
+    for (int j = 0; j < w.s.n; ++j)
+        for (int g = 0; g < p.group; ++g) {
+            const size_t row_head = (size_t)(w.s.r0 + j) * p.heads + kvh * p.group + g;
+            const float lse2 = __ldcg(p.lse2 + row_head);
+            if (lse2 == -INFINITY) continue;
+            const float* s = p.scores + row_head * p.score_stride;
+#pragma unroll
+            for (int i = 0; i < PA_COLLECT / PA_THREADS; ++i) {
+                const int t = first + i * PA_THREADS + threadIdx.x;
+                if (t >= w.start && t < end) sum[i] += exp2f(__ldcg(s + t) - lse2);
+            }
+        }
+    float* weight = p.c.weight + ((size_t)b * p.c.kv_heads + kvh) * p.c.cap;
+#pragma unroll
+    for (int i = 0; i < PA_COLLECT / PA_THREADS; ++i) {
+        const int t = first + i * PA_THREADS + threadIdx.x;
+        if (t >= w.start && t < end) weight[t] += sum[i];
+    }
+}
+
+}  // namespace cd

@@ -1,0 +1,479 @@
+// cd_verify_drafts: which drafted tokens of a batch stay, and the token drawn behind them.
+//
+// verify_rows_kernel reads every logit row once: a CTA leaves (max, sum of exp, arg-max) of a chunk of a row.  It is bound by those
+// bytes.  verify_pick_kernel, a cluster of CTAs per sequence, puts the chunks together, tests the drafts, and draws from the one row (pair
+// of rows) it ended at, which it reads again.
+//
+// What is decided there are comparisons with given random numbers, so sums must not blur them: the test u q(x) < p(x) takes p(x) and q(x)
+// in 64 bits over row sums of fp32 terms added in 64 bits (off by a few 2^-24 divided by the number of terms that count), and the
+// draw, where every one of `vocab` running sums is a border, is in 64 bits throughout, its row sums included.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "serve.cuh"
+
+namespace cg = cooperative_groups;
+using namespace cd;
+
+namespace {
+const char* CALL = "cd_verify_drafts";
+constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32, VD_CHUNKS = 32, VD_CLUSTER = 8, VD_TILE = 256, VD_VOCAB = 1 << 22;
+
+struct Part {
+    float m;   // NaN: the chunk holds NaN
+    int at;    // lowest place of m
+    double s;  // sum of exp((x - m) / temperature)
+};
+struct VerifyArgs {
+    const void *target, *draft;
+    long long target_stride, draft_stride;
+    const int *tokens, *row_start;
+    const float *uniforms, *draws;
+    int *accepted, *out, *status;
+    Part* parts;  // [2 nrows][VD_CHUNKS]: target rows, then draft rows
+    double inv_t;
+    int nseq, nrows, max_rows, vocab, chunks, chunk;  // chunk: elements, a multiple of 8
+};
+
+template <typename T> __device__ inline float wide(T v);
+template <> __device__ inline float wide<float>(float v) { return v; }
+template <> __device__ inline float wide<__half>(__half v) { return __half2float(v); }
+template <> __device__ inline float wide<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+__device__ inline uint4 load_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// (m, at, s) of one chunk.  GREEDY: no sums.
+template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_constant__ VerifyArgs p) {
+    constexpr int VEC = 16 / sizeof(T), DEEP = 4;
+    __shared__ float red_m[VD_WARPS];
+    __shared__ int red_at[VD_WARPS];
+    __shared__ double red_s[VD_WARPS];
+    const int row = blockIdx.x / p.chunks, ch = blockIdx.x % p.chunks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool is_draft = row >= p.nrows;
+    const int r = is_draft ? row - p.nrows : row;
+    // rows behind the last sequence, and draft rows with no draft behind them, are not looked at
+    bool skip = tid == 0 && r >= p.row_start[p.nseq];
+    if (is_draft)
+        for (int b = tid; b < p.nseq; b += VD_THREADS) skip |= p.row_start[b + 1] - 1 == r;
+    if (__syncthreads_or(skip)) return;
+    const T* x = is_draft ? static_cast<const T*>(p.draft) + r * p.draft_stride : static_cast<const T*>(p.target) + r * p.target_stride;
+    const int head = (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T);  // elements before the first 16-byte boundary
+    const int e0 = ch == 0 ? 0 : min(p.vocab, head + ch * p.chunk), e1 = ch == p.chunks - 1 ? p.vocab : min(p.vocab, head + (ch + 1) * p.chunk);
+    const float scale = (float)(p.inv_t * 1.4426950408889634074);
+    float m = -INFINITY, s = 0.f;
+    int at = 0x7fffffff;
+    bool nan = false;
+    auto take = [&](const float (&v)[VEC], int place) {
+        float top = v[0];
+        int where = 0;
+#pragma unroll
+        for (int e = 1; e < VEC; ++e)
+            if (v[e] > top) { top = v[e]; where = e; }
+        if (GREEDY) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) nan |= v[e] != v[e];
+            if (top > m) { m = top; at = place + where; }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) top = fmaxf(top, v[e]);
+            if (top > m) {
+                s *= exp2f((m - top) * scale);
+                m = top;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += exp2f((v[e] - base) * scale);
+        }
+    };
+    auto one = [&](int i) {  // a ragged end: the element in the first place, nothing in the others
+        float v[VEC];
+        v[0] = wide(x[i]);
+#pragma unroll
+        for (int e = 1; e < VEC; ++e) v[e] = -INFINITY;
+        take(v, i);
+    };
+    const int v0 = min(e1, max(e0, head)), vecs = (e1 - v0) / VEC;
+    for (int i = e0 + tid; i < v0; i += VD_THREADS) one(i);
+    const uint4* body = reinterpret_cast<const uint4*>(x + v0);
+    for (int i = tid; i < vecs; i += VD_THREADS * DEEP) {
+        uint4 w[DEEP];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (i + d * VD_THREADS < vecs) w[d] = load_once(body + i + d * VD_THREADS);
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (i + d * VD_THREADS < vecs) {
+                float v[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = wide(reinterpret_cast<const T*>(&w[d])[e]);
+                take(v, v0 + (i + d * VD_THREADS) * VEC);
+            }
+    }
+    for (int i = v0 + vecs * VEC + tid; i < e1; i += VD_THREADS) one(i);
+
+    if (GREEDY) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m, o);
+            const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+            if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+        }
+        if (lane == 0) { red_m[warp] = m; red_at[warp] = at; }
+        nan = __syncthreads_or(nan);
+        if (tid == 0) {
+            for (int i = 1; i < VD_WARPS; ++i)
+                if (red_m[i] > m || (red_m[i] == m && red_at[i] < at)) { m = red_m[i]; at = red_at[i]; }
+            p.parts[(size_t)row * VD_CHUNKS + ch] = Part{nan ? NAN : m, at, 0.0};
+        }
+    } else {
+        const float top = warp_max(m);
+        double sum = (double)s * (double)exp2f((m - (top == -INFINITY ? 0.f : top)) * scale);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) { red_m[warp] = top; red_s[warp] = sum; }
+        __syncthreads();
+        if (tid == 0) {
+            float all = red_m[0];
+            for (int i = 1; i < VD_WARPS; ++i) all = fmaxf(all, red_m[i]);
+            sum = 0.0;
+            for (int i = 0; i < VD_WARPS; ++i) sum += red_s[i] * (double)exp2f((red_m[i] - (all == -INFINITY ? 0.f : all)) * scale);
+            p.parts[(size_t)row * VD_CHUNKS + ch] = Part{all, 0, sum};
+        }
+    }
+}
+
+__device__ inline double warp_sum_d(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+struct RowStat {
+    float m;
+    int at;
+    double z;
+    __device__ bool good() const { return isfinite(m) && isfinite(z); }
+};
+// a row's chunks together (all lanes of a warp)
+template <bool GREEDY> __device__ inline RowStat row_stat(const VerifyArgs& p, int row) {
+    const int lane = threadIdx.x & 31;
+    Part q{-INFINITY, 0x7fffffff, 0.0};
+    if (lane < p.chunks) {
+        const Part* src = p.parts + (size_t)row * VD_CHUNKS + lane;
+        q.m = __ldcg(&src->m);
+        q.at = __ldcg(&src->at);
+        q.s = __ldcg(&src->s);
+    }
+    RowStat r;
+    if (GREEDY) {
+        const bool nan = __any_sync(0xffffffffu, q.m != q.m);
+        float m = q.m;
+        int at = q.at;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m, o);
+            const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+            if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+        }
+        r.m = nan ? NAN : m;
+        r.at = at;
+        r.z = 1.0;
+    } else {
+        r.m = warp_max(q.m);
+        r.at = 0;
+        r.z = warp_sum_d(isfinite(r.m) ? q.s * exp(((double)q.m - (double)r.m) * p.inv_t) : NAN);
+    }
+    return r;
+}
+
+struct PickShared {
+    int first_bad, valid, at;
+    double total[3];  // of this CTA: p's sum, q's sum, what is drawn from
+    double red[2][VD_WARPS];
+    float pm, qm;
+};
+
+template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_constant__ VerifyArgs p) {
+    extern __shared__ double tiles[];  // sums of this CTA's tiles
+    __shared__ PickShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / size;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r0 = p.row_start[b], r1 = p.row_start[b + 1], n = r1 - r0;
+    pdl_wait();
+    if (r0 < 0 || n < 0 || r1 > p.nrows || n > p.max_rows || n == 0) {
+        if (rank == 0 && tid == 0) {
+            p.accepted[b] = 0;
+            if (n != 0) report(p.status, CD_STATUS_BATCH);
+        }
+        return;
+    }
+    if (tid == 0) {
+        sh.first_bad = n - 1;
+        sh.valid = 1;
+    }
+    __syncthreads();
+    const T *target = static_cast<const T*>(p.target), *draft = static_cast<const T*>(p.draft);
+    for (int j = warp; j < n - 1; j += VD_WARPS) {
+        const int x = p.tokens[r0 + j + 1];
+        const RowStat t = row_stat<GREEDY>(p, r0 + j);
+        bool stays = t.good() && (unsigned)x < (unsigned)p.vocab;
+        if (GREEDY) stays = stays && t.at == x;
+        else if (stays) {
+            const double px = exp(((double)wide(target[(r0 + j) * p.target_stride + x]) - (double)t.m) * p.inv_t) / t.z;
+            double qx = 1.0;
+            if (draft) {
+                const RowStat q = row_stat<GREEDY>(p, p.nrows + r0 + j);
+                qx = q.good() ? exp(((double)wide(draft[(r0 + j) * p.draft_stride + x]) - (double)q.m) * p.inv_t) / q.z : NAN;
+            }
+            stays = (double)p.uniforms[r0 + j] * qx < px;
+        }
+        if (!stays && lane == 0) atomicMin(&sh.first_bad, j);
+    }
+    __syncthreads();
+    const int end = sh.first_bad, row = r0 + end;
+    const bool left = end < n - 1;  // a draft was turned down: draw from what p has over q
+    if (warp == 0) {
+        const RowStat t = row_stat<GREEDY>(p, row);
+        bool good = t.good();
+        if (lane == 0) {
+            sh.pm = t.m;
+            sh.at = t.at;
+        }
+        if (!GREEDY && left && draft) {
+            const RowStat q = row_stat<GREEDY>(p, p.nrows + row);
+            good = good && q.good();
+            if (lane == 0) sh.qm = q.m;
+        }
+        if (lane == 0 && !good) sh.valid = 0;
+    }
+    __syncthreads();
+    if (rank == 0) {
+        for (int j = tid; j < n; j += VD_THREADS)
+            if (j != end) p.out[r0 + j] = j < end ? p.tokens[r0 + j + 1] : -1;
+        if (tid == 0) p.accepted[b] = end;
+    }
+    if (!sh.valid || GREEDY) {  // the same in every CTA of the cluster
+        if (rank == 0 && tid == 0) {
+            p.out[row] = sh.valid ? sh.at : -1;
+            if (!sh.valid) report(p.status, CD_STATUS_LOGITS);
+        }
+        return;
+    }
+    const T *pt = target + row * p.target_stride, *pd = left && draft ? draft + row * p.draft_stride : nullptr;
+    const int gone = left && !draft ? p.tokens[row + 1] : -1;
+    const double pm = sh.pm, qm = sh.qm;
+    const int all_tiles = (p.vocab + VD_TILE - 1) / VD_TILE, per = (all_tiles + size - 1) / size;
+    const int t0 = min(all_tiles, rank * per), t1 = min(all_tiles, t0 + per);
+    double ip = 1.0, iq = 0.0;
+    if (pd) {
+        double sp = 0.0, sq = 0.0;
+        for (int t = t0 + warp; t < t1; t += VD_WARPS)
+#pragma unroll
+            for (int e = 0; e < VD_TILE / 32; ++e) {
+                const int i = t * VD_TILE + e * 32 + lane;
+                if (i < p.vocab) {
+                    sp += exp(((double)wide(pt[i]) - pm) * p.inv_t);
+                    sq += exp(((double)wide(pd[i]) - qm) * p.inv_t);
+                }
+            }
+        sp = warp_sum_d(sp);
+        sq = warp_sum_d(sq);
+        if (lane == 0) { sh.red[0][warp] = sp; sh.red[1][warp] = sq; }
+        __syncthreads();
+        if (tid < 2) {
+            double v = 0.0;
+            for (int i = 0; i < VD_WARPS; ++i) v += sh.red[tid][i];
+            sh.total[tid] = v;
+        }
+        cluster.sync();
+        sp = sq = 0.0;
+        for (int r = 0; r < size; ++r) {
+            const double* o = cluster.map_shared_rank(sh.total, r);
+            sp += o[0];
+            sq += o[1];
+        }
+        ip = 1.0 / sp;
+        iq = 1.0 / sq;
+    }
+    auto share = [&](int i, bool rest) -> double {  // of token i in what is drawn from
+        if (i >= p.vocab || (rest && i == gone)) return 0.0;
+        const double v = exp(((double)wide(pt[i]) - pm) * p.inv_t);
+        if (!rest || !pd) return v;
+        return fmax(v * ip - exp(((double)wide(pd[i]) - qm) * p.inv_t) * iq, 0.0);
+    };
+    double whole = 0.0, before = 0.0, mine = 0.0;
+    bool rest = left;
+    for (int turn = 0; turn < 2; ++turn) {  // again from p alone where rounding leaves nothing of p - q
+        for (int t = t0 + warp; t < t1; t += VD_WARPS) {
+            double v = 0.0;
+#pragma unroll
+            for (int e = 0; e < VD_TILE / 32; ++e) v += share(t * VD_TILE + e * 32 + lane, rest);
+            v = warp_sum_d(v);
+            if (lane == 0) tiles[t - t0] = v;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            double v = 0.0;
+            for (int t = lane; t < t1 - t0; t += 32) v += tiles[t];
+            v = warp_sum_d(v);
+            if (lane == 0) sh.total[2] = v;
+        }
+        cluster.sync();
+        whole = before = 0.0;
+        for (int r = 0; r < size; ++r) {
+            const double v = *cluster.map_shared_rank(&sh.total[2], r);
+            if (r < rank) before += v;
+            if (r == rank) mine = v;
+            whole += v;
+        }
+        cluster.sync();
+        if (whole > 0.0 || !rest) break;
+        rest = false;
+    }
+    // the first token whose running sum exceeds u * whole: the CTA, then the tile, then the token.  Sums of sums round, so where none
+    // does the last one that has a share is it.
+    const double goal = (double)p.draws[b] * whole;
+    double run = 0.0;
+    int owner = -1;
+    for (int r = 0; r < size; ++r) {
+        const double v = *cluster.map_shared_rank(&sh.total[2], r);
+        if (v > 0.0) owner = r;
+        run += v;
+        if (run > goal) break;
+    }
+    cluster.sync();  // nobody reads this CTA's shared memory any more
+    if (owner != rank || warp != 0) return;
+    (void)mine;
+    int tile = 0;
+    run = before;
+    {
+        double acc = before;
+        int last = 0;
+        double last_before = before;
+        for (int t = 0; t < t1 - t0; ++t) {
+            const double v = tiles[t];
+            if (v > 0.0) { last = t; last_before = acc; }
+            acc += v;
+            if (acc > goal && v > 0.0) break;
+        }
+        tile = last;
+        run = last_before;
+    }
+    int found = -1, fallback = 0;
+    for (int e = 0; e < VD_TILE / 32 && found < 0; ++e) {
+        const int i = (t0 + tile) * VD_TILE + e * 32 + lane;
+        const double v = share(i, rest);
+        double incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        const uint32_t some = __ballot_sync(0xffffffffu, v > 0.0), over = __ballot_sync(0xffffffffu, v > 0.0 && run + incl > goal);
+        if (some) fallback = i - lane + 31 - __clz(some);
+        if (over) found = i - lane + __ffs(over) - 1;
+        run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) p.out[row] = found >= 0 ? found : fallback;
+}
+
+template <typename T, bool GREEDY> cudaError_t launch(const VerifyArgs& a, bool draft, cudaStream_t s) {
+    verify_rows_kernel<T, GREEDY><<<(unsigned)(a.nrows * (draft ? 2 : 1)) * a.chunks, VD_THREADS, 0, s>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const int size = GREEDY ? 1 : VD_CLUSTER, tiles = (a.vocab + VD_TILE - 1) / VD_TILE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.nseq * size);
+    cfg.blockDim = dim3(VD_THREADS);
+    cfg.dynamicSmemBytes = GREEDY ? 0 : (size_t)((tiles + size - 1) / size) * 8;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = size;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, verify_pick_kernel<T, GREEDY>, a);
+}
+template <typename T> cudaError_t launch_mode(const VerifyArgs& a, bool greedy, bool draft, cudaStream_t s) {
+    return greedy ? launch<T, true>(a, false, s) : launch<T, false>(a, draft, s);
+}
+int check(int nrows, int nseq, int vocab) {
+    if (nseq < 0 || nseq > 65535) return refuse(CD_ERR_INVALID, CALL, "nseq must be in 0..65535");
+    if (nrows < 0 || nrows > 1 << 20) return refuse(CD_ERR_INVALID, CALL, "nrows must be in 0..1048576");
+    if (vocab < 1) return refuse(CD_ERR_INVALID, CALL, "vocab must be positive");
+    if (vocab > VD_VOCAB) return refuse(CD_ERR_UNSUPPORTED, CALL, "at most 4194304 tokens");
+    return CD_OK;
+}
+size_t workspace_of(int nrows) { return (size_t)nrows * 2 * VD_CHUNKS * sizeof(Part) + 256; }
+}  // namespace
+
+extern "C" int cd_verify_drafts_workspace(int nrows, int nseq, int vocab, size_t* bytes) {
+    if (!bytes) return refuse(CD_ERR_INVALID, CALL, "null argument");
+    if (int rc = check(nrows, nseq, vocab)) return rc;
+    *bytes = workspace_of(nrows);
+    return CD_OK;
+}
+
+extern "C" int cd_verify_drafts(int device, int dtype, int nseq, int nrows, int max_rows, int vocab, const void* target, int64_t target_stride,
+                                const void* draft, int64_t draft_stride, const int32_t* tokens, const int32_t* row_start, const float* uniforms,
+                                const float* draws, double temperature, int32_t* accepted, int32_t* out_tokens, int32_t* status, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+    if (int rc = check(nrows, nseq, vocab)) return rc;
+    if (dtype < CD_DTYPE_F32 || dtype > CD_DTYPE_BF16) return refuse(CD_ERR_INVALID, CALL, "logits are f32, f16 or bf16");
+    if (max_rows < 1) return refuse(CD_ERR_INVALID, CALL, "max_rows must be positive");
+    if (!(temperature == 0.0 || (temperature >= 1e-6 && temperature <= 1e6))) return refuse(CD_ERR_INVALID, CALL, "temperature must be 0 or in 1e-6..1e6");
+    if (nseq == 0) return CD_OK;
+    if (!row_start || !accepted || !workspace) return refuse(CD_ERR_INVALID, CALL, "null argument");
+    if (nrows > 0 && (!target || !tokens || !out_tokens)) return refuse(CD_ERR_INVALID, CALL, "null argument");
+    const bool greedy = temperature == 0.0;
+    if (nrows > 0 && !greedy && (!uniforms || !draws)) return refuse(CD_ERR_INVALID, CALL, "uniforms and draws are needed above temperature 0");
+    if (target_stride == 0) target_stride = vocab;
+    if (draft_stride == 0) draft_stride = vocab;
+    if (target_stride < vocab || draft_stride < vocab) return refuse(CD_ERR_INVALID, CALL, "a row stride is shorter than a row");
+    if (!aligned(target, dtype_size(dtype)) || !aligned(draft, dtype_size(dtype))) return refuse(CD_ERR_INVALID, CALL, "logits are not aligned to their type");
+    if (!aligned(tokens, 4) || !aligned(row_start, 4) || !aligned(uniforms, 4) || !aligned(draws, 4) || !aligned(accepted, 4) || !aligned(out_tokens, 4) ||
+        !aligned(status, 4) || !aligned(workspace, 256))
+        return refuse(CD_ERR_INVALID, CALL, "int32 and fp32 arrays start on 4-byte boundaries, the workspace on a 256-byte one");
+    if (workspace_bytes < workspace_of(nrows)) return refuse(CD_ERR_CAPACITY, CALL, "the workspace is smaller than cd_verify_drafts_workspace says");
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return cuda_status(guard.err, CALL);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (nrows == 0) return cuda_status(cudaMemsetAsync(accepted, 0, (size_t)nseq * 4, s), CALL);
+    VerifyArgs a;
+    a.target = target;
+    a.draft = greedy ? nullptr : draft;
+    a.target_stride = target_stride;
+    a.draft_stride = draft_stride;
+    a.tokens = tokens;
+    a.row_start = row_start;
+    a.uniforms = uniforms;
+    a.draws = draws;
+    a.accepted = accepted;
+    a.out = out_tokens;
+    a.status = status;
+    a.parts = static_cast<Part*>(workspace);
+    a.inv_t = greedy ? 1.0 : 1.0 / temperature;
+    a.nseq = nseq;
+    a.nrows = nrows;
+    a.max_rows = max_rows;
+    a.vocab = vocab;
+    // chunks of a row: enough CTAs for the GPU (148 SMs, eight each), none below 2048 elements
+    const long long rows = (long long)nrows * (a.draft ? 2 : 1), want = std::max<long long>(1, (148 * 8 + rows - 1) / rows);
+    a.chunks = (int)std::max<long long>(1, std::min<long long>({want, (vocab + 2047) / 2048, VD_CHUNKS}));
+    a.chunk = ((vocab + a.chunks - 1) / a.chunks + 7) & ~7;
+    cudaError_t e;
+    if (dtype == CD_DTYPE_F32) e = launch_mode<float>(a, greedy, a.draft != nullptr, s);
+    else if (dtype == CD_DTYPE_F16) e = launch_mode<__half>(a, greedy, a.draft != nullptr, s);
+    else e = launch_mode<__nv_bfloat16>(a, greedy, a.draft != nullptr, s);
+    return cuda_status(e, CALL);
+}
