@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged_attn.cuh"
+#include "paged_mma.cuh"
 
 using namespace cd;
 
@@ -16,11 +16,11 @@ struct Plan {
 };
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// A warp of the FMA kernel has 4 rows; a unit as many of its warps as its rows need.
+// A warp has 4 rows of a unit with an fp32 pool (FMAs), 16 with a 16-bit one (tensor cores); a unit as many of its warps as its rows need.
 Plan plan_of(const cd_paged_cache* c, int heads, int nrows, int max_rows, int collect) {
     Plan p;
     p.group = heads / c->kv_heads;
-    const int per_warp = 4;
+    const int per_warp = c->dtype == CD_DTYPE_F32 ? 4 : 16;
     const long long rows = (long long)max_rows * p.group;
     p.row_warps = rows <= per_warp ? 1 : rows <= 2 * per_warp ? 2 : 4;
     p.ru = per_warp * p.row_warps;
@@ -53,8 +53,13 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
-    const int ctas = std::min(2 * sms, PA_MAX_CTAS);
-    attn_fma_kernel<KT, QT, HD><<<ctas, PA_THREADS, (size_t)(a.c.nseq + 1) * 8, s>>>(a);
+    if constexpr (std::is_same<KT, float>::value) {
+        attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 8, s>>>(a);
+    } else {
+        const size_t shared = mma_shared<KT, QT, HD>(a.c.nseq, a.row_warps);
+        if (shared > 48 * 1024 && (e = allow_shared_memory((const void*)attn_mma_kernel<KT, QT, HD>)) != cudaSuccess) return e;
+        attn_mma_kernel<KT, QT, HD><<<std::min(mma_ctas<HD>() * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
+    }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const dim3 grid((unsigned)plan.units, (unsigned)std::min<long long>(a.ru, (long long)a.max_rows * a.group));
     if ((e = launch_dependent(attn_join_kernel<QT, HD>, grid, dim3(PA_THREADS), 0, s, a)) != cudaSuccess) return e;
