@@ -68,29 +68,36 @@ def _code(t, what):
     return code
 
 
-def _tensor(t, what, dtype, shape, device):
-    """A packed tensor of the given type on the cache's device; None in `shape`: any size."""
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError("%s must be a contiguous %s tensor on %s" % (what, str(dtype).replace("torch.", ""), device))
-    if len(t.shape) != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+def _tensor(t, what, dtype, shape, index):
+    """The address of a packed tensor of the given type and shape on CUDA device `index`."""
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous %s tensor on cuda:%d" % (what, str(dtype).replace("torch.", ""), index))
+    if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (what, list(shape), list(t.shape)))
     return t.data_ptr()
 
 
-def _row_stride(t, what, rows, hd, device):
+def _row_stride(t, what, rows, hd, index):
     """[rows][heads][hd] with packed heads; the distance of its rows."""
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != hd:
-        raise ValueError("%s must have shape [%d, heads, %d], got %s" % (what, rows, hd, list(t.shape)))
-    if t.device != device:
-        raise ValueError("%s must be on %s" % (what, device))
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != hd:
+        raise ValueError("%s must have shape [%d, heads, %d], got %s" % (what, rows, hd, list(shape)))
+    if t.get_device() != index:
+        raise ValueError("%s must be on cuda:%d" % (what, index))
     row, head, one = t.stride()
-    if one != 1 or (head != hd and t.shape[1] != 1):
+    if one != 1 or (head != hd and shape[1] != 1):
         raise ValueError("%s: the heads of a row must lie next to each other" % what)
     return row if rows > 1 else 0
 
 
-def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+_STREAM = []  # torch's call for a device's current stream as an address
+
+
+def _stream(index):
+    if not _STREAM:
+        torch = _torch()
+        _STREAM.append(getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream))
+    return _STREAM[0](index)
 
 
 def _check(rc):
@@ -110,7 +117,7 @@ class PagedCache:
             raise ValueError("the pool must be a CUDA tensor")
         if pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
             raise ValueError("the pool must be contiguous, [npages, 2, kv_heads, page_tokens, hd]")
-        self.device = pool.device
+        self.device, self._index = pool.device, pool.device.index
         if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != self.device or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be int32 [nseq, max_pages] on the pool's device, its rows packed")
         npages, _, kv_heads, page_tokens, hd = pool.shape
@@ -123,8 +130,8 @@ class PagedCache:
         c.pool, c.page_table = pool.data_ptr(), page_table.data_ptr()
         c.table_stride = page_table.stride(0) if nseq > 1 else max_pages
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device) if status is None else status
-        c.status = _tensor(self.status, "status", torch.int32, (1,), self.device)
-        self._ref, self._workspaces = C.byref(c), {}
+        c.status = _tensor(self.status, "status", torch.int32, (1,), self._index)
+        self._ref, self._workspaces, self._starts = C.byref(c), {}, (nseq + 1,)
         self.lens = self.weight = self.position = None
         self.replace(lens, weight, position)
 
@@ -132,14 +139,14 @@ class PagedCache:
         """Take other tensors for the lengths or the bookkeeping, as cache_evict returned them."""
         torch = _torch()
         if lens is not None:
-            self._c.lens = _tensor(lens, "lens", torch.int32, (self.nseq,), self.device)
+            self._c.lens = _tensor(lens, "lens", torch.int32, (self.nseq,), self._index)
             self.lens = lens
         shape = (self.nseq, self.kv_heads, self.capacity)
         if weight is not None:
-            self._c.weight = _tensor(weight, "weight", torch.float32, shape, self.device)
+            self._c.weight = _tensor(weight, "weight", torch.float32, shape, self._index)
             self.weight = weight
         if position is not None:
-            self._c.position = _tensor(position, "position", torch.int32, shape, self.device)
+            self._c.position = _tensor(position, "position", torch.int32, shape, self._index)
             self.position = position
 
     def _workspace(self, given, size, *key):
@@ -193,20 +200,20 @@ def rope_append(cache, rope, q, k, v, positions, row_start, out=None):
     """Rotate q [rows, heads, hd] and k [rows, kv_heads, hd] at `positions` [rows] int32, write k and v to their entries in the cache (with
     bookkeeping: weight 0, the position noted), return the rotated q.  q, k and v are f32 or of the pool's type; they may be
     slices of one fused projection.  out: a packed tensor for the result; q itself where q is packed."""
-    torch, device, hd = _torch(), cache.device, cache.hd
-    rows = q.shape[0]
-    sq, sk, sv = _row_stride(q, "q", rows, hd, device), _row_stride(k, "k", rows, hd, device), _row_stride(v, "v", rows, hd, device)
+    torch, index, hd = _torch(), cache._index, cache.hd
+    rows, dtype = q.shape[0], q.dtype
+    sq, sk, sv = _row_stride(q, "q", rows, hd, index), _row_stride(k, "k", rows, hd, index), _row_stride(v, "v", rows, hd, index)
     if k.shape[1] != cache.kv_heads or v.shape[1] != cache.kv_heads:
         raise ValueError("k and v must have the cache's %d heads" % cache.kv_heads)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("q, k and v must have one type")
-    if rope.turns.device != device:
-        raise ValueError("rope must be on %s" % device)
+    if rope.turns.get_device() != index:
+        raise ValueError("rope must be on cuda:%d" % index)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty(q.shape, dtype=dtype, device=cache.device)
     _check(lib.cd_rope_append(cache._ref, rope._ref, _code(q, "q"), q.shape[1], rows, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv,
-                              _tensor(positions, "positions", torch.int32, (rows,), device), _tensor(row_start, "row_start", torch.int32, (cache.nseq + 1,), device),
-                              _tensor(out, "out", q.dtype, q.shape, device), _stream(device)))
+                              _tensor(positions, "positions", torch.int32, (rows,), index), _tensor(row_start, "row_start", torch.int32, cache._starts, index),
+                              _tensor(out, "out", dtype, q.shape, index), _stream(index)))
     return out
 
 
@@ -214,17 +221,17 @@ def paged_attention(cache, q, row_start, max_rows, scale=None, window=0, collect
     """Attention of the new rows q [rows, heads, hd] (f32 or of the pool's type) over the cache, each row up to its own entry, or over its last
     `window` entries.  max_rows: the most rows a sequence has.  collect: add the probabilities to cache.weight.  Returns out, or
     (out, lse [rows, heads] f32) with lse.  Rows from row_start[nseq] on are not written."""
-    torch, device = _torch(), cache.device
-    rows, heads = q.shape[0], q.shape[1]
-    stride = _row_stride(q, "q", rows, cache.hd, device)
+    torch, index = _torch(), cache._index
+    shape = q.shape
+    rows, heads, collect = shape[0], shape[1], 1 if collect else 0
+    stride = _row_stride(q, "q", rows, cache.hd, index)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    norm = torch.empty((rows, heads), dtype=torch.float32, device=device) if lse else None
-    ws = cache._workspace(workspace, lib.cd_paged_attention_workspace, heads, rows, max_rows, int(collect))
+        out = torch.empty(shape, dtype=q.dtype, device=cache.device)
+    norm = torch.empty((rows, heads), dtype=torch.float32, device=cache.device) if lse else None
+    ws = cache._workspace(workspace, lib.cd_paged_attention_workspace, heads, rows, max_rows, collect)
     _check(lib.cd_paged_attention(cache._ref, _code(q, "q"), heads, rows, max_rows, q.data_ptr(), stride,
-                                  _tensor(row_start, "row_start", torch.int32, (cache.nseq + 1,), device), 0.0 if scale is None else scale, window,
-                                  int(collect), _tensor(out, "out", q.dtype, q.shape, device), norm.data_ptr() if lse else None, ws.data_ptr(), ws.numel(),
-                                  _stream(device)))
+                                  _tensor(row_start, "row_start", torch.int32, cache._starts, index), 0.0 if scale is None else scale, window, collect,
+                                  _tensor(out, "out", q.dtype, shape, index), norm.data_ptr() if lse else None, ws.data_ptr(), ws.numel(), _stream(index)))
     return (out, norm) if lse else out
 
 
@@ -232,15 +239,15 @@ def cache_evict(cache, keep, sinks=0, recent=0, out=None, workspace=None):
     """Bring every sequence with more than `keep` entries down to `keep`, each kv head by its own weights; positions below `sinks` and the
     newest `recent` ones stay.  K and V move within the cache's pages.  Returns new (lens, weight, position), which the caller
     hands to cache.replace(); out: tensors for them (weight and position may be the cache's own, lens may not)."""
-    torch, device = _torch(), cache.device
+    torch, index = _torch(), cache._index
     if cache.weight is None:
         raise ValueError("the cache has no weight and position")
     lens, weight, position = out if out is not None else (torch.empty_like(cache.lens), torch.empty_like(cache.weight), torch.empty_like(cache.position))
     ws = cache._workspace(workspace, lib.cd_cache_evict_workspace, keep)
-    shape = (cache.nseq, cache.kv_heads, cache.capacity)
-    _check(lib.cd_cache_evict(cache._ref, keep, sinks, recent, _tensor(lens, "lens", torch.int32, (cache.nseq,), device),
-                              _tensor(weight, "weight", torch.float32, shape, device), _tensor(position, "position", torch.int32, shape, device),
-                              ws.data_ptr(), ws.numel(), _stream(device)))
+    shape = cache.weight.shape
+    _check(lib.cd_cache_evict(cache._ref, keep, sinks, recent, _tensor(lens, "lens", torch.int32, cache.lens.shape, index),
+                              _tensor(weight, "weight", torch.float32, shape, index), _tensor(position, "position", torch.int32, shape, index),
+                              ws.data_ptr(), ws.numel(), _stream(index)))
     return lens, weight, position
 
 
@@ -249,32 +256,32 @@ def verify_drafts(target, tokens, row_start, max_rows, uniforms, draws, draft=No
     of each sequence, then its drafts; uniforms [rows] and draws [nseq] f32 in [0, 1) (not used at temperature 0, and None is fine there);
     draft [rows, vocab]: the logits the token behind each row was drawn from, None: drafts without a distribution.  Returns
     (accepted [nseq] int32, out_tokens [rows] int32: the drafts that stay, the drawn token, then -1)."""
-    torch, device = _torch(), target.device
-    if not target.is_cuda or target.dim() != 2 or (target.shape[1] > 1 and target.stride(1) != 1):
+    torch, device, shape = _torch(), target.device, target.shape
+    index = device.index
+    if not target.is_cuda or len(shape) != 2 or (shape[1] > 1 and target.stride(1) != 1):
         raise ValueError("target must be a CUDA tensor [rows, vocab] with packed rows")
-    if draft is not None and (draft.shape != target.shape or draft.dtype != target.dtype or draft.device != device or (draft.shape[1] > 1 and draft.stride(1) != 1)):
+    if draft is not None and (draft.shape != shape or draft.dtype is not target.dtype or draft.get_device() != index or (shape[1] > 1 and draft.stride(1) != 1)):
         raise ValueError("draft must be as target is")
-    rows, vocab = target.shape
+    rows, vocab = shape
     nseq = row_start.shape[0] - 1
-    starts = _tensor(row_start, "row_start", torch.int32, (nseq + 1,), device)
+    starts = _tensor(row_start, "row_start", torch.int32, (nseq + 1,), index)
     accepted, out = torch.empty(nseq, dtype=torch.int32, device=device), torch.empty(rows, dtype=torch.int32, device=device)
-    key = (rows, nseq, vocab)
-    need = _VERIFY.get(key)
+    need = _VERIFY.get((rows, nseq, vocab))
     if need is None:
         n = C.c_size_t()
         _check(lib.cd_verify_drafts_workspace(rows, nseq, vocab, C.byref(n)))
         if len(_VERIFY) > 256:
             _VERIFY.clear()
-        need = _VERIFY[key] = n.value
+        need = _VERIFY[(rows, nseq, vocab)] = n.value
     ws = _workspace(workspace, need, device)
     random = temperature != 0
-    _check(lib.cd_verify_drafts(device.index, _code(target, "target"), nseq, rows, max_rows, vocab, target.data_ptr(), target.stride(0) if rows > 1 else 0,
+    _check(lib.cd_verify_drafts(index, _code(target, "target"), nseq, rows, max_rows, vocab, target.data_ptr(), target.stride(0) if rows > 1 else 0,
                                 None if draft is None else draft.data_ptr(), 0 if draft is None or rows < 2 else draft.stride(0),
-                                _tensor(tokens, "tokens", torch.int32, (rows,), device), starts,
-                                _tensor(uniforms, "uniforms", torch.float32, (rows,), device) if random else None,
-                                _tensor(draws, "draws", torch.float32, (nseq,), device) if random else None, temperature, accepted.data_ptr(),
-                                out.data_ptr(), None if status is None else _tensor(status, "status", torch.int32, (1,), device), ws.data_ptr(), ws.numel(),
-                                _stream(device)))
+                                _tensor(tokens, "tokens", torch.int32, (rows,), index), starts,
+                                _tensor(uniforms, "uniforms", torch.float32, (rows,), index) if random else None,
+                                _tensor(draws, "draws", torch.float32, (nseq,), index) if random else None, temperature, accepted.data_ptr(),
+                                out.data_ptr(), None if status is None else _tensor(status, "status", torch.int32, (1,), index), ws.data_ptr(), ws.numel(),
+                                _stream(index)))
     return accepted, out
 
 
