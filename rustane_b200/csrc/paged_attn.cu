@@ -56,9 +56,10 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     if constexpr (std::is_same<KT, float>::value) {
         attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 8, s>>>(a);
     } else {
-        const size_t shared = mma_shared<KT, QT, HD>(a.c.nseq, a.row_warps);
-        if (shared > 48 * 1024 && (e = allow_shared_memory((const void*)attn_mma_kernel<KT, QT, HD>)) != cudaSuccess) return e;
-        attn_mma_kernel<KT, QT, HD><<<std::min(mma_ctas<HD>() * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
+        void (*kernel)(AttnArgs) = a.row_warps == 1 ? attn_mma_kernel<KT, QT, HD, 1> : a.row_warps == 2 ? attn_mma_kernel<KT, QT, HD, 2> : attn_mma_kernel<KT, QT, HD, 4>;
+        const size_t shared = a.row_warps == 1 ? mma_shared<KT, QT, HD, 1>(a.c.nseq) : a.row_warps == 2 ? mma_shared<KT, QT, HD, 2>(a.c.nseq) : mma_shared<KT, QT, HD, 4>(a.c.nseq);
+        if ((e = allow_shared_memory((const void*)kernel)) != cudaSuccess) return e;
+        kernel<<<std::min(MMA_CTAS * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const dim3 grid((unsigned)plan.units, (unsigned)std::min<long long>(a.ru, (long long)a.max_rows * a.group));
