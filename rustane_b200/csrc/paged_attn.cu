@@ -44,7 +44,8 @@ int check_shape(const cd_paged_cache* c, int heads, int nrows, int max_rows, int
     if (max_rows < 1 || max_rows > 65536) return refuse(CD_ERR_INVALID, CALL, "max_rows must be in 1..65536");
     if (collect && !c->weight) return refuse(CD_ERR_INVALID, CALL, "collect needs the cache's weight");
     const Plan p = plan_of(c, heads, nrows, max_rows, collect);
-    if (p.units > 0x7fffffffu / 2) return refuse(CD_ERR_UNSUPPORTED, CALL, "too many sequences, heads and rows at once");
+    const long long tiles = ((long long)c->max_pages * c->page_tokens + PA_TILE - 1) / PA_TILE;
+    if (p.units > 0x7fffffffull || (long long)p.units * tiles >= 0x7fffffffll - PA_MAX_CTAS) return refuse(CD_ERR_UNSUPPORTED, CALL, "sequences x kv heads x row blocks x (max_pages x page_tokens / 64) must stay below 2^31");
     return CD_OK;
 }
 
@@ -54,7 +55,7 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
     if constexpr (std::is_same<KT, float>::value) {
-        attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 8, s>>>(a);
+        attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);
     } else {
         void (*kernel)(AttnArgs) = a.row_warps == 1 ? attn_mma_kernel<KT, QT, HD, 1> : a.row_warps == 2 ? attn_mma_kernel<KT, QT, HD, 2> : attn_mma_kernel<KT, QT, HD, 4>;
         const size_t shared = a.row_warps == 1 ? mma_shared<KT, QT, HD, 1>(a.c.nseq) : a.row_warps == 2 ? mma_shared<KT, QT, HD, 2>(a.c.nseq) : mma_shared<KT, QT, HD, 4>(a.c.nseq);
@@ -63,7 +64,9 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const dim3 grid((unsigned)plan.units, (unsigned)std::min<long long>(a.ru, (long long)a.max_rows * a.group));
-    if ((e = launch_dependent(attn_join_kernel<QT, HD>, grid, dim3(PA_THREADS), 0, s, a)) != cudaSuccess) return e;
+    // about 2 sms / units parts a unit: 32 units over 296 CTAs join in 5.3 us with 256 threads a row, 48 units of 48 rows in 8 us with 64 (13 with 256)
+    e = plan.units >= 24 ? launch_dependent(attn_join_kernel<QT, HD, 64>, grid, dim3(64), 0, s, a) : launch_dependent(attn_join_kernel<QT, HD, 256>, grid, dim3(256), 0, s, a);
+    if (e != cudaSuccess) return e;
     if (collect)
         e = launch_dependent(attn_collect_kernel, dim3((a.c.cap + PA_COLLECT - 1) / PA_COLLECT, a.c.kv_heads, a.c.nseq), dim3(PA_THREADS), 0, s, a);
     return e;

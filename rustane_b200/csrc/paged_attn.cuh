@@ -2,8 +2,8 @@
 //
 // o = sum_t p_t v_t, p = softmax(scale q k_t) over the entries a row sees.  A unit is (sequence, kv head, block of RU rows): its
 // rows are the q heads of the kv head times the sequence's new rows, so K and V are read once for all of them.  A unit's entries are cut into tiles of 64 and
-// all units' tiles lie on one line, which the CTAs share evenly: CTA i of G = min(grid, T) takes tiles [i T / G, (i + 1) T / G), whatever the lengths
-// are (they are known on the device only; every CTA adds them up for itself).  A unit that one CTA has whole is finished there;
+// all units' tiles lie on one line, which the CTAs share evenly: each of G = min(grid, T) CTAs takes T / G of them or one more, whatever the lengths are
+// (they are known on the device only; every CTA adds them up for itself).  A unit that one CTA has whole is finished there;
 // the others leave (max, sum, sum of p v) per CTA in slot CTA + unit (both only ever grow along the line, so no two meet),
 // and join_kernel puts them together in the line's order.  Inside a CTA four warps share a unit: `row_warps` of them have different rows of
 // the same entries, the rest other entries.  Statistics are fp32 in the log2 domain.
@@ -47,26 +47,27 @@ __device__ inline SeqWork seq_work(const AttnArgs& p, int b) {
     return w;
 }
 
-// pre[b] = tiles of the sequences before b (all threads; ends with a barrier); returns the total
-__device__ inline long long line_up(const AttnArgs& p, long long* pre, long long* sums) {
+// pre[b] = tiles of the sequences before b (all threads; ends with a barrier); returns the total (the host keeps it below 2^31)
+__device__ inline int line_up(const AttnArgs& p, int* pre, int* sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    long long carry = 0;
+    int carry = 0;
     if (tid == 0) pre[0] = 0;
     for (int base = 0; base < p.c.nseq; base += PA_THREADS) {
         const int b = base + tid;
-        long long v = 0;
+        int v = 0;
         if (b < p.c.nseq) {
             const SeqWork w = seq_work(p, b);
-            v = (long long)w.tiles * w.blocks * p.c.kv_heads;
+            v = w.tiles * w.blocks * p.c.kv_heads;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, v, o);
+            const int x = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += x;
         }
         if (lane == 31) sums[warp] = v;
         __syncthreads();
-        long long before = carry;
+        int before = carry;
+#pragma unroll
         for (int i = 0; i < PA_WARPS; ++i) {
             if (i < warp) before += sums[i];
             carry += sums[i];
@@ -133,11 +134,13 @@ __device__ inline void finish_unit(const AttnArgs& p, const UnitParts<HD, PAD>& 
 }
 
 // Walk this CTA's share of the line; work(w, b, kvh, block, first tile, tiles, whole, slot) handles a run of one unit's tiles.
-template <typename F> __device__ inline void walk_line(const AttnArgs& p, long long* pre, long long* sums, F&& work) {
-    const long long total = line_up(p, pre, sums), ctas = min((long long)gridDim.x, total);  // no share is empty
-    if (blockIdx.x >= ctas) return;
-    long long t = total * blockIdx.x / ctas;
-    const long long end = total * (blockIdx.x + 1) / ctas;
+template <typename F> __device__ inline void walk_line(const AttnArgs& p, int* pre, int* sums, F&& work) {
+    const int total = line_up(p, pre, sums), ctas = min((int)gridDim.x, total), me = blockIdx.x;  // no share is empty
+    if (me >= ctas) return;
+    const int per = total / ctas, more = total - per * ctas, cut = more * (per + 1);  // the first `more` shares have one tile more
+    auto owner = [&](int t) { return t < cut ? t / (per + 1) : more + (t - cut) / per; };
+    int t = me * per + min(me, more);
+    const int end = t + per + (me < more);
     while (t < end) {
         int lo = 0, hi = p.c.nseq - 1;  // the last sequence whose tiles begin at t or before
         while (lo < hi) {
@@ -145,14 +148,12 @@ template <typename F> __device__ inline void walk_line(const AttnArgs& p, long l
             if (pre[mid] <= t) lo = mid; else hi = mid - 1;
         }
         const SeqWork w = seq_work(p, lo);
-        const long long in_seq = t - pre[lo];
-        const int unit = (int)(in_seq / w.tiles), tile = (int)(in_seq % w.tiles), kvh = unit / w.blocks, block = unit % w.blocks;
-        const long long u0 = t - tile, u1 = u0 + w.tiles;  // the unit's tiles on the line
-        const int n = (int)(min(u1, end) - t);
+        const int in_seq = t - pre[lo], unit = in_seq / w.tiles, tile = in_seq - unit * w.tiles, kvh = unit / w.blocks, block = unit - kvh * w.blocks;
+        const int u0 = t - tile, u1 = u0 + w.tiles, n = min(u1, end) - t;  // the unit's tiles on the line; those of them here
         const size_t slot_unit = ((size_t)lo * p.c.kv_heads + kvh) * p.blocks + block;
-        const int c0 = (int)(((u0 + 1) * ctas - 1) / total), c1 = (int)((u1 * ctas - 1) / total);  // the CTAs of its first and last tile
-        if (tile == 0 && threadIdx.x == 0) p.unit_info[slot_unit] = make_int2(c0, c1 - c0 + 1);
-        work(w, lo, kvh, block, tile, n, c0 == c1, slot_unit + blockIdx.x);
+        const bool whole = n == w.tiles;
+        if (tile == 0 && threadIdx.x == 0) p.unit_info[slot_unit] = make_int2(me, whole ? 1 : owner(u1 - 1) - me + 1);
+        work(w, lo, kvh, block, tile, n, whole, slot_unit + me);
         t += n;
     }
 }
@@ -162,14 +163,15 @@ template <typename F> __device__ inline void walk_line(const AttnArgs& p, long l
 // for four rows.
 template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS, 2) attn_fma_kernel(const __grid_constant__ AttnArgs p) {
     constexpr int VEC = 16 / sizeof(KT), NC = HD / 8 / VEC, RW = 4, PAD = 4;  // elements of a load, loads of a lane and row
-    extern __shared__ long long pre[];
-    __shared__ long long sums[PA_WARPS];
+    extern __shared__ int pre[];
+    __shared__ int sums[PA_WARPS];
     __shared__ __align__(16) float so[PA_WARPS * RW * (HD + PAD)];
     __shared__ float2 sml[PA_WARPS * RW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l8 = lane & 7, side = lane >> 3;
     const int rw = warp % p.row_warps, tg = warp / p.row_warps, groups = PA_WARPS / p.row_warps;
     const KT* pool = static_cast<const KT*>(p.c.pool);
 
+    pdl_launch_dependents();
     walk_line(p, pre, sums, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
         float q[RW][NC * VEC], o[RW][NC * VEC], m[RW], l[RW];
         int last[RW];        // the last entry a row sees, -1: none
@@ -260,19 +262,25 @@ template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA
 }
 
 // ------------------------------------------------------------------------------------------------ the joint
-// One row and q head of a unit that several CTAs shared: sum their parts in order.  Rows that see nothing get zeros here.
-template <typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS) attn_join_kernel(const __grid_constant__ AttnArgs p) {
+// One row and q head of a unit that several CTAs shared: sum their parts in order.  Rows that see nothing get zeros here.  A chain of
+// latencies (unit_info, then everything else at once): a warp has its parts' rows in registers before it knows their factors.
+// PJ_THREADS: 64 where units have few parts (sixteen at once), 256 for the units of few long sequences.
+constexpr int PJ_DEEP = 8;
+template <typename QT, int HD, int PJ_THREADS> __global__ void __launch_bounds__(PJ_THREADS) attn_join_kernel(const __grid_constant__ AttnArgs p) {
+    constexpr int PJ_WARPS = PJ_THREADS / 32;
+    constexpr int MLS = (PA_MAX_CTAS + PJ_THREADS - 1) / PJ_THREADS, PER = 128 / HD;  // PER: parts a warp reads side by side, HD / 4 lanes each
     __shared__ float factor[PA_MAX_CTAS], red[32];
-    __shared__ float4 acc[PA_WARPS][HD / 4];
+    __shared__ float4 acc[PJ_WARPS][HD / 4];
     const int b = blockIdx.x / p.blocks / p.c.kv_heads, kvh = blockIdx.x / p.blocks % p.c.kv_heads, block = blockIdx.x % p.blocks, r = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const SeqWork w = seq_work(p, b);
     const int rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
     const size_t row_head = (size_t)(w.s.r0 + j) * p.heads + head;
     pdl_wait();  // (ahead of every return: a grid that ends early would let the next one start before the kernel ahead has ended)
+    if (p.scores) pdl_launch_dependents();
     if (rho >= w.s.n * p.group) return;
     if (w.tiles == 0) {
-        for (int col = tid; col < HD; col += PA_THREADS) store_out<QT>(p, row_head, HD, col, 0.f, 0.f);
+        for (int col = tid; col < HD; col += PJ_THREADS) store_out<QT>(p, row_head, HD, col, 0.f, 0.f);
         if (tid == 0) store_lse(p, row_head, 0.f, 0.f);
         return;
     }
@@ -280,41 +288,54 @@ template <typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS) att
     const int n = info.y;
     if (n <= 1) return;
     const size_t slot0 = (size_t)blockIdx.x + info.x;
+    float2 ml[MLS];
+#pragma unroll
+    for (int i = 0; i < MLS; ++i) ml[i] = tid + i * PJ_THREADS < n ? __ldcg(p.part_ml + (slot0 + tid + i * PJ_THREADS) * p.ru + r) : make_float2(-INFINITY, 0.f);
+    const int c4 = lane % (HD / 4), first = warp * PER + lane / (HD / 4);
+    const float4* rows = reinterpret_cast<const float4*>(p.part_o + (slot0 * p.ru + r) * HD) + c4;
+    const size_t step = (size_t)p.ru * HD / 4;
+    float4 x[PJ_DEEP];
+#pragma unroll
+    for (int d = 0; d < PJ_DEEP; ++d) {
+        const int i = first + d * PJ_WARPS * PER;
+        x[d] = i < n ? __ldcg(rows + i * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     float m = -INFINITY;
     bool nan = false;
-    for (int i = tid; i < n; i += PA_THREADS) {
-        const float x = __ldcg(p.part_ml + (slot0 + i) * p.ru + r).x;
-        m = fmaxf(m, x);
-        nan |= x != x;
+#pragma unroll
+    for (int i = 0; i < MLS; ++i) {
+        m = fmaxf(m, ml[i].x);
+        nan |= ml[i].x != ml[i].x;
     }
     m = block_max(m, red);
     if (__syncthreads_or(nan)) m = NAN;
     float l = 0.f;
-    for (int i = tid; i < n; i += PA_THREADS) {
-        const float2 ml = __ldcg(p.part_ml + (slot0 + i) * p.ru + r);
-        const float f = exp2f(ml.x - (m == -INFINITY ? 0.f : m));
-        factor[i] = f;
-        l += ml.y * f;
+#pragma unroll
+    for (int i = 0; i < MLS; ++i) {
+        const float f = exp2f(ml[i].x - (m == -INFINITY ? 0.f : m));
+        if (tid + i * PJ_THREADS < n) factor[tid + i * PJ_THREADS] = f;
+        l += ml[i].y * f;
     }
     l = block_sum(l, red);  // (its barriers: factor is complete)
-    constexpr int PER = 128 / HD;  // parts a warp reads side by side: a part's row is HD / 4 lanes
-    const int c4 = lane % (HD / 4), side = lane / (HD / 4);
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = warp * PER + side; i < n; i += PA_WARPS * PER) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((slot0 + i) * p.ru + r) * HD) + c4);
-        const float f = factor[i];
-        a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
+    auto add = [&](const float4& v, float f) {
+        a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+    };
+#pragma unroll
+    for (int d = 0; d < PJ_DEEP; ++d) {
+        const int i = first + d * PJ_WARPS * PER;
+        if (i < n) add(x[d], factor[i]);
     }
+    for (int i = first + PJ_DEEP * PJ_WARPS * PER; i < n; i += PJ_WARPS * PER) add(__ldcg(rows + i * step), factor[i]);
     if (PER == 2) {
         a.x += __shfl_xor_sync(0xffffffffu, a.x, 16); a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
         a.z += __shfl_xor_sync(0xffffffffu, a.z, 16); a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
     }
-    if (side == 0) acc[warp][c4] = a;
+    if (lane < HD / 4) acc[warp][c4] = a;
     __syncthreads();
-    for (int col = tid; col < HD; col += PA_THREADS) {
+    for (int col = tid; col < HD; col += PJ_THREADS) {
         float o = 0.f;
-        for (int i = 0; i < PA_WARPS; ++i) o += reinterpret_cast<const float*>(acc[i])[col];
+        for (int i = 0; i < PJ_WARPS; ++i) o += reinterpret_cast<const float*>(acc[i])[col];
         store_out<QT>(p, row_head, HD, col, o, l);
     }
     if (tid == 0) store_lse(p, row_head, m, l);

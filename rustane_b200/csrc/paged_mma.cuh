@@ -77,7 +77,7 @@ __host__ __device__ constexpr int mma_stages(int row_warps) { return row_warps =
 template <typename KT, typename QT, int HD, int ROW_WARPS> inline size_t mma_shared(int nseq) {
     const size_t q = (size_t)ROW_WARPS * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)PA_WARPS / ROW_WARPS * mma_stages(ROW_WARPS) * MMA_STAGE;
     const size_t o = (size_t)PA_WARPS * 16 * (HD + 4) * 4;  // (in the ring's place once it is empty)
-    return ((size_t)(nseq + 1) * 8 + 127) / 128 * 128 + q + (ring > o ? ring : o);
+    return ((size_t)(nseq + 1) * 4 + 127) / 128 * 128 + q + (ring > o ? ring : o);
 }
 
 template <typename KT, typename QT, int HD, int ROW_WARPS> __global__ void __launch_bounds__(PA_THREADS, MMA_CTAS) attn_mma_kernel(const __grid_constant__ AttnArgs p) {
@@ -86,11 +86,11 @@ template <typename KT, typename QT, int HD, int ROW_WARPS> __global__ void __lau
     constexpr int NQ = F::NQ, NP = F::NP, RW = 16, PAD = 4, TS = MMA_STAGE / 4 / HD, CH = HD / 8, KS = HD / 16, HALVES = TS / 16;  // TS: entries of a stage
     constexpr int STAGES = mma_stages(ROW_WARPS), groups = PA_WARPS / ROW_WARPS, gsize = ROW_WARPS * 32, PASS = gsize / CH, PASSES = TS / PASS;  // PASS: rows a copy of the whole group brings
     extern __shared__ __align__(128) char dyn[];
-    __shared__ long long sums[PA_WARPS];
+    __shared__ int sums[PA_WARPS];
     __shared__ float2 sml[PA_WARPS * RW];
     __shared__ float qscale[4 * RW];
-    long long* pre = reinterpret_cast<long long*>(dyn);
-    uint4* sq = reinterpret_cast<uint4*>(dyn + ((size_t)(p.c.nseq + 1) * 8 + 127) / 128 * 128);  // [row warps][NQ][KS][32 lanes]
+    int* pre = reinterpret_cast<int*>(dyn);
+    uint4* sq = reinterpret_cast<uint4*>(dyn + ((size_t)(p.c.nseq + 1) * 4 + 127) / 128 * 128);  // [row warps][NQ][KS][32 lanes]
     char* ring_all = reinterpret_cast<char*>(sq + ROW_WARPS * NQ * KS * 32);
     float* so = reinterpret_cast<float*>(ring_all);  // [warps][RW][HD + PAD]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -107,6 +107,7 @@ template <typename KT, typename QT, int HD, int ROW_WARPS> __global__ void __lau
     const int mr = lane & 7, mj = lane >> 3;
     const uint32_t k_at = (uint32_t)((mj >> 1) * 8 + mr) * HD * 2, v_at = (uint32_t)((mj & 1) * 8 + mr) * HD * 2 + TS * HD * 2;
 
+    pdl_launch_dependents();  // the joint's CTAs come in as these leave
     walk_line(p, pre, sums, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
         const int valid_rows = min(p.ru, w.s.n * p.group - block * p.ru);
         const int first = w.start + tile * PA_TILE, end = min(w.s.len, first + tiles * PA_TILE);
