@@ -14,6 +14,8 @@ struct Plan {
     size_t units, part_o, part_ml, unit_info, lse2, scores, bytes;  // offsets in the workspace
     long long score_stride;
 };
+// What a tile costs by its unit's rows: up to 16, 32, more (tensor-core form).
+constexpr int PA_WEIGHTS[3] = {2, 3, 6};
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // A warp has 4 rows of a unit with an fp32 pool (FMAs), 16 with a 16-bit one (tensor cores); a unit as many of its warps as its rows need.
@@ -44,9 +46,29 @@ int check_shape(const cd_paged_cache* c, int heads, int nrows, int max_rows, int
     if (max_rows < 1 || max_rows > 65536) return refuse(CD_ERR_INVALID, CALL, "max_rows must be in 1..65536");
     if (collect && !c->weight) return refuse(CD_ERR_INVALID, CALL, "collect needs the cache's weight");
     const Plan p = plan_of(c, heads, nrows, max_rows, collect);
+    // (2^31, and a tile's cost is at most PA_WEIGHTS[2])
     const long long tiles = ((long long)c->max_pages * c->page_tokens + PA_TILE - 1) / PA_TILE;
-    if (p.units > 0x7fffffffull || (long long)p.units * tiles >= 0x7fffffffll - PA_MAX_CTAS) return refuse(CD_ERR_UNSUPPORTED, CALL, "sequences x kv heads x row blocks x (max_pages x page_tokens / 64) must stay below 2^31");
+    if (p.units > 0x7fffffffull || (long long)p.units * tiles * PA_WEIGHTS[2] >= 0x7fffffffll - PA_MAX_CTAS) return refuse(CD_ERR_UNSUPPORTED, CALL, "sequences x kv heads x row blocks x (max_pages x page_tokens / 64) must stay below 2^28");
     return CD_OK;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) return nullptr;
+    return (EncodeTiledFn)fn;
+}
+// The pool as {column, row of a page, head of K then of V, page}, in boxes of 64 columns and sixteen rows.  false: by cp.async then.
+bool encode_pool(CUtensorMap* map, const PagedView& c, bool f16, int hd) {
+    static const EncodeTiledFn encode = encode_fn();
+    if (!encode) return false;
+    const cuuint64_t row = (cuuint64_t)hd * 2, head = row * c.page_tokens, page = head * 2 * c.kv_heads;
+    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)c.page_tokens, (cuuint64_t)2 * c.kv_heads, (cuuint64_t)c.npages}, strides[3] = {row, head, page};
+    const cuuint32_t box[4] = {64, 16, 1, 1}, step[4] = {1, 1, 1, 1};
+    return encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, c.pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a, const Plan& plan, int collect, cudaStream_t s) {
@@ -57,10 +79,12 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     if constexpr (std::is_same<KT, float>::value) {
         attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);
     } else {
-        void (*kernel)(AttnArgs) = a.row_warps == 1 ? attn_mma_kernel<KT, QT, HD, 1> : a.row_warps == 2 ? attn_mma_kernel<KT, QT, HD, 2> : attn_mma_kernel<KT, QT, HD, 4>;
-        const size_t shared = a.row_warps == 1 ? mma_shared<KT, QT, HD, 1>(a.c.nseq) : a.row_warps == 2 ? mma_shared<KT, QT, HD, 2>(a.c.nseq) : mma_shared<KT, QT, HD, 4>(a.c.nseq);
+        CUtensorMap map = {};
+        bool tma = (a.c.page_tokens & 15) == 0;
+        if (tma) tma = encode_pool(&map, a.c, std::is_same<KT, __half>::value, HD);
+        void (*kernel)(AttnArgs, CUtensorMap) = tma ? attn_mma_kernel<KT, QT, HD, true> : attn_mma_kernel<KT, QT, HD, false>;
         if ((e = allow_shared_memory((const void*)kernel)) != cudaSuccess) return e;
-        kernel<<<std::min(MMA_CTAS * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
+        kernel<<<std::min(MMA_CTAS * sms, PA_MAX_CTAS), PA_THREADS, mma_shared<KT, QT, HD>(a.c.nseq, a.row_warps), s>>>(a, map);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const dim3 grid((unsigned)plan.units, (unsigned)std::min<long long>(a.ru, (long long)a.max_rows * a.group));
@@ -114,6 +138,7 @@ extern "C" int cd_paged_attention(const cd_paged_cache* c, int dtype, int heads,
     a.scores = collect ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;
     a.q_stride = q_stride;
     a.score_stride = plan.score_stride;
+    for (int i = 0; i < 3; ++i) a.weights[i] = c->dtype == CD_DTYPE_F32 ? 1 : PA_WEIGHTS[i];
     a.scale_log2 = (scale > 0.f ? scale : 1.0f / std::sqrt((float)c->hd)) * 1.44269504088896340736f;
     a.heads = heads;
     a.group = plan.group;

@@ -26,13 +26,14 @@ struct AttnArgs {
     float* lse2;      // [nrows][heads] log2; with scores only
     float* scores;    // [nrows][heads][score_stride] log2 domain, or nullptr
     long long q_stride, score_stride;
+    int weights[3];  // what a tile of a unit of up to 16, 32 and more rows costs on the line; the first is the least
     float scale_log2;
     int heads, group, nrows, max_rows, window, ru, row_warps, blocks;  // blocks: row blocks a sequence may have
 };
 
 struct SeqWork {
     BatchSeq s;
-    int start, tiles, blocks;
+    int start, tiles, blocks, weight;
 };
 __device__ inline SeqWork seq_work(const AttnArgs& p, int b) {
     SeqWork w;
@@ -43,34 +44,44 @@ __device__ inline SeqWork seq_work(const AttnArgs& p, int b) {
         w.start = first > 0 ? first & ~(PA_TILE - 1) : 0;
     }
     w.tiles = w.s.n > 0 && w.s.len > 0 ? (w.s.len - w.start + PA_TILE - 1) / PA_TILE : 0;
-    w.blocks = (w.s.n * p.group + p.ru - 1) / p.ru;
+    const int rows = w.s.n * p.group;
+    w.blocks = (rows + p.ru - 1) / p.ru;
+    w.weight = p.weights[rows <= 16 ? 0 : rows <= 32 ? 1 : 2];
     return w;
 }
 
-// pre[b] = tiles of the sequences before b (all threads; ends with a barrier); returns the total (the host keeps it below 2^31)
-__device__ inline int line_up(const AttnArgs& p, int* pre, int* sums) {
+// pre[b] = cost of the sequences before b (all threads; ends with a barrier), most = the dearest tile; returns the total (the host keeps
+// it below 2^31).  sums: 2 PA_WARPS words.
+__device__ inline int line_up(const AttnArgs& p, int* pre, int* sums, int& most) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int carry = 0;
+    most = 1;
     if (tid == 0) pre[0] = 0;
     for (int base = 0; base < p.c.nseq; base += PA_THREADS) {
         const int b = base + tid;
-        int v = 0;
+        int v = 0, dear = 1;
         if (b < p.c.nseq) {
             const SeqWork w = seq_work(p, b);
-            v = w.tiles * w.blocks * p.c.kv_heads;
+            if (w.tiles) dear = w.weight;
+            v = w.tiles * w.weight * w.blocks * p.c.kv_heads;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += x;
         }
-        if (lane == 31) sums[warp] = v;
+        dear = __reduce_max_sync(0xffffffffu, dear);
+        if (lane == 31) {
+            sums[warp] = v;
+            sums[PA_WARPS + warp] = dear;
+        }
         __syncthreads();
         int before = carry;
 #pragma unroll
         for (int i = 0; i < PA_WARPS; ++i) {
             if (i < warp) before += sums[i];
             carry += sums[i];
+            most = max(most, sums[PA_WARPS + i]);
         }
         if (b < p.c.nseq) pre[b + 1] = before + v;
         __syncthreads();
@@ -93,6 +104,14 @@ constexpr float LN2 = 0.69314718055994530942f;
 template <typename QT> __device__ inline void store_out(const AttnArgs& p, size_t row_head, int hd, int col, float o, float l) {
     static_cast<QT*>(p.out)[row_head * hd + col] = from_float<QT>(l > 0.f || l != l ? o / l : 0.f);
 }
+template <typename QT> __device__ inline void store_out4(const AttnArgs& p, size_t row_head, int hd, int c4, const float4& o, float l) {
+    const bool some = l > 0.f || l != l;
+    const float x[4] = {some ? o.x / l : 0.f, some ? o.y / l : 0.f, some ? o.z / l : 0.f, some ? o.w / l : 0.f};
+    struct alignas(4 * sizeof(QT)) Four { QT e[4]; } v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.e[e] = from_float<QT>(x[e]);
+    *reinterpret_cast<Four*>(static_cast<QT*>(p.out) + row_head * hd + c4 * 4) = v;
+}
 __device__ inline void store_lse(const AttnArgs& p, size_t row_head, float m, float l) {
     const float lse2 = l > 0.f || l != l ? m + log2f(l) : -INFINITY;
     if (p.lse) p.lse[row_head] = lse2 * LN2;
@@ -106,55 +125,62 @@ template <int HD, int PAD> struct UnitParts {
 };
 // Merge the entry groups and store: the result where the unit is this CTA's alone, else this CTA's slot.  All threads.
 template <typename QT, int HD, int PAD>
-__device__ inline void finish_unit(const AttnArgs& p, const UnitParts<HD, PAD>& u, int rows_per_warp, const SeqWork& w, int kvh, int block, bool whole, size_t slot) {
-    const int groups = PA_WARPS / p.row_warps, rows = min(p.ru, w.s.n * p.group - block * p.ru);
-    for (int at = threadIdx.x; at < rows * HD; at += PA_THREADS) {
-        const int r = at / HD, col = at % HD, rw = r / rows_per_warp, rr = r % rows_per_warp;
+__device__ inline void finish_unit(const AttnArgs& p, const UnitParts<HD, PAD>& u, int rows_per_warp, int row_warps, const SeqWork& w, int kvh, int block, bool whole, size_t slot) {
+    const int groups = PA_WARPS / row_warps, rows = min(p.ru, w.s.n * p.group - block * p.ru);
+    for (int at = threadIdx.x; at < rows * (HD / 4); at += PA_THREADS) {
+        const int r = at / (HD / 4), c4 = at % (HD / 4), rw = r / rows_per_warp, rr = r % rows_per_warp;
         float m = -INFINITY;
-        for (int t = 0; t < groups; ++t) m = fmaxf(m, u.ml[(t * p.row_warps + rw) * rows_per_warp + rr].x);
+        for (int t = 0; t < groups; ++t) m = fmaxf(m, u.ml[(t * row_warps + rw) * rows_per_warp + rr].x);
         const float base = m == -INFINITY ? 0.f : m;
-        float l = 0.f, o = 0.f;
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int t = 0; t < groups; ++t) {
-            const int at_w = (t * p.row_warps + rw) * rows_per_warp + rr;
+            const int at_w = (t * row_warps + rw) * rows_per_warp + rr;
             const float2 ml = u.ml[at_w];
             const float f = exp2f(ml.x - base);
+            const float4 x = *reinterpret_cast<const float4*>(u.o + (size_t)at_w * (HD + PAD) + c4 * 4);
             l += ml.y * f;
-            o += u.o[(size_t)at_w * (HD + PAD) + col] * f;
+            o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
         }
         if (whole) {
             const int rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
             const size_t row_head = (size_t)(w.s.r0 + j) * p.heads + head;
-            store_out<QT>(p, row_head, HD, col, o, l);
-            if (col == 0) store_lse(p, row_head, m, l);
+            store_out4<QT>(p, row_head, HD, c4, o, l);
+            if (c4 == 0) store_lse(p, row_head, m, l);
         } else {
-            p.part_o[(slot * p.ru + r) * HD + col] = o;
-            if (col == 0) p.part_ml[slot * p.ru + r] = make_float2(m, l);
+            *reinterpret_cast<float4*>(p.part_o + (slot * p.ru + r) * HD + c4 * 4) = o;
+            if (c4 == 0) p.part_ml[slot * p.ru + r] = make_float2(m, l);
         }
     }
 }
 
 // Walk this CTA's share of the line; work(w, b, kvh, block, first tile, tiles, whole, slot) handles a run of one unit's tiles.
+// A tile belongs to the CTA whose share its first point lies in; no share is shorter than a tile, so none is empty.
 template <typename F> __device__ inline void walk_line(const AttnArgs& p, int* pre, int* sums, F&& work) {
-    const int total = line_up(p, pre, sums), ctas = min((int)gridDim.x, total), me = blockIdx.x;  // no share is empty
-    if (me >= ctas) return;
-    const int per = total / ctas, more = total - per * ctas, cut = more * (per + 1);  // the first `more` shares have one tile more
+    int most;
+    const int total = line_up(p, pre, sums, most), ctas = min((int)gridDim.x, max(1, total / most)), me = blockIdx.x;
+    if (me >= ctas || total == 0) return;
+    const int per = total / ctas, more = total - per * ctas, cut = more * (per + 1);  // the first `more` shares are one longer
     auto owner = [&](int t) { return t < cut ? t / (per + 1) : more + (t - cut) / per; };
     int t = me * per + min(me, more);
     const int end = t + per + (me < more);
     while (t < end) {
-        int lo = 0, hi = p.c.nseq - 1;  // the last sequence whose tiles begin at t or before
+        int lo = 0, hi = p.c.nseq - 1;  // the last sequence that begins at t or before
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (pre[mid] <= t) lo = mid; else hi = mid - 1;
         }
         const SeqWork w = seq_work(p, lo);
-        const int in_seq = t - pre[lo], unit = in_seq / w.tiles, tile = in_seq - unit * w.tiles, kvh = unit / w.blocks, block = unit - kvh * w.blocks;
-        const int u0 = t - tile, u1 = u0 + w.tiles, n = min(u1, end) - t;  // the unit's tiles on the line; those of them here
-        const size_t slot_unit = ((size_t)lo * p.c.kv_heads + kvh) * p.blocks + block;
-        const bool whole = n == w.tiles;
-        if (tile == 0 && threadIdx.x == 0) p.unit_info[slot_unit] = make_int2(me, whole ? 1 : owner(u1 - 1) - me + 1);
-        work(w, lo, kvh, block, tile, n, whole, slot_unit + me);
-        t += n;
+        const int long_ = w.tiles * w.weight, in_seq = t - pre[lo], unit = in_seq / long_, in_unit = in_seq - unit * long_;
+        const int kvh = unit / w.blocks, block = unit - kvh * w.blocks, u0 = t - in_unit;
+        const int first = (in_unit + w.weight - 1) / w.weight, last = min(w.tiles, (end - u0 + w.weight - 1) / w.weight), n = last - first;
+        if (n > 0) {
+            const size_t slot_unit = ((size_t)lo * p.c.kv_heads + kvh) * p.blocks + block;
+            const bool whole = n == w.tiles;
+            if (first == 0 && threadIdx.x == 0) p.unit_info[slot_unit] = make_int2(me, whole ? 1 : owner(u0 + (w.tiles - 1) * w.weight) - me + 1);
+            work(w, lo, kvh, block, first, n, whole, slot_unit + me);
+        }
+        t = u0 + long_;
     }
 }
 
@@ -164,7 +190,7 @@ template <typename F> __device__ inline void walk_line(const AttnArgs& p, int* p
 template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS, 2) attn_fma_kernel(const __grid_constant__ AttnArgs p) {
     constexpr int VEC = 16 / sizeof(KT), NC = HD / 8 / VEC, RW = 4, PAD = 4;  // elements of a load, loads of a lane and row
     extern __shared__ int pre[];
-    __shared__ int sums[PA_WARPS];
+    __shared__ int sums[2 * PA_WARPS];
     __shared__ __align__(16) float so[PA_WARPS * RW * (HD + PAD)];
     __shared__ float2 sml[PA_WARPS * RW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l8 = lane & 7, side = lane >> 3;
@@ -257,7 +283,7 @@ template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA
             }
         }
         __syncthreads();
-        finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sml}, RW, w, kvh, block, whole, slot);
+        finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sml}, RW, p.row_warps, w, kvh, block, whole, slot);
     });
 }
 

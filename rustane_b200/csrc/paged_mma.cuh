@@ -1,20 +1,21 @@
 // The tensor-core form of paged attention, for 16-bit pools: mma.m16n8k16 with sixteen rows of a unit per warp.
 //
-// The warps that have different rows of the same entries are a group with a ring of stages in shared memory: 8 KB of K and V each
-// (sixteen entries at hd 128, 32 at hd 64), brought by cp.async 16 bytes at a time, two or more stages ahead of the products.  A row's 16-byte
-// chunks are exchanged by the low bits of its place (chunk ^ place & 7), so that ldmatrix meets every bank once.  A group of one
-// warp meets no barrier inside the loop at all.
+// The warps that have different rows of the same entries (one, two or four, as the unit's rows need) are a group with a ring of stages in
+// shared memory: 4 KB of K and 4 KB of V each (sixteen entries at hd 128, 32 at hd 64), as boxes of sixteen rows of 128 bytes whose
+// 16-byte chunks are exchanged by the low bits of the row (TMA's 128-byte swizzle), so that ldmatrix meets every bank once and an
+// address is one XOR.  K's half of a stage is filled again as soon as the scores are out, V's as soon as P V is.  One thread of the group issues
+// the boxes; a group of one warp meets no barrier inside the loop.  Pages whose size is no multiple of sixteen have no such
+// boxes; their rows come by cp.async, 16 bytes at a time (TMA = false): sixteen instructions a step, which took a quarter of it.
 //
 // mma.sync and not tcgen05: a token's unit has 1 to 16 rows, of a 64-row minimum there, and the work is bound by the bytes of K and V.
-// cp.async and not TMA tiles: pages may have any number of entries, places behind the last entry arrive as zeros, and the 64 KB an
-// SM needs under way to keep HBM busy are there with two CTAs of four warps.  (K and V straight to registers, no ring: 774
-// instructions per sixteen entries and 3.8 us between them at three CTAs an SM, 130001 entries of four heads 70 us.)
 //
 // Exactness: q of 32 bits is two fp16 parts (scaled by a power of two per row) or three bf16 parts, P two or three parts with an fp32
 // result or a bf16 pool (a single bf16 P would cost 2^-9 a term, half the result's own rounding) and one with fp16 (2^-12).  Sums
 // stay in 32 bits; with an fp32 result every step's product goes to fresh accumulators and is added by the CUDA cores, which round
 // to nearest where the tensor cores cut off.
 #pragma once
+#include <cuda.h>
+
 #include "paged_attn.cuh"
 
 namespace cd {
@@ -66,355 +67,460 @@ __device__ inline void ldsm_t(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
+// (not volatile, unlike Mma16's: the compiler may mix products and other work)
+template <typename KT> __device__ inline void product(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ inline void product<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ inline void product<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 template <typename KT, typename QT> struct MmaForm {
     static constexpr bool F16 = std::is_same<KT, __half>::value, WIDE = std::is_same<QT, float>::value;
     static constexpr int NQ = WIDE ? (F16 ? 2 : 3) : 1, NP = WIDE ? (F16 ? 2 : 3) : F16 ? 1 : 2;
     static constexpr int SHIFT = F16 ? (NP == 2 ? 12 : 8) : 0;  // P is times 2^SHIFT: fp16 parts of small ones keep their digits
 };
-constexpr int MMA_STAGE = 8192, MMA_CTAS = 2;  // bytes of a stage: K, then V; CTAs an SM
-// stages of a group's ring: with one row warp four groups of three (96 KB a CTA), with more row warps fewer groups of six
-__host__ __device__ constexpr int mma_stages(int row_warps) { return row_warps == 1 ? 3 : 6; }
-template <typename KT, typename QT, int HD, int ROW_WARPS> inline size_t mma_shared(int nseq) {
-    const size_t q = (size_t)ROW_WARPS * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)PA_WARPS / ROW_WARPS * mma_stages(ROW_WARPS) * MMA_STAGE;
+constexpr int MMA_STAGE = 8192;  // bytes of a stage: K, then V
+constexpr int MMA_CTAS = 2, MMA_SLOTS = 12;  // CTAs an SM, stages of a CTA, which its groups share
+template <typename KT, typename QT, int HD> inline size_t mma_shared(int nseq, int row_warps) {
+    const size_t q = (size_t)row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)MMA_SLOTS * MMA_STAGE;
     const size_t o = (size_t)PA_WARPS * 16 * (HD + 4) * 4;  // (in the ring's place once it is empty)
-    return ((size_t)(nseq + 1) * 4 + 127) / 128 * 128 + q + (ring > o ? ring : o);
+    return (ring > o ? ring : o) + q + (size_t)(nseq + 1) * 4 + 1024;  // (1024: the ring's own alignment)
 }
+__device__ inline void load_box(uint32_t dst, const CUtensorMap* map, int col, int row, int head, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(row), "r"(head), "r"(page) : "memory");
+}
+__device__ inline void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-template <typename KT, typename QT, int HD, int ROW_WARPS> __global__ void __launch_bounds__(PA_THREADS, MMA_CTAS) attn_mma_kernel(const __grid_constant__ AttnArgs p) {
+template <int HD> struct MmaShared {
+    float2 ml[PA_WARPS * 16];
+    float qscale[4 * 16];
+    unsigned long long bars[2 * MMA_SLOTS];  // of stage s: K at 2 s, V at 2 s + 1; at the start of a unit all are in an even phase
+};
+
+// A run of one unit's tiles, its rows on ROW_WARPS warps.
+template <typename KT, typename QT, int HD, int ROW_WARPS, bool TMA>
+__device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* map, char* ring_all, uint4* sq, MmaShared<HD>& sh, const SeqWork& w, int b, int kvh, int block, int tile, int tiles,
+                                         bool whole, size_t slot) {
     using X = Mma16<KT>;
     using F = MmaForm<KT, QT>;
     constexpr int NQ = F::NQ, NP = F::NP, RW = 16, PAD = 4, TS = MMA_STAGE / 4 / HD, CH = HD / 8, KS = HD / 16, HALVES = TS / 16;  // TS: entries of a stage
-    constexpr int STAGES = mma_stages(ROW_WARPS), groups = PA_WARPS / ROW_WARPS, gsize = ROW_WARPS * 32, PASS = gsize / CH, PASSES = TS / PASS;  // PASS: rows a copy of the whole group brings
-    extern __shared__ __align__(128) char dyn[];
-    __shared__ int sums[PA_WARPS];
-    __shared__ float2 sml[PA_WARPS * RW];
-    __shared__ float qscale[4 * RW];
-    int* pre = reinterpret_cast<int*>(dyn);
-    uint4* sq = reinterpret_cast<uint4*>(dyn + ((size_t)(p.c.nseq + 1) * 4 + 127) / 128 * 128);  // [row warps][NQ][KS][32 lanes]
-    char* ring_all = reinterpret_cast<char*>(sq + ROW_WARPS * NQ * KS * 32);
+    constexpr int groups = PA_WARPS / ROW_WARPS, gsize = ROW_WARPS * 32, STAGES = MMA_SLOTS / groups < 4 ? MMA_SLOTS / groups : 4;
+    constexpr int PASS = gsize / CH, PASSES = TS / PASS, VOFF = MMA_STAGE / 2, BOX = 2048;  // PASS: rows that one copy of the whole group brings
     float* so = reinterpret_cast<float*>(ring_all);  // [warps][RW][HD + PAD]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int rw = warp % ROW_WARPS, tg = warp / ROW_WARPS, gt = rw * 32 + lane;
     const uint32_t ring_base = (uint32_t)__cvta_generic_to_shared(ring_all), ring = ring_base + tg * STAGES * MMA_STAGE;
     const KT* pool = static_cast<const KT*>(p.c.pool);
-    const bool page16 = (p.c.page_tokens & 15) == 0;
     const size_t v_off = (size_t)p.c.kv_heads * p.c.page_tokens * HD;
     auto group_sync = [&]() {
         if constexpr (ROW_WARPS == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(tg + 1), "r"(gsize) : "memory");
     };
-    // ldmatrix: lane l points at row l % 8 of matrix l / 8
+    // ldmatrix: lane l points at row l % 8 of matrix l / 8; a chunk's place is XORed in
     const int mr = lane & 7, mj = lane >> 3;
-    const uint32_t k_at = (uint32_t)((mj >> 1) * 8 + mr) * HD * 2, v_at = (uint32_t)((mj & 1) * 8 + mr) * HD * 2 + TS * HD * 2;
+    const uint32_t k_at = (uint32_t)((mj >> 1) * 8 + mr) * 128 + (((mj & 1) ^ mr) << 4), v_at = (uint32_t)((mj & 1) * 8 + mr) * 128 + VOFF + (((mj >> 1) ^ mr) << 4);
+    auto box_of = [](int pair, int half) { return HD == 128 ? pair / 4 * BOX : half * BOX; };  // of 32 bytes `pair` of a row, entries 16 half ..
+    auto word_at = [](int row, int chunk) { return (HD == 128 ? chunk / 8 * BOX : 0) / 4 + row * 32 + (((chunk & 7) ^ (row & 7)) << 2); };  // 32-bit words
 
-    pdl_launch_dependents();  // the joint's CTAs come in as these leave
-    walk_line(p, pre, sums, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
-        const int valid_rows = min(p.ru, w.s.n * p.group - block * p.ru);
-        const int first = w.start + tile * PA_TILE, end = min(w.s.len, first + tiles * PA_TILE);
-        const int span = end - first - tg * TS, steps = span > 0 ? (span + groups * TS - 1) / (groups * TS) : 0;  // of this group
-        __syncthreads();  // the unit before has been read
-        // ---- the ring: page ids are looked up a step ahead of the copies
-        int pages[HALVES];
-        auto look_up = [&](int t0) {
-            if (page16)
+    const int valid_rows = min(p.ru, w.s.n * p.group - block * p.ru);
+    const int first = w.start + tile * PA_TILE, end = min(w.s.len, first + tiles * PA_TILE);
+    if (TMA) async_proxy_fence();  // (what was written over the ring comes before the copies into it)
+    __syncthreads();               // the unit before has been read
+    // ---- the ring: page ids are looked up a step ahead of the copies
+    const bool leader = TMA && rw == 0 && lane == 0;
+    const uint32_t bars = smem_addr(sh.bars) + tg * STAGES * 16;
+    int pages[HALVES];
+    auto look_up = [&](int t0) {
+        if (TMA)
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) pages[h] = t0 + 16 * h < end ? page_at(p.c, b, t0 + 16 * h) : -1;
-        };
-        uint32_t gaps = 0;  // bit s: stage s lacks a page
-        const int row0 = gt / CH, ch = gt % CH;  // this thread's place in a pass
-        int next = 0, put = 0;                      // the step to issue, its stage
-        auto issue = [&]() {
-            if (next < steps) {
-                const int t0 = first + (next * groups + tg) * TS;
-                const uint32_t to = ring + put * MMA_STAGE + row0 * HD * 2;
-                bool lacks = false;
-                if (page16) {
-                    const KT* half_at[HALVES];
+            for (int h = 0; h < HALVES; ++h) pages[h] = t0 + 16 * h < end ? page_word(p.c, b, t0 + 16 * h) : 0;
+    };
+    uint32_t gaps = 0;                                           // bit s: stage s lacks a page
+    int next = first + tg * TS, put = 0;                         // the step whose K is next, its stage
+    int now_page[HALVES], now_off[HALVES];                       // of the stage whose V is next
+    uint32_t has = 0;                                            // bit k: this thread's row of pass k is there
+    const KT* from[TMA ? 1 : PASSES];
+    const int row0 = gt / CH, ch = gt % CH;                      // this thread's place in a pass
+    auto copy_half = [&](int half) {                             // 0: K, 1: V of the stage that `put` and the above describe
+        if constexpr (TMA) {
+            if (leader) {
+                const uint32_t to = ring + put * MMA_STAGE + half * VOFF, bar = bars + put * 16 + half * 8;
+                int boxes = 0;
 #pragma unroll
-                    for (int h = 0; h < HALVES; ++h) {
-                        half_at[h] = pool + (pages[h] >= 0 ? row_at(p.c, pages[h], 0, kvh, t0 + 16 * h, HD) : 0) + row0 * HD + ch * 8;
-                        lacks |= pages[h] < 0;
-                    }
-                    if (t0 + TS <= end && !lacks) {
+                for (int h = 0; h < HALVES; ++h) boxes += now_page[h] >= 0 ? HD / 64 : 0;
+                mbar_arrive_expect_tx(bar, boxes * BOX);
 #pragma unroll
-                        for (int k = 0; k < PASSES; ++k) {
-                            const KT* src = half_at[k * PASS / 16] + k * PASS % 16 * HD;
-                            const uint32_t dst = to + k * PASS * HD * 2 + ((ch ^ ((row0 + k * PASS) & 7)) << 4);
-                            copy16(dst, src, true);
-                            copy16(dst + TS * HD * 2, src + v_off, true);
-                        }
-                    } else {
-                        lacks = false;
+                for (int h = 0; h < HALVES; ++h)
+                    if (now_page[h] >= 0)
 #pragma unroll
-                        for (int k = 0; k < PASSES; ++k) {
-                            const bool there = pages[k * PASS / 16] >= 0 && t0 + row0 + k * PASS < end;
-                            const KT* src = half_at[k * PASS / 16] + k * PASS % 16 * HD;
-                            const uint32_t dst = to + k * PASS * HD * 2 + ((ch ^ ((row0 + k * PASS) & 7)) << 4);
-                            copy16(dst, there ? src : pool, there);
-                            copy16(dst + TS * HD * 2, there ? src + v_off : pool, there);
-                        }
-#pragma unroll
-                        for (int h = 0; h < HALVES; ++h) lacks |= pages[h] < 0 && t0 + 16 * h < end;
-                    }
-                    look_up(t0 + groups * TS);
-                } else {  // pages of odd sizes: lane r looks up row r (every warp of the group all of them: they agree on gaps)
-                    const bool in = lane < TS && t0 + lane < end;
-                    const int mine = in ? page_at(p.c, b, t0 + lane) : -1;
-                    lacks = __any_sync(0xffffffffu, in && mine < 0);
-#pragma unroll
-                    for (int k = 0; k < PASSES; ++k) {
-                        const int row = row0 + k * PASS, pg = __shfl_sync(0xffffffffu, mine, row);
-                        const bool there = pg >= 0;
-                        const KT* src = pool + (there ? row_at(p.c, pg, 0, kvh, t0 + row, HD) + ch * 8 : 0);
-                        const uint32_t dst = to + k * PASS * HD * 2 + ((ch ^ (row & 7)) << 4);
-                        copy16(dst, src, there);
-                        copy16(dst + TS * HD * 2, src + (there ? v_off : 0), there);
-                    }
-                }
-                gaps = (gaps & ~(1u << put)) | (uint32_t)lacks << put;
+                        for (int j = 0; j < HD / 64; ++j) load_box(to + (HD == 128 ? j : h) * BOX, map, j * 64, now_off[h], half * p.c.kv_heads + kvh, now_page[h], bar);
             }
-            ++next;
-            put = put + 1 == STAGES ? 0 : put + 1;
-            copies_close();
-        };
-        look_up(first + tg * TS);
+        } else {
+            const size_t off = half ? v_off : 0;
 #pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) issue();
-        // ---- q, as the products' operand
-        for (int r = warp; r < ROW_WARPS * RW; r += PA_WARPS) {
-            constexpr int EL = HD / 32;  // elements of a lane: EL lane .. EL lane + EL - 1
-            float x[EL];
-            if (r < valid_rows) {
-                const int rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
-                const QT* src = static_cast<const QT*>(p.q) + (size_t)(w.s.r0 + j) * p.q_stride + (size_t)head * HD + lane * EL;
-#pragma unroll
-                for (int e = 0; e < EL; ++e) x[e] = as_float(src[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < EL; ++e) x[e] = 0.f;
+            for (int k = 0; k < PASSES; ++k) {
+                const bool there = has >> k & 1u;
+                copy16(ring + put * MMA_STAGE + half * VOFF + word_at(row0 + k * PASS, ch) * 4, there ? from[k] + off : pool, there);
             }
-            float back = 1.f;
-            if (F::F16 && F::WIDE) {
-                float most = 0.f;
-#pragma unroll
-                for (int e = 0; e < EL; ++e) most = fmaxf(most, fabsf(x[e]));
-                most = warp_max(most);
-                if (most > 0.f && most < INFINITY) {
-                    const int ex = max(-100, ilogbf(most)) - 7;
-                    back = __int_as_float((127 + ex) << 23);
-                    const float by = __int_as_float((127 - ex) << 23);
-#pragma unroll
-                    for (int e = 0; e < EL; ++e) x[e] *= by;
-                }
-            }
-            if (lane == 0) qscale[r] = back * p.scale_log2;
-            // row r, column d: register (d % 16 / 8) * 2 + r % 16 / 8 of lane (r % 8) * 4 + d % 8 / 2, k-step d / 16
-#pragma unroll
-            for (int part = 0; part < NQ; ++part)
-#pragma unroll
-                for (int e = 0; e < EL; e += 2) {
-                    const int d = lane * EL + e;
-                    uint32_t* dst = reinterpret_cast<uint32_t*>(sq + ((size_t)(r / RW * NQ + part) * KS + d / 16) * 32 + (r % 8) * 4 + d % 8 / 2);
-                    dst[d % 16 / 8 * 2 + r % RW / 8] = X::part(x[e], x[e + 1]);
-                }
         }
-        __syncthreads();
-        float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, scale[2];
-        int last[2];
-        float* srow[2];
+    };
+    auto issue_k = [&]() {
+        if (next < end) {
+            bool lacks = false;
+            if constexpr (TMA) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = rw * RW + g + 8 * h, rho = block * p.ru + r, j = rho / p.group;
-            last[h] = r < valid_rows ? w.s.len - w.s.n + j : -1;
-            scale[h] = qscale[r];
-            srow[h] = p.scores && r < valid_rows ? p.scores + ((size_t)(w.s.r0 + j) * p.heads + kvh * p.group + rho % p.group) * p.score_stride : nullptr;
+                for (int h = 0; h < HALVES; ++h) {
+                    const int t = next + 16 * h;
+                    now_page[h] = t < end ? checked_page(p.c, pages[h]) : -1;
+                    now_off[h] = p.c.page_shift >= 0 ? t & (p.c.page_tokens - 1) : t % p.c.page_tokens;
+                    lacks |= now_page[h] < 0 && t < end;
+                }
+                look_up(next + groups * TS);
+            } else {  // lane r looks up row r (every warp of the group all of them: they agree on gaps)
+                const bool in = lane < TS && next + lane < end;
+                const int mine = in ? page_at(p.c, b, next + lane) : -1;
+                lacks = __any_sync(0xffffffffu, in && mine < 0);
+                has = 0;
+#pragma unroll
+                for (int k = 0; k < PASSES; ++k) {
+                    const int row = row0 + k * PASS, pg = __shfl_sync(0xffffffffu, mine, row);
+                    from[k] = pool + (pg >= 0 ? row_at(p.c, pg, 0, kvh, next + row, HD) + ch * 8 : 0);
+                    has |= (uint32_t)(pg >= 0) << k;
+                }
+            }
+            gaps = (gaps & ~(1u << put)) | (uint32_t)lacks << put;
+            copy_half(0);
         }
+        if (!TMA) copies_close();
+    };
+    auto issue_v = [&]() {
+        if (next < end) copy_half(1);
+        next += groups * TS;
+        put = put + 1 == STAGES ? 0 : put + 1;
+        if (!TMA) copies_close();
+    };
+    bool lost = false;
+    auto arrived = [&](int stage, int half, uint32_t phase) {
+        if constexpr (TMA) {
+            if (!lost && !mbar_wait(bars + stage * 16 + half * 8, phase)) {  // (bounded: a copy that never lands is reported, not waited for again)
+                lost = true;
+                report(p.c.status, CD_STATUS_WAIT);
+            }
+        } else copies_wait<2 * STAGES - 2>();
+    };
+    look_up(next);
+    // q is asked for ahead of the copies, which would otherwise be served first
+    constexpr int EL = HD / 32, QR = ROW_WARPS * RW / PA_WARPS;  // elements of a lane: EL lane .. EL lane + EL - 1; rows of a warp
+    struct alignas(EL * sizeof(QT)) QWord { QT e[EL]; } q_raw[QR];
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
+    for (int k = 0; k < QR; ++k) {
+        const int r = warp + k * PA_WARPS;
+        if (r < valid_rows) {
+            const int rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
+            q_raw[k] = *reinterpret_cast<const QWord*>(static_cast<const QT*>(p.q) + (size_t)(w.s.r0 + j) * p.q_stride + (size_t)head * HD + lane * EL);
+        }
+    }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-        const uint4* q4 = sq + (size_t)rw * NQ * KS * 32 + lane;
-        const int all_see = w.s.len - w.s.n, none_out = p.window > 0 ? w.s.len - p.window : 0;  // every row sees entries none_out .. all_see
-        const bool mixed = w.s.n > 1 || p.window > 0;
-        auto sees = [&](int t, int h) { return t <= last[h] && (p.window == 0 || t > last[h] - p.window); };
+    for (int i = 0; i < STAGES - 1; ++i) {
+        issue_k();
+        issue_v();
+    }
+    issue_k();
+    // ---- q, as the products' operand
+#pragma unroll
+    for (int qk = 0; qk < QR; ++qk) {
+        const int r = warp + qk * PA_WARPS;
+        float x[EL];
+#pragma unroll
+        for (int e = 0; e < EL; ++e) x[e] = r < valid_rows ? as_float(q_raw[qk].e[e]) : 0.f;
+        float back = 1.f;
+        if (F::F16 && F::WIDE) {
+            float most = 0.f;
+#pragma unroll
+            for (int e = 0; e < EL; ++e) most = fmaxf(most, fabsf(x[e]));
+            most = warp_max(most);
+            if (most > 0.f && most < INFINITY) {
+                const int ex = max(-100, ilogbf(most)) - 7;
+                back = __int_as_float((127 + ex) << 23);
+                const float by = __int_as_float((127 - ex) << 23);
+#pragma unroll
+                for (int e = 0; e < EL; ++e) x[e] *= by;
+            }
+        }
+        if (lane == 0) sh.qscale[r] = back * p.scale_log2;
+        // row r, column d: register (d % 16 / 8) * 2 + r % 16 / 8 of lane (r % 8) * 4 + d % 8 / 2, k-step d / 16
+#pragma unroll
+        for (int part = 0; part < NQ; ++part)
+#pragma unroll
+            for (int e = 0; e < EL; e += 2) {
+                const int d = lane * EL + e;
+                uint32_t* dst = reinterpret_cast<uint32_t*>(sq + ((size_t)(r / RW * NQ + part) * KS + d / 16) * 32 + (r % 8) * 4 + d % 8 / 2);
+                dst[d % 16 / 8 * 2 + r % RW / 8] = X::part(x[e], x[e + 1]);
+            }
+    }
+    __syncthreads();
+    float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, scale[2];
+    int last[2];
+    float* srow[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = rw * RW + g + 8 * h, rho = block * p.ru + r, j = rho / p.group;
+        last[h] = r < valid_rows ? w.s.len - w.s.n + j : -1;
+        scale[h] = sh.qscale[r];
+        srow[h] = p.scores && r < valid_rows ? p.scores + ((size_t)(w.s.r0 + j) * p.heads + kvh * p.group + rho % p.group) * p.score_stride : nullptr;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    const uint4* q4 = sq + (size_t)rw * NQ * KS * 32 + lane;
+    const int all_see = w.s.len - w.s.n, none_out = p.window > 0 ? w.s.len - p.window : 0;  // every row sees entries none_out .. all_see
+    const bool mixed = w.s.n > 1 || p.window > 0;
+    auto sees = [&](int t, int h) { return t <= last[h] && (p.window == 0 || t > last[h] - p.window); };
 
-        int get = 0;
-        for (int t0 = first + tg * TS; t0 < end; t0 += groups * TS) {
-            copies_wait<STAGES - 2>();
-            group_sync();  // the stage is complete, and the one behind it has been read
-            const bool lacks = gaps >> get & 1u;
-            issue();
-            const uint32_t stage = ring + get * MMA_STAGE;
-            get = get + 1 == STAGES ? 0 : get + 1;
-            // scores s[n][row half * 2 + column] of entries t0 + 8 n + 2 c + column
-            float s[TS / 8][4];
+    int get = 0;
+    uint32_t phase = 0;
+    for (int t0 = first + tg * TS; t0 < end; t0 += groups * TS) {
+        arrived(get, 0, phase);
+        group_sync();  // K is there, and V of the step before has been read
+        issue_v();
+        const bool lacks = gaps >> get & 1u;
+        const uint32_t stage = ring + get * MMA_STAGE;
+        // scores s[n][row half * 2 + column] of entries t0 + 8 n + 2 c + column; operands in two batches, each with sums of its own
+        float s[TS / 8][4], s2[TS / 8][4];
 #pragma unroll
-            for (int n = 0; n < TS / 8; ++n)
+        for (int n = 0; n < TS / 8; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+            for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint32_t a[NQ][4];
+        for (int kb = 0; kb < 2; ++kb) {
+            constexpr int KB = KS / 2;
+            const uint32_t at = stage + k_at;
+            uint32_t a[KB][NQ][4], k[KB][HALVES][4];
+#pragma unroll
+            for (int i = 0; i < KB; ++i) {
+                const int ks = kb * KB + i;
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) ldsm(k[i][h], (at ^ ((ks & 3) << 5)) + box_of(ks, h));
 #pragma unroll
                 for (int part = 0; part < NQ; ++part) {
                     const uint4 x = q4[(part * KS + ks) * 32];
-                    a[part][0] = x.x; a[part][1] = x.y; a[part][2] = x.z; a[part][3] = x.w;
-                }
-#pragma unroll
-                for (int h = 0; h < HALVES; ++h) {
-                    uint32_t k[4];
-                    ldsm(k, stage + h * 16 * HD * 2 + k_at + (((ks * 2 + (mj & 1)) ^ mr) << 4));
-#pragma unroll
-                    for (int part = NQ - 1; part >= 0; --part) {
-                        X::mma(s[2 * h], a[part], k[0], k[1]);
-                        X::mma(s[2 * h + 1], a[part], k[2], k[3]);
-                    }
+                    a[i][part][0] = x.x; a[i][part][1] = x.y; a[i][part][2] = x.z; a[i][part][3] = x.w;
                 }
             }
-            const bool masked = t0 + TS - 1 > all_see || t0 < none_out || t0 + TS > end || lacks;
-            if (masked)
 #pragma unroll
-                for (int n = 0; n < TS / 8; ++n)
+            for (int i = 0; i < KB; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int t = t0 + n * 8 + 2 * c + (e & 1);
-                        if (!(sees(t, e >> 1) && t < end && (!lacks || page_at(p.c, b, t) >= 0))) s[n][e] = -INFINITY;
+                for (int part = NQ - 1; part >= 0; --part)
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) {
+                        product<KT>(kb ? s2[2 * h] : s[2 * h], a[i][part], k[i][h][0], k[i][h][1]);
+                        product<KT>(kb ? s2[2 * h + 1] : s[2 * h + 1], a[i][part], k[i][h][2], k[i][h][3]);
                     }
-            if (p.scores)
+        }
 #pragma unroll
-                for (int n = 0; n < TS / 8; ++n)
+        for (int n = 0; n < TS / 8; ++n)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int t = t0 + n * 8 + 2 * c;
-                        if (srow[h] && t + 1 < end) *reinterpret_cast<float2*>(srow[h] + t) = make_float2(s[n][2 * h] * scale[h], s[n][2 * h + 1] * scale[h]);
-                        else if (srow[h] && t < end) srow[h][t] = s[n][2 * h] * scale[h];
-                    }
-            float top[2];
-            bool raise = false;
+            for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+        const bool masked = t0 + TS - 1 > all_see || t0 < none_out || t0 + TS > end || lacks;
+        if (masked)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float x = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+            for (int n = 0; n < TS / 8; ++n)
 #pragma unroll
-                for (int n = 1; n < TS / 8; ++n) x = fmaxf(x, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                top[h] = fmaxf(m[h], x * scale[h]);  // (scale is positive)
-                raise |= top[h] > m[h];
-            }
-            if (__any_sync(0xffffffffu, raise)) {
+                for (int e = 0; e < 4; ++e) {
+                    const int t = t0 + n * 8 + 2 * c + (e & 1);
+                    if (!(sees(t, e >> 1) && t < end && (!lacks || page_at(p.c, b, t) >= 0))) s[n][e] = -INFINITY;
+                }
+        if (p.scores)
+#pragma unroll
+            for (int n = 0; n < TS / 8; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float f = top[h] == -INFINITY ? 1.f : ex2(m[h] - top[h]);
-                    m[h] = top[h];
-                    l[h] *= f;
-#pragma unroll
-                    for (int n = 0; n < CH; ++n) {
-                        o[n][2 * h] *= f;
-                        o[n][2 * h + 1] *= f;
-                    }
+                    const int t = t0 + n * 8 + 2 * c;
+                    if (srow[h] && t + 1 < end) *reinterpret_cast<float2*>(srow[h] + t) = make_float2(s[n][2 * h] * scale[h], s[n][2 * h + 1] * scale[h]);
+                    else if (srow[h] && t < end) srow[h][t] = s[n][2 * h] * scale[h];
                 }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float base = (m[h] == -INFINITY ? 0.f : m[h]) - (float)F::SHIFT;
-#pragma unroll
-                for (int n = 0; n < TS / 8; ++n) {
-                    s[n][2 * h] = ex2(fmaf(s[n][2 * h], scale[h], -base));
-                    s[n][2 * h + 1] = ex2(fmaf(s[n][2 * h + 1], scale[h], -base));
-                    l[h] += s[n][2 * h] + s[n][2 * h + 1];
-                }
-            }
-            if (masked && mixed) {  // what some rows do not see must not reach them through 0 * inf
-                const uint32_t* v = reinterpret_cast<const uint32_t*>(ring_all) + ((stage - ring_base) + TS * HD * 2) / 4;
-                bool odd = false;
-                for (int at = lane; at < TS * HD / 2; at += 32) odd |= not_finite<KT>(v[at]);
-                if (__any_sync(0xffffffffu, odd)) {  // rare: what is not finite goes, entry by entry, to the rows that see it
-#pragma unroll 1
-                    for (int at = 0; at < TS; ++at) {
-                        const int t = t0 + at, from = (lane & ~3) | (at & 7) >> 1;
-                        float e0 = 0.f, e1 = 0.f;
-#pragma unroll
-                        for (int n = 0; n < TS / 8; ++n)
-                            if (at >> 3 == n) {
-                                e0 = at & 1 ? s[n][1] : s[n][0];
-                                e1 = at & 1 ? s[n][3] : s[n][2];
-                            }
-                        e0 = __shfl_sync(0xffffffffu, e0, from);
-                        e1 = __shfl_sync(0xffffffffu, e1, from);
-                        if (t >= end) continue;
-                        const bool see0 = sees(t, 0), see1 = sees(t, 1);
-#pragma unroll
-                        for (int n = 0; n < CH; ++n) {
-                            const uint32_t word = v[at * HD / 2 + ((n ^ (at & 7)) << 2) + c];
-                            if (!not_finite<KT>(word)) continue;
-                            const float v0 = as_float(reinterpret_cast<const KT*>(&word)[0]), v1 = as_float(reinterpret_cast<const KT*>(&word)[1]);
-                            if (!isfinite(v0)) {
-                                if (see0) o[n][0] = fmaf(e0, v0, o[n][0]);
-                                if (see1) o[n][2] = fmaf(e1, v0, o[n][2]);
-                            }
-                            if (!isfinite(v1)) {
-                                if (see0) o[n][1] = fmaf(e0, v1, o[n][1]);
-                                if (see1) o[n][3] = fmaf(e1, v1, o[n][3]);
-                            }
-                        }
-                    }
-                    group_sync();  // the group's warps have all read the stage: take what is not finite out of it
-                    uint32_t* clean = const_cast<uint32_t*>(v);
-                    for (int at = gt; at < TS * HD / 2; at += gsize) clean[at] = finite_part<KT>(clean[at]);
-                    group_sync();
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h) {
-                uint32_t pp[NP][4];
-#pragma unroll
-                for (int part = 0; part < NP; ++part) {
-                    pp[part][0] = take_part<KT>(s[2 * h][0], s[2 * h][1]);
-                    pp[part][1] = take_part<KT>(s[2 * h][2], s[2 * h][3]);
-                    pp[part][2] = take_part<KT>(s[2 * h + 1][0], s[2 * h + 1][1]);
-                    pp[part][3] = take_part<KT>(s[2 * h + 1][2], s[2 * h + 1][3]);
-                }
-#pragma unroll
-                for (int n = 0; n < CH; n += 2) {
-                    uint32_t v[4];
-                    ldsm_t(v, stage + h * 16 * HD * 2 + v_at + (((n + (mj >> 1)) ^ mr) << 4));
-                    if constexpr (F::WIDE) {
-                        float f0[4] = {0.f, 0.f, 0.f, 0.f}, f1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int part = NP - 1; part >= 0; --part) {
-                            X::mma(f0, pp[part], v[0], v[1]);
-                            X::mma(f1, pp[part], v[2], v[3]);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            o[n][e] += f0[e];
-                            o[n + 1][e] += f1[e];
-                        }
-                    } else {
-#pragma unroll
-                        for (int part = NP - 1; part >= 0; --part) {
-                            X::mma(o[n], pp[part], v[0], v[1]);
-                            X::mma(o[n + 1], pp[part], v[2], v[3]);
-                        }
-                    }
-                }
-            }
-        }
-        copies_wait<0>();
-        __syncthreads();  // the ring is empty; its place takes the parts
-        constexpr float DOWN = 1.0f / (1 << F::SHIFT);
+        float top[2];
+        bool raise = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            const int r = warp * RW + g + 8 * h;
-            if (c == 0) sml[r] = make_float2(m[h], l[h] * DOWN);
+            float x = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
 #pragma unroll
-            for (int n = 0; n < CH; ++n)
-                *reinterpret_cast<float2*>(so + (size_t)r * (HD + PAD) + n * 8 + 2 * c) = make_float2(o[n][2 * h] * DOWN, o[n][2 * h + 1] * DOWN);
+            for (int n = 1; n < TS / 8; ++n) x = fmaxf(x, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            top[h] = fmaxf(m[h], x * scale[h]);  // (scale is positive)
+            raise |= top[h] > m[h];
         }
-        __syncthreads();
-        finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sml}, RW, w, kvh, block, whole, slot);
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float f = top[h] == -INFINITY ? 1.f : ex2(m[h] - top[h]);
+                m[h] = top[h];
+                l[h] *= f;
+#pragma unroll
+                for (int n = 0; n < CH; ++n) {
+                    o[n][2 * h] *= f;
+                    o[n][2 * h + 1] *= f;
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float base = (m[h] == -INFINITY ? 0.f : m[h]) - (float)F::SHIFT;
+#pragma unroll
+            for (int n = 0; n < TS / 8; ++n) {
+                s[n][2 * h] = ex2(fmaf(s[n][2 * h], scale[h], -base));
+                s[n][2 * h + 1] = ex2(fmaf(s[n][2 * h + 1], scale[h], -base));
+                l[h] += s[n][2 * h] + s[n][2 * h + 1];
+            }
+        }
+        arrived(get, 1, phase);
+        group_sync();  // V is there, and K has been read
+        issue_k();
+        get = get + 1 == STAGES ? 0 : get + 1;
+        phase ^= get == 0;
+        if (TMA && (t0 + TS > end || lacks)) {  // boxes are whole: rows that are not entries become zeros
+            uint32_t* v = reinterpret_cast<uint32_t*>(ring_all + (stage - ring_base) + VOFF);
+            for (int at = gt; at < TS * CH; at += gsize) {
+                const int row = at / CH, t = t0 + row;
+                if (t >= end || (lacks && page_at(p.c, b, t) < 0)) *reinterpret_cast<uint4*>(v + word_at(row, at % CH)) = make_uint4(0, 0, 0, 0);
+            }
+            async_proxy_fence();
+            group_sync();
+        }
+        if (masked && mixed) {  // what some rows do not see must not reach them through 0 * inf
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(ring_all + (stage - ring_base) + VOFF);
+            bool odd = false;
+            for (int at = lane; at < TS * HD / 2; at += 32) odd |= not_finite<KT>(v[at]);
+            if (__any_sync(0xffffffffu, odd)) {  // rare: what is not finite goes, entry by entry, to the rows that see it
+#pragma unroll 1
+                for (int at = 0; at < TS; ++at) {
+                    const int t = t0 + at, lane_of = (lane & ~3) | (at & 7) >> 1;
+                    float e0 = 0.f, e1 = 0.f;
+#pragma unroll
+                    for (int n = 0; n < TS / 8; ++n)
+                        if (at >> 3 == n) {
+                            e0 = at & 1 ? s[n][1] : s[n][0];
+                            e1 = at & 1 ? s[n][3] : s[n][2];
+                        }
+                    e0 = __shfl_sync(0xffffffffu, e0, lane_of);
+                    e1 = __shfl_sync(0xffffffffu, e1, lane_of);
+                    if (t >= end) continue;
+                    const bool see0 = sees(t, 0), see1 = sees(t, 1);
+#pragma unroll
+                    for (int n = 0; n < CH; ++n) {
+                        const uint32_t word = v[word_at(at, n) + c];
+                        if (!not_finite<KT>(word)) continue;
+                        const float v0 = as_float(reinterpret_cast<const KT*>(&word)[0]), v1 = as_float(reinterpret_cast<const KT*>(&word)[1]);
+                        if (!isfinite(v0)) {
+                            if (see0) o[n][0] = fmaf(e0, v0, o[n][0]);
+                            if (see1) o[n][2] = fmaf(e1, v0, o[n][2]);
+                        }
+                        if (!isfinite(v1)) {
+                            if (see0) o[n][1] = fmaf(e0, v1, o[n][1]);
+                            if (see1) o[n][3] = fmaf(e1, v1, o[n][3]);
+                        }
+                    }
+                }
+                group_sync();  // the group's warps have all read the stage: take what is not finite out of it
+                uint32_t* clean = const_cast<uint32_t*>(v);
+                for (int at = gt; at < TS * HD / 2; at += gsize) clean[at] = finite_part<KT>(clean[at]);
+                if (TMA) async_proxy_fence();
+                group_sync();
+            }
+        }
+        const uint32_t at = stage + v_at;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            uint32_t v[CH / 2][4], pp[NP][4];
+#pragma unroll
+            for (int n = 0; n < CH / 2; ++n) ldsm_t(v[n], (at ^ ((n & 3) << 5)) + box_of(n, h));
+#pragma unroll
+            for (int part = 0; part < NP; ++part) {
+                pp[part][0] = take_part<KT>(s[2 * h][0], s[2 * h][1]);
+                pp[part][1] = take_part<KT>(s[2 * h][2], s[2 * h][3]);
+                pp[part][2] = take_part<KT>(s[2 * h + 1][0], s[2 * h + 1][1]);
+                pp[part][3] = take_part<KT>(s[2 * h + 1][2], s[2 * h + 1][3]);
+            }
+            if constexpr (F::WIDE) {
+#pragma unroll
+                for (int n = 0; n < CH / 2; n += 2) {
+                    float f[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[i][e] = 0.f;
+#pragma unroll
+                    for (int part = NP - 1; part >= 0; --part)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) product<KT>(f[i], pp[part], v[n + i / 2][i % 2 * 2], v[n + i / 2][i % 2 * 2 + 1]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[2 * n + i][e] += f[i][e];
+                }
+            } else {
+#pragma unroll
+                for (int part = NP - 1; part >= 0; --part)
+#pragma unroll
+                    for (int n = 0; n < CH; ++n) product<KT>(o[n], pp[part], v[n / 2][n % 2 * 2], v[n / 2][n % 2 * 2 + 1]);
+            }
+        }
+    }
+    if constexpr (TMA) {  // bring every barrier back to an even phase
+        if (leader) {
+            const int steps = end > first + tg * TS ? (end - first - tg * TS + groups * TS - 1) / (groups * TS) : 0;
+#pragma unroll
+            for (int st = 0; st < STAGES; ++st)
+                if ((steps - st + STAGES - 1) / STAGES & 1 && steps > st) {
+                    mbar_arrive(bars + st * 16);
+                    mbar_arrive(bars + st * 16 + 8);
+                }
+        }
+    } else copies_wait<0>();
+    __syncthreads();  // the ring is empty; its place takes the parts
+    constexpr float DOWN = 1.0f / (1 << F::SHIFT);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const int r = warp * RW + g + 8 * h;
+        if (c == 0) sh.ml[r] = make_float2(m[h], l[h] * DOWN);
+#pragma unroll
+        for (int n = 0; n < CH; ++n)
+            *reinterpret_cast<float2*>(so + (size_t)r * (HD + PAD) + n * 8 + 2 * c) = make_float2(o[n][2 * h] * DOWN, o[n][2 * h + 1] * DOWN);
+    }
+    __syncthreads();
+    finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sh.ml}, RW, ROW_WARPS, w, kvh, block, whole, slot);
+}
+
+template <typename KT, typename QT, int HD, bool TMA>
+__global__ void __launch_bounds__(PA_THREADS, MMA_CTAS) attn_mma_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUtensorMap map) {
+    extern __shared__ char dyn[];
+    __shared__ int sums[2 * PA_WARPS];
+    __shared__ MmaShared<HD> sh;
+    constexpr size_t RING = (size_t)MMA_SLOTS * MMA_STAGE, OUT = (size_t)PA_WARPS * 16 * (HD + 4) * 4;
+    char* ring = dyn + ((1024 - (smem_addr(dyn) & 1023)) & 1023);
+    uint4* sq = reinterpret_cast<uint4*>(ring + (RING > OUT ? RING : OUT));  // [row warps][NQ][KS][32 lanes]
+    int* pre = reinterpret_cast<int*>(sq + (size_t)p.row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32);
+    const CUtensorMap* boxes = &map;
+    if (TMA && threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(boxes) : "memory");
+        for (int i = 0; i < 2 * MMA_SLOTS; ++i) mbar_init(smem_addr(&sh.bars[i]), 1);
+        mbar_fence_init();
+    }
+    pdl_launch_dependents();  // the joint's CTAs come in as these leave
+    walk_line(p, pre, sums, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
+        const int rows = min(p.ru, w.s.n * p.group - block * p.ru);
+        if (rows <= 16) mma_unit<KT, QT, HD, 1, TMA>(p, boxes, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        else if (rows <= 32) mma_unit<KT, QT, HD, 2, TMA>(p, boxes, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        else mma_unit<KT, QT, HD, 4, TMA>(p, boxes, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
     });
 }
 

@@ -39,13 +39,19 @@ __device__ inline BatchSeq batch_seq(const PagedView& c, const int* row_start, i
     return s;
 }
 __device__ inline int page_of(const PagedView& c, int entry) { return c.page_shift >= 0 ? entry >> c.page_shift : entry / c.page_tokens; }
-// The page that holds `entry` (0 <= entry < cap) of sequence b, or -1 where the table names none of the pool's.
-__device__ inline int page_at(const PagedView& c, int b, int entry) {
-    const int page = __ldg(c.page_table + b * c.table_stride + page_of(c, entry));
+// The table's word for the page that holds `entry` (0 <= entry < cap) of sequence b, and what it names: a page of the pool, or -1.
+// (Apart, so that a word can be asked for long before it is looked at.)
+__device__ inline int page_word(const PagedView& c, int b, int entry) {
+    int w;  // (volatile: the compiler leaves the load where it is written)
+    asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(w) : "l"(c.page_table + b * c.table_stride + page_of(c, entry)));
+    return w;
+}
+__device__ inline int checked_page(const PagedView& c, int page) {
     if ((unsigned)page < (unsigned)c.npages) return page;
     report(c.status, CD_STATUS_PAGE);
     return -1;
 }
+__device__ inline int page_at(const PagedView& c, int b, int entry) { return checked_page(c, page_word(c, b, entry)); }
 // Element offset of entry's row in the pool; which: 0 K, 1 V.  64 bits: a pool passes 2^31 elements.
 __device__ inline size_t row_at(const PagedView& c, int page, int which, int head, int entry, int hd) {
     const int off = entry - page_of(c, entry) * c.page_tokens;
