@@ -364,8 +364,7 @@ int cd_flash_decode_static(int dtype, int heads, int kv_heads, int hd, size_t at
  * Row j of n is entry lens[b] - n + j.  Rows from row_start[nseq] on are not touched. */
 enum { CD_STATUS_BATCH = 1,   /* row_start not ascending, past nrows or max_rows, or lens outside the page table: the sequence is left out */
        CD_STATUS_PAGE = 2,    /* a page id outside the pool: its entries are not written, or count as masked */
-       CD_STATUS_LOGITS = 4,  /* a logit row that was needed holds NaN or has no finite maximum */
-       CD_STATUS_WAIT = 8 };  /* a bounded wait for a copy ran out: the call's results are void */
+       CD_STATUS_LOGITS = 4 };/* a logit row that was needed holds NaN or has no finite maximum */
 
 typedef struct cd_paged_cache {
     int32_t dtype;        /* of the pool: CD_DTYPE_F32 / F16 / BF16 */

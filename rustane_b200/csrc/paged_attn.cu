@@ -52,25 +52,6 @@ int check_shape(const cd_paged_cache* c, int heads, int nrows, int max_rows, int
     return CD_OK;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult res;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) return nullptr;
-    return (EncodeTiledFn)fn;
-}
-// The pool as {column, row of a page, head of K then of V, page}, in boxes of 64 columns and sixteen rows.  false: by cp.async then.
-bool encode_pool(CUtensorMap* map, const PagedView& c, bool f16, int hd) {
-    static const EncodeTiledFn encode = encode_fn();
-    if (!encode) return false;
-    const cuuint64_t row = (cuuint64_t)hd * 2, head = row * c.page_tokens, page = head * 2 * c.kv_heads;
-    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)c.page_tokens, (cuuint64_t)2 * c.kv_heads, (cuuint64_t)c.npages}, strides[3] = {row, head, page};
-    const cuuint32_t box[4] = {64, 16, 1, 1}, step[4] = {1, 1, 1, 1};
-    return encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, c.pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a, const Plan& plan, int collect, cudaStream_t s) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -79,12 +60,9 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     if constexpr (std::is_same<KT, float>::value) {
         attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);
     } else {
-        CUtensorMap map = {};
-        bool tma = (a.c.page_tokens & 15) == 0;
-        if (tma) tma = encode_pool(&map, a.c, std::is_same<KT, __half>::value, HD);
-        void (*kernel)(AttnArgs, CUtensorMap) = tma ? attn_mma_kernel<KT, QT, HD, true> : attn_mma_kernel<KT, QT, HD, false>;
-        if ((e = allow_shared_memory((const void*)kernel)) != cudaSuccess) return e;
-        kernel<<<std::min(MMA_CTAS * sms, PA_MAX_CTAS), PA_THREADS, mma_shared<KT, QT, HD>(a.c.nseq, a.row_warps), s>>>(a, map);
+        if ((e = allow_shared_memory((const void*)attn_mma_kernel<KT, QT, HD>)) != cudaSuccess) return e;
+        const size_t shared = mma_shared<KT, QT, HD>(a.c.nseq, a.row_warps);
+        attn_mma_kernel<KT, QT, HD><<<std::min((shared > 112 * 1024 ? 1 : MMA_CTAS) * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const dim3 grid((unsigned)plan.units, (unsigned)std::min<long long>(a.ru, (long long)a.max_rows * a.group));

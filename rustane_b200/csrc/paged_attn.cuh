@@ -156,9 +156,8 @@ __device__ inline void finish_unit(const AttnArgs& p, const UnitParts<HD, PAD>& 
 
 // Walk this CTA's share of the line; work(w, b, kvh, block, first tile, tiles, whole, slot) handles a run of one unit's tiles.
 // A tile belongs to the CTA whose share its first point lies in; no share is shorter than a tile, so none is empty.
-template <typename F> __device__ inline void walk_line(const AttnArgs& p, int* pre, int* sums, F&& work) {
-    int most;
-    const int total = line_up(p, pre, sums, most), ctas = min((int)gridDim.x, max(1, total / most)), me = blockIdx.x;
+template <typename F> __device__ inline void walk_line(const AttnArgs& p, const int* pre, int total, int most, F&& work) {
+    const int ctas = min((int)gridDim.x, max(1, total / most)), me = blockIdx.x;
     if (me >= ctas || total == 0) return;
     const int per = total / ctas, more = total - per * ctas, cut = more * (per + 1);  // the first `more` shares are one longer
     auto owner = [&](int t) { return t < cut ? t / (per + 1) : more + (t - cut) / per; };
@@ -198,7 +197,9 @@ template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA
     const KT* pool = static_cast<const KT*>(p.c.pool);
 
     pdl_launch_dependents();
-    walk_line(p, pre, sums, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
+    int most;
+    const int total = line_up(p, pre, sums, most);
+    walk_line(p, pre, total, most, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
         float q[RW][NC * VEC], o[RW][NC * VEC], m[RW], l[RW];
         int last[RW];        // the last entry a row sees, -1: none
         float* srow[RW];

@@ -1,11 +1,16 @@
 // The tensor-core form of paged attention, for 16-bit pools: mma.m16n8k16 with sixteen rows of a unit per warp.
 //
 // The warps that have different rows of the same entries (one, two or four, as the unit's rows need) are a group with a ring of stages in
-// shared memory: 4 KB of K and 4 KB of V each (sixteen entries at hd 128, 32 at hd 64), as boxes of sixteen rows of 128 bytes whose
-// 16-byte chunks are exchanged by the low bits of the row (TMA's 128-byte swizzle), so that ldmatrix meets every bank once and an
-// address is one XOR.  K's half of a stage is filled again as soon as the scores are out, V's as soon as P V is.  One thread of the group issues
-// the boxes; a group of one warp meets no barrier inside the loop.  Pages whose size is no multiple of sixteen have no such
-// boxes; their rows come by cp.async, 16 bytes at a time (TMA = false): sixteen instructions a step, which took a quarter of it.
+// shared memory: 4 KB of K and 4 KB of V each (sixteen entries at hd 128, 32 at hd 64), brought by cp.async 16 bytes at a time.  K's
+// half of a stage is filled again as soon as the scores are out, V's as soon as P V is.  A row's 16-byte chunks are exchanged by the low
+// bits of its place (chunk ^ place & 7), so that ldmatrix meets every bank once and an address is one XOR.  A group of one warp meets no
+// barrier inside the loop.
+//
+// What bounds a step (two row blocks' worth of products, 2700 to 3200 cycles at eight warps an SM) is HBM where one warp has a unit's rows
+// (5.4 TB/s inside the loop), and the chain of its instructions, 5 to 9 cycles each, where four do.  Measured against this form:
+// K and V straight to registers (no ring) 130001 entries of four heads in 70 us for 61; boxes by TMA instead of cp.async, issued by a
+// group's first thread, 59 (but 317 us for 296 on the ragged batch of fp32 rows), issued by producer warps of their own 64; three CTAs of two
+// stages an SM instead of two of three 58, and the joint 6 us later, for which they leave no registers.
 //
 // mma.sync and not tcgen05: a token's unit has 1 to 16 rows, of a 64-row minimum there, and the work is bound by the bytes of K and V.
 //
@@ -14,8 +19,6 @@
 // stay in 32 bits; with an fp32 result every step's product goes to fresh accumulators and is added by the CUDA cores, which round
 // to nearest where the tensor cores cut off.
 #pragma once
-#include <cuda.h>
-
 #include "paged_attn.cuh"
 
 namespace cd {
@@ -84,134 +87,113 @@ template <typename KT, typename QT> struct MmaForm {
     static constexpr int SHIFT = F16 ? (NP == 2 ? 12 : 8) : 0;  // P is times 2^SHIFT: fp16 parts of small ones keep their digits
 };
 constexpr int MMA_STAGE = 8192;  // bytes of a stage: K, then V
-constexpr int MMA_CTAS = 2, MMA_SLOTS = 12;  // CTAs an SM, stages of a CTA, which its groups share
+// CTAs an SM, stages of a CTA, which its groups share, and registers of a thread: they leave 8192 of an SM's to the joint's CTAs
+constexpr int MMA_CTAS = 2, MMA_SLOTS = 12, MMA_REGS = 224;
 template <typename KT, typename QT, int HD> inline size_t mma_shared(int nseq, int row_warps) {
     const size_t q = (size_t)row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)MMA_SLOTS * MMA_STAGE;
     const size_t o = (size_t)PA_WARPS * 16 * (HD + 4) * 4;  // (in the ring's place once it is empty)
     return (ring > o ? ring : o) + q + (size_t)(nseq + 1) * 4 + 1024;  // (1024: the ring's own alignment)
 }
-__device__ inline void load_box(uint32_t dst, const CUtensorMap* map, int col, int row, int head, int page, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(col), "r"(row), "r"(head), "r"(page) : "memory");
-}
-__device__ inline void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 template <int HD> struct MmaShared {
     float2 ml[PA_WARPS * 16];
     float qscale[4 * 16];
-    unsigned long long bars[2 * MMA_SLOTS];  // of stage s: K at 2 s, V at 2 s + 1; at the start of a unit all are in an even phase
 };
 
 // A run of one unit's tiles, its rows on ROW_WARPS warps.
-template <typename KT, typename QT, int HD, int ROW_WARPS, bool TMA>
-__device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* map, char* ring_all, uint4* sq, MmaShared<HD>& sh, const SeqWork& w, int b, int kvh, int block, int tile, int tiles,
+template <typename KT, typename QT, int HD, int ROW_WARPS>
+__device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint4* sq, MmaShared<HD>& sh, const SeqWork& w, int b, int kvh, int block, int tile, int tiles,
                                          bool whole, size_t slot) {
     using X = Mma16<KT>;
     using F = MmaForm<KT, QT>;
     constexpr int NQ = F::NQ, NP = F::NP, RW = 16, PAD = 4, TS = MMA_STAGE / 4 / HD, CH = HD / 8, KS = HD / 16, HALVES = TS / 16;  // TS: entries of a stage
     constexpr int groups = PA_WARPS / ROW_WARPS, gsize = ROW_WARPS * 32, STAGES = MMA_SLOTS / groups < 4 ? MMA_SLOTS / groups : 4;
-    constexpr int PASS = gsize / CH, PASSES = TS / PASS, VOFF = MMA_STAGE / 2, BOX = 2048;  // PASS: rows that one copy of the whole group brings
+    constexpr int PASS = gsize / CH, PASSES = TS / PASS, VOFF = MMA_STAGE / 2;  // PASS: rows that one copy of the whole group brings
     float* so = reinterpret_cast<float*>(ring_all);  // [warps][RW][HD + PAD]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int rw = warp % ROW_WARPS, tg = warp / ROW_WARPS, gt = rw * 32 + lane;
     const uint32_t ring_base = (uint32_t)__cvta_generic_to_shared(ring_all), ring = ring_base + tg * STAGES * MMA_STAGE;
     const KT* pool = static_cast<const KT*>(p.c.pool);
-    const size_t v_off = (size_t)p.c.kv_heads * p.c.page_tokens * HD;
+    const bool page16 = (p.c.page_tokens & 15) == 0;
+    const size_t v_off = (size_t)p.c.kv_heads * p.c.page_tokens * HD, page_step = 2 * v_off;
     auto group_sync = [&]() {
         if constexpr (ROW_WARPS == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(tg + 1), "r"(gsize) : "memory");
     };
     // ldmatrix: lane l points at row l % 8 of matrix l / 8; a chunk's place is XORed in
     const int mr = lane & 7, mj = lane >> 3;
-    const uint32_t k_at = (uint32_t)((mj >> 1) * 8 + mr) * 128 + (((mj & 1) ^ mr) << 4), v_at = (uint32_t)((mj & 1) * 8 + mr) * 128 + VOFF + (((mj >> 1) ^ mr) << 4);
-    auto box_of = [](int pair, int half) { return HD == 128 ? pair / 4 * BOX : half * BOX; };  // of 32 bytes `pair` of a row, entries 16 half ..
-    auto word_at = [](int row, int chunk) { return (HD == 128 ? chunk / 8 * BOX : 0) / 4 + row * 32 + (((chunk & 7) ^ (row & 7)) << 2); };  // 32-bit words
+    const uint32_t k_at = (uint32_t)((mj >> 1) * 8 + mr) * HD * 2 + (((mj & 1) ^ mr) << 4), v_at = (uint32_t)((mj & 1) * 8 + mr) * HD * 2 + VOFF + (((mj >> 1) ^ mr) << 4);
 
     const int valid_rows = min(p.ru, w.s.n * p.group - block * p.ru);
     const int first = w.start + tile * PA_TILE, end = min(w.s.len, first + tiles * PA_TILE);
-    if (TMA) async_proxy_fence();  // (what was written over the ring comes before the copies into it)
-    __syncthreads();               // the unit before has been read
+    __syncthreads();  // the unit before has been read
     // ---- the ring: page ids are looked up a step ahead of the copies
-    const bool leader = TMA && rw == 0 && lane == 0;
-    const uint32_t bars = smem_addr(sh.bars) + tg * STAGES * 16;
     int pages[HALVES];
     auto look_up = [&](int t0) {
-        if (TMA)
+        if (page16)
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) pages[h] = t0 + 16 * h < end ? page_word(p.c, b, t0 + 16 * h) : 0;
     };
     uint32_t gaps = 0;                                           // bit s: stage s lacks a page
-    int next = first + tg * TS, put = 0;                         // the step whose K is next, its stage
-    int now_page[HALVES], now_off[HALVES];                       // of the stage whose V is next
-    uint32_t has = 0;                                            // bit k: this thread's row of pass k is there
-    const KT* from[TMA ? 1 : PASSES];
     const int row0 = gt / CH, ch = gt % CH;                      // this thread's place in a pass
+    const uint32_t put_at = ring + row0 * HD * 2 + ((ch ^ (row0 & 7)) << 4);
+    const KT* head_at = pool + (size_t)kvh * p.c.page_tokens * HD + row0 * HD + ch * 8;
+    int next = first + tg * TS, put = 0;                         // the step whose K is next, its stage
+    const KT* from[HALVES];                                      // rows of the stage whose V is next: of each page
+    uint32_t has = 0;                                            // bit k: this thread's row of pass k is there
+    int odd_page = -1;                                           // (pages of odd sizes: of row `lane`)
     auto copy_half = [&](int half) {                             // 0: K, 1: V of the stage that `put` and the above describe
-        if constexpr (TMA) {
-            if (leader) {
-                const uint32_t to = ring + put * MMA_STAGE + half * VOFF, bar = bars + put * 16 + half * 8;
-                int boxes = 0;
+        const uint32_t to = put_at + put * MMA_STAGE + half * VOFF;
+        const size_t off = half ? v_off : 0;
+        constexpr uint32_t ALL = (1u << PASSES) - 1;
+        if (page16 && has == ALL) {
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) boxes += now_page[h] >= 0 ? HD / 64 : 0;
-                mbar_arrive_expect_tx(bar, boxes * BOX);
-#pragma unroll
-                for (int h = 0; h < HALVES; ++h)
-                    if (now_page[h] >= 0)
-#pragma unroll
-                        for (int j = 0; j < HD / 64; ++j) load_box(to + (HD == 128 ? j : h) * BOX, map, j * 64, now_off[h], half * p.c.kv_heads + kvh, now_page[h], bar);
-            }
-        } else {
-            const size_t off = half ? v_off : 0;
+            for (int k = 0; k < PASSES; ++k) copy16((to ^ ((k * PASS & 7) << 4)) + k * PASS * HD * 2, from[k * PASS / 16] + off + k * PASS % 16 * HD, true);
+        } else if (page16) {
 #pragma unroll
             for (int k = 0; k < PASSES; ++k) {
                 const bool there = has >> k & 1u;
-                copy16(ring + put * MMA_STAGE + half * VOFF + word_at(row0 + k * PASS, ch) * 4, there ? from[k] + off : pool, there);
+                copy16((to ^ ((k * PASS & 7) << 4)) + k * PASS * HD * 2, there ? from[k * PASS / 16] + off + k * PASS % 16 * HD : pool, there);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < PASSES; ++k) {
+                const int row = row0 + k * PASS, pg = __shfl_sync(0xffffffffu, odd_page, row);
+                copy16((to ^ ((k * PASS & 7) << 4)) + k * PASS * HD * 2, pg >= 0 ? pool + row_at(p.c, pg, 0, kvh, next + row, HD) + off + ch * 8 : pool, pg >= 0);
             }
         }
     };
     auto issue_k = [&]() {
         if (next < end) {
             bool lacks = false;
-            if constexpr (TMA) {
+            if (page16) {
+                has = 0;
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
-                    const int t = next + 16 * h;
-                    now_page[h] = t < end ? checked_page(p.c, pages[h]) : -1;
-                    now_off[h] = p.c.page_shift >= 0 ? t & (p.c.page_tokens - 1) : t % p.c.page_tokens;
-                    lacks |= now_page[h] < 0 && t < end;
+                    const int t = next + 16 * h, off = p.c.page_shift >= 0 ? t & (p.c.page_tokens - 1) : t % p.c.page_tokens;
+                    pages[h] = t < end ? checked_page(p.c, pages[h]) : -1;
+                    from[h] = head_at + (size_t)max(pages[h], 0) * page_step + off * HD;
+                    lacks |= pages[h] < 0 && t < end;
                 }
+                if (next + TS <= end && !lacks) has = (1u << PASSES) - 1;
+                else
+#pragma unroll
+                    for (int k = 0; k < PASSES; ++k) has |= (uint32_t)(pages[k * PASS / 16] >= 0 && next + row0 + k * PASS < end) << k;
                 look_up(next + groups * TS);
             } else {  // lane r looks up row r (every warp of the group all of them: they agree on gaps)
                 const bool in = lane < TS && next + lane < end;
-                const int mine = in ? page_at(p.c, b, next + lane) : -1;
-                lacks = __any_sync(0xffffffffu, in && mine < 0);
-                has = 0;
-#pragma unroll
-                for (int k = 0; k < PASSES; ++k) {
-                    const int row = row0 + k * PASS, pg = __shfl_sync(0xffffffffu, mine, row);
-                    from[k] = pool + (pg >= 0 ? row_at(p.c, pg, 0, kvh, next + row, HD) + ch * 8 : 0);
-                    has |= (uint32_t)(pg >= 0) << k;
-                }
+                odd_page = in ? page_at(p.c, b, next + lane) : -1;
+                lacks = __any_sync(0xffffffffu, in && odd_page < 0);
             }
             gaps = (gaps & ~(1u << put)) | (uint32_t)lacks << put;
             copy_half(0);
         }
-        if (!TMA) copies_close();
+        copies_close();
     };
     auto issue_v = [&]() {
         if (next < end) copy_half(1);
         next += groups * TS;
         put = put + 1 == STAGES ? 0 : put + 1;
-        if (!TMA) copies_close();
-    };
-    bool lost = false;
-    auto arrived = [&](int stage, int half, uint32_t phase) {
-        if constexpr (TMA) {
-            if (!lost && !mbar_wait(bars + stage * 16 + half * 8, phase)) {  // (bounded: a copy that never lands is reported, not waited for again)
-                lost = true;
-                report(p.c.status, CD_STATUS_WAIT);
-            }
-        } else copies_wait<2 * STAGES - 2>();
+        copies_close();
     };
     look_up(next);
     // q is asked for ahead of the copies, which would otherwise be served first
@@ -284,29 +266,28 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* m
     auto sees = [&](int t, int h) { return t <= last[h] && (p.window == 0 || t > last[h] - p.window); };
 
     int get = 0;
-    uint32_t phase = 0;
     for (int t0 = first + tg * TS; t0 < end; t0 += groups * TS) {
-        arrived(get, 0, phase);
+        copies_wait<2 * STAGES - 2>();
         group_sync();  // K is there, and V of the step before has been read
         issue_v();
         const bool lacks = gaps >> get & 1u;
         const uint32_t stage = ring + get * MMA_STAGE;
-        // scores s[n][row half * 2 + column] of entries t0 + 8 n + 2 c + column; operands in two batches, each with sums of its own
+        // scores s[n][row half * 2 + column] of entries t0 + 8 n + 2 c + column; two k-steps' operands at a time, into two sets of sums in turn
         float s[TS / 8][4], s2[TS / 8][4];
 #pragma unroll
         for (int n = 0; n < TS / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            constexpr int KB = KS / 2;
+        for (int kb = 0; kb < KS / 2; ++kb) {
+            constexpr int KB = 2;
             const uint32_t at = stage + k_at;
             uint32_t a[KB][NQ][4], k[KB][HALVES][4];
 #pragma unroll
             for (int i = 0; i < KB; ++i) {
                 const int ks = kb * KB + i;
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) ldsm(k[i][h], (at ^ ((ks & 3) << 5)) + box_of(ks, h));
+                for (int h = 0; h < HALVES; ++h) ldsm(k[i][h], (at ^ (ks << 5)) + h * 16 * HD * 2);
 #pragma unroll
                 for (int part = 0; part < NQ; ++part) {
                     const uint4 x = q4[(part * KS + ks) * 32];
@@ -319,8 +300,8 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* m
                 for (int part = NQ - 1; part >= 0; --part)
 #pragma unroll
                     for (int h = 0; h < HALVES; ++h) {
-                        product<KT>(kb ? s2[2 * h] : s[2 * h], a[i][part], k[i][h][0], k[i][h][1]);
-                        product<KT>(kb ? s2[2 * h + 1] : s[2 * h + 1], a[i][part], k[i][h][2], k[i][h][3]);
+                        product<KT>(kb & 1 ? s2[2 * h] : s[2 * h], a[i][part], k[i][h][0], k[i][h][1]);
+                        product<KT>(kb & 1 ? s2[2 * h + 1] : s[2 * h + 1], a[i][part], k[i][h][2], k[i][h][3]);
                     }
         }
 #pragma unroll
@@ -380,20 +361,10 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* m
                 l[h] += s[n][2 * h] + s[n][2 * h + 1];
             }
         }
-        arrived(get, 1, phase);
+        copies_wait<2 * STAGES - 2>();
         group_sync();  // V is there, and K has been read
         issue_k();
         get = get + 1 == STAGES ? 0 : get + 1;
-        phase ^= get == 0;
-        if (TMA && (t0 + TS > end || lacks)) {  // boxes are whole: rows that are not entries become zeros
-            uint32_t* v = reinterpret_cast<uint32_t*>(ring_all + (stage - ring_base) + VOFF);
-            for (int at = gt; at < TS * CH; at += gsize) {
-                const int row = at / CH, t = t0 + row;
-                if (t >= end || (lacks && page_at(p.c, b, t) < 0)) *reinterpret_cast<uint4*>(v + word_at(row, at % CH)) = make_uint4(0, 0, 0, 0);
-            }
-            async_proxy_fence();
-            group_sync();
-        }
         if (masked && mixed) {  // what some rows do not see must not reach them through 0 * inf
             const uint32_t* v = reinterpret_cast<const uint32_t*>(ring_all + (stage - ring_base) + VOFF);
             bool odd = false;
@@ -415,7 +386,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* m
                     const bool see0 = sees(t, 0), see1 = sees(t, 1);
 #pragma unroll
                     for (int n = 0; n < CH; ++n) {
-                        const uint32_t word = v[word_at(at, n) + c];
+                        const uint32_t word = v[at * HD / 2 + ((n ^ (at & 7)) << 2) + c];
                         if (!not_finite<KT>(word)) continue;
                         const float v0 = as_float(reinterpret_cast<const KT*>(&word)[0]), v1 = as_float(reinterpret_cast<const KT*>(&word)[1]);
                         if (!isfinite(v0)) {
@@ -431,16 +402,13 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* m
                 group_sync();  // the group's warps have all read the stage: take what is not finite out of it
                 uint32_t* clean = const_cast<uint32_t*>(v);
                 for (int at = gt; at < TS * HD / 2; at += gsize) clean[at] = finite_part<KT>(clean[at]);
-                if (TMA) async_proxy_fence();
                 group_sync();
             }
         }
         const uint32_t at = stage + v_at;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-            uint32_t v[CH / 2][4], pp[NP][4];
-#pragma unroll
-            for (int n = 0; n < CH / 2; ++n) ldsm_t(v[n], (at ^ ((n & 3) << 5)) + box_of(n, h));
+            uint32_t pp[NP][4];
 #pragma unroll
             for (int part = 0; part < NP; ++part) {
                 pp[part][0] = take_part<KT>(s[2 * h][0], s[2 * h][1]);
@@ -448,42 +416,38 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* m
                 pp[part][2] = take_part<KT>(s[2 * h + 1][0], s[2 * h + 1][1]);
                 pp[part][3] = take_part<KT>(s[2 * h + 1][2], s[2 * h + 1][3]);
             }
-            if constexpr (F::WIDE) {
 #pragma unroll
-                for (int n = 0; n < CH / 2; n += 2) {
-                    float f[4][4];
+            for (int nb = 0; nb < CH / 2; nb += 4) {  // 64 columns
+                uint32_t v[4][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                for (int n = 0; n < 4; ++n) ldsm_t(v[n], (at ^ ((nb + n) << 5)) + h * 16 * HD * 2);
+                if constexpr (F::WIDE) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) f[i][e] = 0.f;
+                    for (int n = 0; n < 4; n += 2) {
+                        float f[4][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) f[i][e] = 0.f;
+#pragma unroll
+                        for (int part = NP - 1; part >= 0; --part)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) product<KT>(f[i], pp[part], v[n + i / 2][i % 2 * 2], v[n + i / 2][i % 2 * 2 + 1]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[2 * (nb + n) + i][e] += f[i][e];
+                    }
+                } else {
 #pragma unroll
                     for (int part = NP - 1; part >= 0; --part)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) product<KT>(f[i], pp[part], v[n + i / 2][i % 2 * 2], v[n + i / 2][i % 2 * 2 + 1]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[2 * n + i][e] += f[i][e];
+                        for (int n = 0; n < 8; ++n) product<KT>(o[2 * nb + n], pp[part], v[n / 2][n % 2 * 2], v[n / 2][n % 2 * 2 + 1]);
                 }
-            } else {
-#pragma unroll
-                for (int part = NP - 1; part >= 0; --part)
-#pragma unroll
-                    for (int n = 0; n < CH; ++n) product<KT>(o[n], pp[part], v[n / 2][n % 2 * 2], v[n / 2][n % 2 * 2 + 1]);
             }
         }
     }
-    if constexpr (TMA) {  // bring every barrier back to an even phase
-        if (leader) {
-            const int steps = end > first + tg * TS ? (end - first - tg * TS + groups * TS - 1) / (groups * TS) : 0;
-#pragma unroll
-            for (int st = 0; st < STAGES; ++st)
-                if ((steps - st + STAGES - 1) / STAGES & 1 && steps > st) {
-                    mbar_arrive(bars + st * 16);
-                    mbar_arrive(bars + st * 16 + 8);
-                }
-        }
-    } else copies_wait<0>();
+    copies_wait<0>();
     __syncthreads();  // the ring is empty; its place takes the parts
     constexpr float DOWN = 1.0f / (1 << F::SHIFT);
 #pragma unroll
@@ -500,8 +464,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, const CUtensorMap* m
     finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sh.ml}, RW, ROW_WARPS, w, kvh, block, whole, slot);
 }
 
-template <typename KT, typename QT, int HD, bool TMA>
-__global__ void __launch_bounds__(PA_THREADS, MMA_CTAS) attn_mma_kernel(const __grid_constant__ AttnArgs p, const __grid_constant__ CUtensorMap map) {
+template <typename KT, typename QT, int HD> __global__ void __maxnreg__(MMA_REGS) attn_mma_kernel(const __grid_constant__ AttnArgs p) {
     extern __shared__ char dyn[];
     __shared__ int sums[2 * PA_WARPS];
     __shared__ MmaShared<HD> sh;
@@ -509,18 +472,14 @@ __global__ void __launch_bounds__(PA_THREADS, MMA_CTAS) attn_mma_kernel(const __
     char* ring = dyn + ((1024 - (smem_addr(dyn) & 1023)) & 1023);
     uint4* sq = reinterpret_cast<uint4*>(ring + (RING > OUT ? RING : OUT));  // [row warps][NQ][KS][32 lanes]
     int* pre = reinterpret_cast<int*>(sq + (size_t)p.row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32);
-    const CUtensorMap* boxes = &map;
-    if (TMA && threadIdx.x == 0) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(boxes) : "memory");
-        for (int i = 0; i < 2 * MMA_SLOTS; ++i) mbar_init(smem_addr(&sh.bars[i]), 1);
-        mbar_fence_init();
-    }
-    pdl_launch_dependents();  // the joint's CTAs come in as these leave
-    walk_line(p, pre, sums, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
+    pdl_launch_dependents();  // the joint's CTAs come in beside these
+    int most;
+    const int total = line_up(p, pre, sums, most);
+    walk_line(p, pre, total, most, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
         const int rows = min(p.ru, w.s.n * p.group - block * p.ru);
-        if (rows <= 16) mma_unit<KT, QT, HD, 1, TMA>(p, boxes, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
-        else if (rows <= 32) mma_unit<KT, QT, HD, 2, TMA>(p, boxes, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
-        else mma_unit<KT, QT, HD, 4, TMA>(p, boxes, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        if (rows <= 16) mma_unit<KT, QT, HD, 1>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        else if (rows <= 32) mma_unit<KT, QT, HD, 2>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        else mma_unit<KT, QT, HD, 4>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
     });
 }
 
