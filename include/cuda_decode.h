@@ -424,7 +424,8 @@ int cd_paged_attention(const cd_paged_cache* cache, int dtype, int heads, int nr
  * the one in the lower place; NaN counts as the lightest.  Kept entries that lie in places from `keep` on move into the places that
  * fell free below, in order; the others stay where they are.  K and V move in the pool, so its pages must not be shared between
  * sequences; lens_out [nseq], weight_out and position_out (shaped as the cache's, and may be those) receive the bookkeeping, places
- * from the new length on as they were.  lens_out must not be lens.  Entries of a page outside the pool do not move (CD_STATUS_PAGE). */
+ * from the new length on as they were.  lens_out must not be lens.
+ * max_pages * page_tokens <= 2^30, nseq * kv_heads <= 65535.  Entries of a page outside the pool do not move (CD_STATUS_PAGE). */
 int cd_cache_evict_workspace(const cd_paged_cache* cache, int keep, size_t* bytes);
 int cd_cache_evict(const cd_paged_cache* cache, int keep, int sinks, int recent, int32_t* lens_out, float* weight_out, int32_t* position_out,
                    void* workspace, size_t workspace_bytes, void* stream);

@@ -37,8 +37,8 @@ __device__ inline uint32_t weight_key(float w) {
 }
 
 struct Shared {
-    uint32_t hist[EV_BINS];
-    int warp_sums[EV_WARPS], warp_sums2[EV_WARPS];
+    alignas(16) uint32_t hist[EV_BINS];
+    alignas(16) int warp_sums[EV_WARPS], warp_sums2[EV_WARPS];
     int newest, ties, holes, sources;  // this CTA's, read by the cluster
     uint32_t bin, above;               // of the pass: the bin that holds the keep-th largest, keys above it
     int red[32];
@@ -51,12 +51,29 @@ __device__ inline int warps_before(int v, int* sums, int& total) {
     __syncthreads();
     int before = 0;
     total = 0;
-    for (int i = 0; i < EV_WARPS; ++i) {
-        if (i < warp) before += sums[i];
-        total += sums[i];
+#pragma unroll
+    for (int i = 0; i < EV_WARPS; i += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(sums + i);
+        before += (i < warp ? x.x : 0) + (i + 1 < warp ? x.y : 0) + (i + 2 < warp ? x.z : 0) + (i + 3 < warp ? x.w : 0);
+        total += x.x + x.y + x.z + x.w;
     }
     __syncthreads();
     return before;
+}
+
+// use(i, load(i)) for i = first, first + step .. below end, eight loads at a time: one after the other, each would wait for memory
+template <typename L, typename U> __device__ inline void for_batches(int first, int end, int step, L&& load, U&& use, bool any) {
+    if (!any) return;
+    constexpr int DEEP = 8;
+    for (int i = first; i < end; i += step * DEEP) {
+        decltype(load(0)) v[DEEP];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (i + d * step < end) v[d] = load(i + d * step);
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (i + d * step < end) use(i + d * step, v[d]);
+    }
 }
 
 template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const __grid_constant__ EvictArgs p) {
@@ -72,63 +89,80 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
     int* position_out = p.position_out + (size_t)unit * p.c.cap;
     const int given = p.c.lens[b], len = given < 0 || given > p.c.cap ? 0 : given, keep = p.keep;
     if (len != given) report(p.c.status, CD_STATUS_BATCH);
-    if (weight_out != weight)
-        for (int i = rank * EV_THREADS + tid; i < p.c.cap; i += size * EV_THREADS)
-            if (len <= keep || i >= keep) weight_out[i] = weight[i];  // places below: at the end, where they are not holes
-    if (position_out != position)
-        for (int i = rank * EV_THREADS + tid; i < p.c.cap; i += size * EV_THREADS)
-            if (len <= keep || i >= keep) position_out[i] = position[i];
     if (unit % p.c.kv_heads == 0 && rank == 0 && tid == 0) p.lens_out[b] = len != given ? given : min(len, keep);
+    const bool same_w = weight_out == weight, same_p = position_out == position;
     if (len <= keep || keep == 0) {
+        for_batches(rank * EV_THREADS + tid, p.c.cap, size * EV_THREADS, [&](int i) { return make_int2(__float_as_int(weight[i]), position[i]); }, [&](int i, int2 v) {
+            if (!same_w) weight_out[i] = __int_as_float(v.x);
+            if (!same_p) position_out[i] = v.y;
+        }, !same_w || !same_p);
         if (rank == 0 && tid == 0) p.counts[unit] = 0;
         return;
     }
     const int per = (len + size - 1) / size, s0 = min(len, rank * per), s1 = min(len, s0 + per), mine = s1 - s0;
+    auto sync_all = [&]() {
+        if (size == 1) __syncthreads();
+        else cluster.sync();
+    };
+    auto of_rank = [&](auto* mine_, int r) { return r == rank ? mine_ : cluster.map_shared_rank(mine_, r); };
 
-    // the newest position
+    // One pass over weights and positions: the keys as if nothing were protected, the newest position, and a copy of the
+    // bookkeeping (what a hole keeps of it the moves write over).
     int newest = INT_MIN;
-    for (int i = s0 + tid; i < s1; i += EV_THREADS) newest = max(newest, position[i]);
+    for_batches(tid, mine, EV_THREADS, [&](int i) { return make_int2(__float_as_int(weight[s0 + i]), position[s0 + i]); }, [&](int i, int2 v) {
+        if (RESIDENT) keys[i] = weight_key(__int_as_float(v.x));
+        if (!same_w) weight_out[s0 + i] = __int_as_float(v.x);
+        if (!same_p) position_out[s0 + i] = v.y;
+        newest = max(newest, v.y);
+    }, true);
+    for_batches(len + rank * EV_THREADS + tid, p.c.cap, size * EV_THREADS, [&](int i) { return make_int2(__float_as_int(weight[i]), position[i]); }, [&](int i, int2 v) {
+        if (!same_w) weight_out[i] = __int_as_float(v.x);
+        if (!same_p) position_out[i] = v.y;
+    }, !same_w || !same_p);
     newest = __reduce_max_sync(0xffffffffu, newest);
     if (lane == 0) sh.red[warp] = newest;
     __syncthreads();
-    if (tid == 0) {
-        for (int i = 1; i < EV_WARPS; ++i) newest = max(newest, sh.red[i]);
-        sh.newest = newest;
+    if (warp == 0) {
+        newest = __reduce_max_sync(0xffffffffu, lane < EV_WARPS ? sh.red[lane] : INT_MIN);
+        if (lane == 0) sh.newest = newest;
     }
-    cluster.sync();
+    sync_all();
     newest = INT_MIN;
-    for (int r = 0; r < size; ++r) newest = max(newest, *cluster.map_shared_rank(&sh.newest, r));
+#pragma unroll
+    for (int r = 0; r < EV_CLUSTER; ++r)
+        if (r < size) newest = max(newest, *of_rank(&sh.newest, r));
     const long long recent_from = (long long)newest - p.recent;
-    auto make_key = [&](int i) {
-        const int pos = position[i];
-        return pos < p.sinks || pos > recent_from ? 0xffffffffu : weight_key(weight[i]);
-    };
-    auto key = [&](int i) { return RESIDENT ? keys[i] : make_key(s0 + i); };
-    if (RESIDENT)
-        for (int i = tid; i < mine; i += EV_THREADS) keys[i] = make_key(s0 + i);
+    auto protects = [&](int pos) { return pos < p.sinks || pos > recent_from; };
+    auto key = [&](int i) { return RESIDENT ? keys[i] : protects(position[s0 + i]) ? 0xffffffffu : weight_key(weight[s0 + i]); };
+    if (RESIDENT && (p.sinks > 0 || p.recent > 0))
+        for_batches(tid, mine, EV_THREADS, [&](int i) { return position[s0 + i]; }, [&](int i, int pos) {
+            if (protects(pos)) keys[i] = 0xffffffffu;
+        }, true);
 
-    // the keep-th largest key, digit by digit; `rest`: how many of the keys with this prefix stay
+    // the keep-th largest key, digit by digit, until all keys with its digits so far stay; `rest`: how many of those do
     uint32_t prefix = 0;
     int rest = keep, bits = 32, equal = 0;
     for (int pass = 0; pass < 3; ++pass) {
         const int width = pass < 2 ? 11 : 10, bins = 1 << width, shift = bits - width;
-        for (int i = tid; i < bins; i += EV_THREADS) sh.hist[i] = 0;
+        reinterpret_cast<uint4*>(sh.hist)[tid] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         for (int i = tid; i < mine; i += EV_THREADS) {
             const uint32_t k = key(i);
             if (pass == 0 || k >> bits == prefix) atomicAdd(&sh.hist[k >> shift & (bins - 1)], 1u);
         }
-        cluster.sync();
-        // from the top: thread t has the bins below bins - 4 t (bins - 2 t in the last pass)
-        const int each = bins / EV_THREADS;
-        uint32_t count[4], sum = 0;
-        for (int j = 0; j < each; ++j) {
-            const int bin = bins - 1 - (tid * each + j);
-            uint32_t n = 0;
-            for (int r = 0; r < size; ++r) n += cluster.map_shared_rank(sh.hist, r)[bin];
-            count[j] = n;
-            sum += n;
+        sync_all();
+        // from the top: thread t has the four bins below bins - 4 t
+        const int low = bins - 4 - 4 * tid;
+        uint4 sum4 = make_uint4(0, 0, 0, 0);
+        if (low >= 0) {
+#pragma unroll
+            for (int r = 0; r < EV_CLUSTER; ++r)
+                if (r < size) {
+                    const uint4 h = *reinterpret_cast<const uint4*>(of_rank(sh.hist, r) + low);
+                    sum4.x += h.x; sum4.y += h.y; sum4.z += h.z; sum4.w += h.w;
+                }
         }
+        const uint32_t count[4] = {sum4.w, sum4.z, sum4.y, sum4.x}, sum = sum4.x + sum4.y + sum4.z + sum4.w;
         uint32_t before = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -138,21 +172,23 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
         int total;
         const uint32_t warps = (uint32_t)warps_before((int)__shfl_sync(0xffffffffu, before, 31), sh.warp_sums, total);
         before += warps - sum;
-        for (int j = 0; j < each; ++j) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
             if (before < (uint32_t)rest && before + count[j] >= (uint32_t)rest) {
-                sh.bin = bins - 1 - (tid * each + j);
+                sh.bin = low + 3 - j;
                 sh.above = before;
                 sh.red[0] = (int)count[j];
             }
             before += count[j];
         }
-        cluster.sync();  // every CTA has read the histograms, too
+        sync_all();  // every CTA has read the histograms, too
         prefix = prefix << width | sh.bin;
         rest -= (int)sh.above;
         equal = sh.red[0];
         bits = shift;
+        if (rest == equal) break;
     }
-    // `equal` keys are the threshold itself, the first `rest` of them stay
+    // `equal` keys begin with the threshold's digits, the first `rest` of them stay (fewer than all only with all digits known)
     const int chunk = (mine + EV_WARPS - 1) / EV_WARPS, w0 = min(mine, warp * chunk), w1 = min(mine, w0 + chunk);  // a warp's run of places
     const bool ties = rest < equal;
     int tie_at = 0;
@@ -161,8 +197,10 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
         for (int i = w0; i < w1; i += 32) n += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && key(min(i + lane, w1 - 1)) == prefix));
         tie_at = warps_before(n, sh.warp_sums, total);
         if (tid == 0) sh.ties = total;
-        cluster.sync();
-        for (int r = 0; r < rank; ++r) tie_at += *cluster.map_shared_rank(&sh.ties, r);
+        sync_all();
+#pragma unroll
+        for (int r = 0; r < EV_CLUSTER; ++r)
+            if (r < rank) tie_at += *of_rank(&sh.ties, r);
     }
     const uint32_t below = lane == 0 ? 0u : 0xffffffffu >> (32 - lane);
     // which stay, in order: f(place, in, stays) for 32 places at a time (without ties tie_at is 0 and `rest` all equal keys: all stay)
@@ -170,7 +208,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
         int tie = tie_at;
         for (int i = w0; i < w1; i += 32) {
             const bool in = i + lane < w1;
-            const uint32_t k = in ? key(i + lane) : 0u;
+            const uint32_t k = in ? key(i + lane) >> bits : 0u;
             const uint32_t same = __ballot_sync(0xffffffffu, in && k == prefix);
             const bool stays = in && (k > prefix || (k == prefix && tie + __popc(same & below) < rest));
             tie += __popc(same);
@@ -188,16 +226,18 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
         sh.holes = total_h;
         sh.sources = total_s;
     }
-    cluster.sync();
+    sync_all();
     int all = 0;
-    for (int r = 0; r < size; ++r) {
-        const int h = *cluster.map_shared_rank(&sh.holes, r), s = *cluster.map_shared_rank(&sh.sources, r);
-        if (r < rank) {
-            hole_at += h;
-            source_at += s;
+#pragma unroll
+    for (int r = 0; r < EV_CLUSTER; ++r)
+        if (r < size) {
+            const int h = *of_rank(&sh.holes, r), n = *of_rank(&sh.sources, r);
+            if (r < rank) {
+                hole_at += h;
+                source_at += n;
+            }
+            all += h;
         }
-        all += h;
-    }
     if (rank == 0 && tid == 0) p.counts[unit] = all;
     int *hole_list = p.holes + (size_t)unit * p.moves, *source_list = p.sources + (size_t)unit * p.moves;
     walk([&](int place, bool in, bool stays) {
@@ -207,12 +247,8 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
         if (source) source_list[source_at + __popc(ss & below)] = place;
         hole_at += __popc(hs);
         source_at += __popc(ss);
-        if (in && place < keep && stays) {
-            if (weight_out != weight) weight_out[place] = weight[place];
-            if (position_out != position) position_out[place] = position[place];
-        }
     });
-    cluster.sync();  // nobody reads this CTA's shared memory any more
+    sync_all();  // nobody reads this CTA's shared memory any more
 }
 
 // One pair a group of LANES lanes: K and V rows of LANES * 16 bytes, weight and position.
@@ -224,19 +260,49 @@ template <int LANES> __global__ void __launch_bounds__(EV_MOVE_THREADS) evict_mo
     const int *holes = p.holes + (size_t)unit * p.moves, *sources = p.sources + (size_t)unit * p.moves;
     const size_t at = (size_t)unit * p.c.cap;
     char* pool = static_cast<char*>(p.c.pool);
-#pragma unroll 4
-    for (int i = group; i < n; i += groups) {
-        const int to = __ldcg(holes + i), from = __ldcg(sources + i);
-        const int page_to = page_at(p.c, b, to), page_from = page_at(p.c, b, from);
-        if (page_to >= 0 && page_from >= 0) {
-            const uint4 k = *(reinterpret_cast<const uint4*>(pool + row_at(p.c, page_from, 0, head, from, LANES * 16)) + sub);
-            const uint4 v = *(reinterpret_cast<const uint4*>(pool + row_at(p.c, page_from, 1, head, from, LANES * 16)) + sub);
-            *(reinterpret_cast<uint4*>(pool + row_at(p.c, page_to, 0, head, to, LANES * 16)) + sub) = k;
-            *(reinterpret_cast<uint4*>(pool + row_at(p.c, page_to, 1, head, to, LANES * 16)) + sub) = v;
+    constexpr int DEEP = 4;  // pairs under way: places, then pages, then rows
+    for (int i0 = group; i0 < n; i0 += groups * DEEP) {
+        int to[DEEP], from[DEEP];
+        uint4 k[DEEP], v[DEEP];
+        float w[DEEP];
+        int pos[DEEP], page_to[DEEP];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int i = i0 + d * groups;
+            to[d] = i < n ? __ldcg(holes + i) : -1;
+            from[d] = i < n ? __ldcg(sources + i) : 0;
         }
-        const int kept = page_to >= 0 && page_from >= 0 ? from : to;
-        if (sub == 0) p.weight_out[at + to] = p.c.weight[at + kept];
-        if (sub == 1) p.position_out[at + to] = p.c.position[at + kept];
+        int word_to[DEEP], word_from[DEEP];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (to[d] >= 0) {
+                word_to[d] = page_word(p.c, b, to[d]);
+                word_from[d] = page_word(p.c, b, from[d]);
+            }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (to[d] >= 0) {
+                page_to[d] = checked_page(p.c, word_to[d]);
+                const int page_from = checked_page(p.c, word_from[d]);
+                if (page_from < 0) page_to[d] = -1;
+                if (page_to[d] >= 0) {
+                    k[d] = *(reinterpret_cast<const uint4*>(pool + row_at(p.c, page_from, 0, head, from[d], LANES * 16)) + sub);
+                    v[d] = *(reinterpret_cast<const uint4*>(pool + row_at(p.c, page_from, 1, head, from[d], LANES * 16)) + sub);
+                }
+                const int kept = page_to[d] >= 0 ? from[d] : to[d];
+                if (sub == 0) w[d] = p.c.weight[at + kept];
+                if (sub == 1) pos[d] = p.c.position[at + kept];
+            }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (to[d] >= 0) {
+                if (page_to[d] >= 0) {
+                    *(reinterpret_cast<uint4*>(pool + row_at(p.c, page_to[d], 0, head, to[d], LANES * 16)) + sub) = k[d];
+                    *(reinterpret_cast<uint4*>(pool + row_at(p.c, page_to[d], 1, head, to[d], LANES * 16)) + sub) = v[d];
+                }
+                if (sub == 0) p.weight_out[at + to[d]] = w[d];
+                if (sub == 1) p.position_out[at + to[d]] = pos[d];
+            }
     }
 }
 
@@ -258,6 +324,7 @@ int check(const cd_paged_cache* c, int keep) {
     if (int rc = check_cache(c, CALL)) return rc;
     if (!c->weight) return refuse(CD_ERR_INVALID, CALL, "the cache needs its bookkeeping (weight and position)");
     if (keep < 0) return refuse(CD_ERR_INVALID, CALL, "keep must not be negative");
+    if ((long long)c->max_pages * c->page_tokens > 1 << 30) return refuse(CD_ERR_UNSUPPORTED, CALL, "max_pages * page_tokens must not exceed 2^30");
     return CD_OK;
 }
 

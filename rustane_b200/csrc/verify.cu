@@ -19,7 +19,7 @@ using namespace cd;
 
 namespace {
 const char* CALL = "cd_verify_drafts";
-constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32, VD_CHUNKS = 32, VD_CLUSTER = 8, VD_TILE = 256, VD_VOCAB = 1 << 22;
+constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32, VD_PICK_THREADS = 512, VD_PICK_WARPS = VD_PICK_THREADS / 32, VD_CHUNKS = 32, VD_CLUSTER = 8, VD_TILE = 256, VD_VOCAB = 1 << 22;
 
 struct Part {
     float m;   // NaN: the chunk holds NaN
@@ -42,6 +42,29 @@ template <> __device__ inline float wide<float>(float v) { return v; }
 template <> __device__ inline float wide<__half>(__half v) { return __half2float(v); }
 template <> __device__ inline float wide<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// 2^x to 2^-22 of itself; 0 for -inf
+__device__ inline float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// e^x in 64 bits for x <= 0: e^x = 2^(n / 32) e^r with |r| <= ln 2 / 64, e^r by its series up to r^6 / 720 (the next term is below
+// 4e-18), 2^(j / 32) from a table of 32.  Off by some 1e-16 (and x times 2e-17); half the 64-bit operations of exp().
+__device__ inline double exp_neg(double x, const double* two_to) {
+    constexpr double ROUND = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the integer
+    const double t = fma(x, 46.166241308446828384, ROUND);  // 32 / ln 2
+    const int n = __double2loint(t);
+    const double r = fma(t - ROUND, -0.021660849392498290195, x);  // ln 2 / 32
+    double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    const double y = e * two_to[n & 31];
+    const double v = __hiloint2double(__double2hiint(y) + ((n >> 5) << 20), __double2loint(y));
+    return x > -708.0 ? v : x != x ? x : 0.0;  // (no branch: a lane's terms go through the pipe together)
+}
 __device__ inline uint4 load_once(const void* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -57,63 +80,72 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
     const int row = blockIdx.x / p.chunks, ch = blockIdx.x % p.chunks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool is_draft = row >= p.nrows;
     const int r = is_draft ? row - p.nrows : row;
+    const T* x = is_draft ? static_cast<const T*>(p.draft) + r * p.draft_stride : static_cast<const T*>(p.target) + r * p.target_stride;
+    const int head = (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T);  // elements before the first 16-byte boundary
+    const int e0 = ch == 0 ? 0 : min(p.vocab, head + ch * p.chunk), e1 = ch == p.chunks - 1 ? p.vocab : min(p.vocab, head + (ch + 1) * p.chunk);
+    const int v0 = min(e1, max(e0, head)), vecs = (e1 - v0) / VEC;
+    const uint4* body = reinterpret_cast<const uint4*>(x + v0);
+    uint4 w[DEEP];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (i + d * VD_THREADS < vecs) w[d] = load_once(body + i + d * VD_THREADS);
+    };
+    fetch(tid);
     // rows behind the last sequence, and draft rows with no draft behind them, are not looked at
     bool skip = tid == 0 && r >= p.row_start[p.nseq];
     if (is_draft)
         for (int b = tid; b < p.nseq; b += VD_THREADS) skip |= p.row_start[b + 1] - 1 == r;
     if (__syncthreads_or(skip)) return;
-    const T* x = is_draft ? static_cast<const T*>(p.draft) + r * p.draft_stride : static_cast<const T*>(p.target) + r * p.target_stride;
-    const int head = (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T);  // elements before the first 16-byte boundary
-    const int e0 = ch == 0 ? 0 : min(p.vocab, head + ch * p.chunk), e1 = ch == p.chunks - 1 ? p.vocab : min(p.vocab, head + (ch + 1) * p.chunk);
     const float scale = (float)(p.inv_t * 1.4426950408889634074);
     float m = -INFINITY, s = 0.f;
     int at = 0x7fffffff;
     bool nan = false;
-    auto take = [&](const float (&v)[VEC], int place) {
-        float top = v[0];
-        int where = 0;
-#pragma unroll
-        for (int e = 1; e < VEC; ++e)
-            if (v[e] > top) { top = v[e]; where = e; }
+    auto one = [&](int i) {  // a ragged end
+        const float v = wide(x[i]);
         if (GREEDY) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) nan |= v[e] != v[e];
-            if (top > m) { m = top; at = place + where; }
+            nan |= v != v;
+            if (v > m || (v == m && i < at)) { m = v; at = i; }
         } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) top = fmaxf(top, v[e]);
-            if (top > m) {
-                s *= exp2f((m - top) * scale);
-                m = top;
+            if (v > m) {
+                s *= ex2(m == -INFINITY ? 0.f : (m - v) * scale);
+                m = v;
             }
-            const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) s += exp2f((v[e] - base) * scale);
+            s += ex2((v - (m == -INFINITY ? 0.f : m)) * scale);
         }
     };
-    auto one = [&](int i) {  // a ragged end: the element in the first place, nothing in the others
-        float v[VEC];
-        v[0] = wide(x[i]);
-#pragma unroll
-        for (int e = 1; e < VEC; ++e) v[e] = -INFINITY;
-        take(v, i);
-    };
-    const int v0 = min(e1, max(e0, head)), vecs = (e1 - v0) / VEC;
     for (int i = e0 + tid; i < v0; i += VD_THREADS) one(i);
-    const uint4* body = reinterpret_cast<const uint4*>(x + v0);
     for (int i = tid; i < vecs; i += VD_THREADS * DEEP) {
-        uint4 w[DEEP];
+        float v[DEEP][VEC];
 #pragma unroll
         for (int d = 0; d < DEEP; ++d)
-            if (i + d * VD_THREADS < vecs) w[d] = load_once(body + i + d * VD_THREADS);
 #pragma unroll
-        for (int d = 0; d < DEEP; ++d)
-            if (i + d * VD_THREADS < vecs) {
-                float v[VEC];
+            for (int e = 0; e < VEC; ++e) v[d][e] = i + d * VD_THREADS < vecs ? wide(reinterpret_cast<const T*>(&w[d])[e]) : -INFINITY;
+        if (i + VD_THREADS * DEEP < vecs) fetch(i + VD_THREADS * DEEP);
+        if (GREEDY) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = wide(reinterpret_cast<const T*>(&w[d])[e]);
-                take(v, v0 + (i + d * VD_THREADS) * VEC);
+            for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    nan |= v[d][e] != v[d][e];
+                    if (v[d][e] > m) { m = v[d][e]; at = v0 + (i + d * VD_THREADS) * VEC + e; }
+                }
+        } else {
+            float top = m;
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) top = fmaxf(top, v[d][e]);
+            if (top > m) {
+                s *= ex2(m == -INFINITY ? 0.f : (m - top) * scale);
+                m = top;
             }
+            const float base = (m == -INFINITY ? 0.f : m);
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s += ex2((v[d][e] - base) * scale);
+        }
     }
     for (int i = v0 + vecs * VEC + tid; i < e1; i += VD_THREADS) one(i);
 
@@ -133,7 +165,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
         }
     } else {
         const float top = warp_max(m);
-        double sum = (double)s * (double)exp2f((m - (top == -INFINITY ? 0.f : top)) * scale);
+        double sum = (double)s * (double)ex2((m - (top == -INFINITY ? 0.f : top)) * scale);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) { red_m[warp] = top; red_s[warp] = sum; }
@@ -142,7 +174,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
             float all = red_m[0];
             for (int i = 1; i < VD_WARPS; ++i) all = fmaxf(all, red_m[i]);
             sum = 0.0;
-            for (int i = 0; i < VD_WARPS; ++i) sum += red_s[i] * (double)exp2f((red_m[i] - (all == -INFINITY ? 0.f : all)) * scale);
+            for (int i = 0; i < VD_WARPS; ++i) sum += red_s[i] * (double)ex2((red_m[i] - (all == -INFINITY ? 0.f : all)) * scale);
             p.parts[(size_t)row * VD_CHUNKS + ch] = Part{all, 0, sum};
         }
     }
@@ -160,8 +192,7 @@ struct RowStat {
     double z;
     __device__ bool good() const { return isfinite(m) && isfinite(z); }
 };
-// a row's chunks together (all lanes of a warp)
-template <bool GREEDY> __device__ inline RowStat row_stat(const VerifyArgs& p, int row) {
+__device__ inline Part load_part(const VerifyArgs& p, int row) {  // this lane's chunk of a row
     const int lane = threadIdx.x & 31;
     Part q{-INFINITY, 0x7fffffff, 0.0};
     if (lane < p.chunks) {
@@ -170,6 +201,10 @@ template <bool GREEDY> __device__ inline RowStat row_stat(const VerifyArgs& p, i
         q.at = __ldcg(&src->at);
         q.s = __ldcg(&src->s);
     }
+    return q;
+}
+// a row's chunks together (all lanes of a warp)
+template <bool GREEDY> __device__ inline RowStat row_stat(const VerifyArgs& p, const Part& q, const double* two_to) {
     RowStat r;
     if (GREEDY) {
         const bool nan = __any_sync(0xffffffffu, q.m != q.m);
@@ -187,7 +222,7 @@ template <bool GREEDY> __device__ inline RowStat row_stat(const VerifyArgs& p, i
     } else {
         r.m = warp_max(q.m);
         r.at = 0;
-        r.z = warp_sum_d(isfinite(r.m) ? q.s * exp(((double)q.m - (double)r.m) * p.inv_t) : NAN);
+        r.z = warp_sum_d(isfinite(r.m) ? q.s * exp_neg(((double)q.m - (double)r.m) * p.inv_t, two_to) : NAN);
     }
     return r;
 }
@@ -195,11 +230,11 @@ template <bool GREEDY> __device__ inline RowStat row_stat(const VerifyArgs& p, i
 struct PickShared {
     int first_bad, valid, at;
     double total[3];  // of this CTA: p's sum, q's sum, what is drawn from
-    double red[2][VD_WARPS];
+    double red[2][VD_PICK_WARPS];
     float pm, qm;
 };
 
-template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_constant__ VerifyArgs p) {
+template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const __grid_constant__ VerifyArgs p) {
     extern __shared__ double tiles[];  // sums of this CTA's tiles
     __shared__ PickShared sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -214,25 +249,31 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
         }
         return;
     }
+    __shared__ double two_to[32];
+    if (tid < 32) two_to[tid] = exp2((double)tid / 32.0);
     if (tid == 0) {
         sh.first_bad = n - 1;
         sh.valid = 1;
     }
     __syncthreads();
     const T *target = static_cast<const T*>(p.target), *draft = static_cast<const T*>(p.draft);
-    for (int j = warp; j < n - 1; j += VD_WARPS) {
+    for (int j = warp; j < n - 1; j += VD_PICK_WARPS) {  // (every load that does not hang on another is asked for at once)
         const int x = p.tokens[r0 + j + 1];
-        const RowStat t = row_stat<GREEDY>(p, r0 + j);
-        bool stays = t.good() && (unsigned)x < (unsigned)p.vocab;
+        const Part tp = load_part(p, r0 + j), qp = draft ? load_part(p, p.nrows + r0 + j) : Part{};
+        const float u = GREEDY ? 0.f : p.uniforms[r0 + j];
+        const bool in = (unsigned)x < (unsigned)p.vocab;
+        const float tx = in && !GREEDY ? wide(target[(r0 + j) * p.target_stride + x]) : 0.f, qx_logit = in && draft ? wide(draft[(r0 + j) * p.draft_stride + x]) : 0.f;
+        const RowStat t = row_stat<GREEDY>(p, tp, two_to);
+        bool stays = t.good() && in;
         if (GREEDY) stays = stays && t.at == x;
-        else if (stays) {
-            const double px = exp(((double)wide(target[(r0 + j) * p.target_stride + x]) - (double)t.m) * p.inv_t) / t.z;
+        else {
+            const double px = exp_neg(((double)tx - (double)t.m) * p.inv_t, two_to) / t.z;
             double qx = 1.0;
             if (draft) {
-                const RowStat q = row_stat<GREEDY>(p, p.nrows + r0 + j);
-                qx = q.good() ? exp(((double)wide(draft[(r0 + j) * p.draft_stride + x]) - (double)q.m) * p.inv_t) / q.z : NAN;
+                const RowStat q = row_stat<GREEDY>(p, qp, two_to);
+                qx = q.good() ? exp_neg(((double)qx_logit - (double)q.m) * p.inv_t, two_to) / q.z : NAN;
             }
-            stays = (double)p.uniforms[r0 + j] * qx < px;
+            stays = stays && (double)u * qx < px;
         }
         if (!stays && lane == 0) atomicMin(&sh.first_bad, j);
     }
@@ -240,14 +281,15 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
     const int end = sh.first_bad, row = r0 + end;
     const bool left = end < n - 1;  // a draft was turned down: draw from what p has over q
     if (warp == 0) {
-        const RowStat t = row_stat<GREEDY>(p, row);
+        const Part tp = load_part(p, row), qp = left && draft ? load_part(p, p.nrows + row) : Part{};
+        const RowStat t = row_stat<GREEDY>(p, tp, two_to);
         bool good = t.good();
         if (lane == 0) {
             sh.pm = t.m;
             sh.at = t.at;
         }
         if (!GREEDY && left && draft) {
-            const RowStat q = row_stat<GREEDY>(p, p.nrows + row);
+            const RowStat q = row_stat<GREEDY>(p, qp, two_to);
             good = good && q.good();
             if (lane == 0) sh.qm = q.m;
         }
@@ -255,7 +297,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
     }
     __syncthreads();
     if (rank == 0) {
-        for (int j = tid; j < n; j += VD_THREADS)
+        for (int j = tid; j < n; j += VD_PICK_THREADS)
             if (j != end) p.out[r0 + j] = j < end ? p.tokens[r0 + j + 1] : -1;
         if (tid == 0) p.accepted[b] = end;
     }
@@ -268,33 +310,43 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
     }
     const T *pt = target + row * p.target_stride, *pd = left && draft ? draft + row * p.draft_stride : nullptr;
     const int gone = left && !draft ? p.tokens[row + 1] : -1;
-    const double pm = sh.pm, qm = sh.qm;
+    // e^((logit - largest) / temperature) as one multiplication and addition ahead of exp_neg (rounding may leave it above 0 by 1e-13)
+    const double pb = -(double)sh.pm * p.inv_t, qb = -(double)sh.qm * p.inv_t;
+    auto ep = [&](float x) { return exp_neg(fma((double)x, p.inv_t, pb), two_to); };
+    auto eq = [&](float x) { return exp_neg(fma((double)x, p.inv_t, qb), two_to); };
+    constexpr int PER = VD_TILE / 32;  // tokens of a tile a lane has
+    auto logits = [&](const T* row_, int first, int step, float (&x)[PER]) {  // all of them asked for before one is used
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[e] = first + e * step < p.vocab ? wide(row_[first + e * step]) : -INFINITY;
+    };
     const int all_tiles = (p.vocab + VD_TILE - 1) / VD_TILE, per = (all_tiles + size - 1) / size;
     const int t0 = min(all_tiles, rank * per), t1 = min(all_tiles, t0 + per);
     double ip = 1.0, iq = 0.0;
     if (pd) {
         double sp = 0.0, sq = 0.0;
-        for (int t = t0 + warp; t < t1; t += VD_WARPS)
+        for (int t = t0 + warp; t < t1; t += VD_PICK_WARPS) {
+            float a[PER], d[PER];
+            logits(pt, t * VD_TILE + lane, 32, a);
+            logits(pd, t * VD_TILE + lane, 32, d);
 #pragma unroll
-            for (int e = 0; e < VD_TILE / 32; ++e) {
-                const int i = t * VD_TILE + e * 32 + lane;
-                if (i < p.vocab) {
-                    sp += exp(((double)wide(pt[i]) - pm) * p.inv_t);
-                    sq += exp(((double)wide(pd[i]) - qm) * p.inv_t);
-                }
+            for (int e = 0; e < PER; ++e) {
+                sp += ep(a[e]);
+                sq += eq(d[e]);
             }
+        }
         sp = warp_sum_d(sp);
         sq = warp_sum_d(sq);
         if (lane == 0) { sh.red[0][warp] = sp; sh.red[1][warp] = sq; }
         __syncthreads();
         if (tid < 2) {
             double v = 0.0;
-            for (int i = 0; i < VD_WARPS; ++i) v += sh.red[tid][i];
+            for (int i = 0; i < VD_PICK_WARPS; ++i) v += sh.red[tid][i];
             sh.total[tid] = v;
         }
         cluster.sync();
         sp = sq = 0.0;
-        for (int r = 0; r < size; ++r) {
+#pragma unroll
+        for (int r = 0; r < VD_CLUSTER; ++r) {
             const double* o = cluster.map_shared_rank(sh.total, r);
             sp += o[0];
             sq += o[1];
@@ -302,19 +354,25 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
         ip = 1.0 / sp;
         iq = 1.0 / sq;
     }
-    auto share = [&](int i, bool rest) -> double {  // of token i in what is drawn from
-        if (i >= p.vocab || (rest && i == gone)) return 0.0;
-        const double v = exp(((double)wide(pt[i]) - pm) * p.inv_t);
-        if (!rest || !pd) return v;
-        return fmax(v * ip - exp(((double)wide(pd[i]) - qm) * p.inv_t) * iq, 0.0);
+    auto shares = [&](int first, int step, bool rest, double (&v)[PER]) {  // of a lane's tokens in what is drawn from
+        float a[PER], d[PER];
+        logits(pt, first, step, a);
+        if (rest && pd) logits(pd, first, step, d);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            v[e] = ep(a[e]);
+            if (rest && pd) v[e] = fmax(v[e] * ip - eq(d[e]) * iq, 0.0);
+            if (rest && first + e * step == gone) v[e] = 0.0;
+        }
     };
-    double whole = 0.0, before = 0.0, mine = 0.0;
+    double whole = 0.0, before = 0.0, totals[VD_CLUSTER];
     bool rest = left;
     for (int turn = 0; turn < 2; ++turn) {  // again from p alone where rounding leaves nothing of p - q
-        for (int t = t0 + warp; t < t1; t += VD_WARPS) {
-            double v = 0.0;
+        for (int t = t0 + warp; t < t1; t += VD_PICK_WARPS) {
+            double x[PER], v = 0.0;
+            shares(t * VD_TILE + lane, 32, rest, x);
 #pragma unroll
-            for (int e = 0; e < VD_TILE / 32; ++e) v += share(t * VD_TILE + e * 32 + lane, rest);
+            for (int e = 0; e < PER; ++e) v += x[e];
             v = warp_sum_d(v);
             if (lane == 0) tiles[t - t0] = v;
         }
@@ -327,11 +385,12 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
         }
         cluster.sync();
         whole = before = 0.0;
-        for (int r = 0; r < size; ++r) {
-            const double v = *cluster.map_shared_rank(&sh.total[2], r);
-            if (r < rank) before += v;
-            if (r == rank) mine = v;
-            whole += v;
+#pragma unroll
+        for (int r = 0; r < VD_CLUSTER; ++r) totals[r] = *cluster.map_shared_rank(&sh.total[2], r);
+#pragma unroll
+        for (int r = 0; r < VD_CLUSTER; ++r) {
+            if (r < rank) before += totals[r];
+            whole += totals[r];
         }
         cluster.sync();
         if (whole > 0.0 || !rest) break;
@@ -342,46 +401,60 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
     const double goal = (double)p.draws[b] * whole;
     double run = 0.0;
     int owner = -1;
-    for (int r = 0; r < size; ++r) {
-        const double v = *cluster.map_shared_rank(&sh.total[2], r);
-        if (v > 0.0) owner = r;
-        run += v;
-        if (run > goal) break;
+    bool open = true;
+#pragma unroll
+    for (int r = 0; r < VD_CLUSTER; ++r) {
+        if (open && totals[r] > 0.0) owner = r;
+        run += totals[r];
+        open = open && !(run > goal);
     }
-    cluster.sync();  // nobody reads this CTA's shared memory any more
+    // (the barrier behind the totals: nobody reads this CTA's shared memory any more)
     if (owner != rank || warp != 0) return;
-    (void)mine;
-    int tile = 0;
-    run = before;
-    {
-        double acc = before;
-        int last = 0;
-        double last_before = before;
-        for (int t = 0; t < t1 - t0; ++t) {
-            const double v = tiles[t];
-            if (v > 0.0) { last = t; last_before = acc; }
-            acc += v;
-            if (acc > goal && v > 0.0) break;
-        }
-        tile = last;
-        run = last_before;
-    }
-    int found = -1, fallback = 0;
-    for (int e = 0; e < VD_TILE / 32 && found < 0; ++e) {
-        const int i = (t0 + tile) * VD_TILE + e * 32 + lane;
-        const double v = share(i, rest);
+    // exclusive sums over the lanes' values in order; the first of them whose end exceeds the goal, or the last one with a share
+    auto pick = [&](double v, double& before_it, double& all_) {
         double incl = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
-        const uint32_t some = __ballot_sync(0xffffffffu, v > 0.0), over = __ballot_sync(0xffffffffu, v > 0.0 && run + incl > goal);
-        if (some) fallback = i - lane + 31 - __clz(some);
-        if (over) found = i - lane + __ffs(over) - 1;
-        run += __shfl_sync(0xffffffffu, incl, 31);
+        const uint32_t over = __ballot_sync(0xffffffffu, v > 0.0 && run + incl > goal), some = __ballot_sync(0xffffffffu, v > 0.0);
+        const int at = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
+        before_it = __shfl_sync(0xffffffffu, run + (incl - v), max(at, 0));
+        all_ = __shfl_sync(0xffffffffu, incl, 31);
+        return over ? at : at < 0 ? -64 : at - 32;  // below 0: none exceeds it
+    };
+    run = before;
+    int tile = 0;
+    double tile_run = before;
+    for (int t = 0; t < t1 - t0; t += 32) {
+        double from, all_;
+        const int at = pick(t + lane < t1 - t0 ? tiles[t + lane] : 0.0, from, all_);
+        if (at != -64) {
+            tile = t + (at < 0 ? at + 32 : at);
+            tile_run = from;
+        }
+        if (at >= 0) break;
+        run += all_;
     }
-    if (lane == 0) p.out[row] = found >= 0 ? found : fallback;
+    run = tile_run;
+    const int first = (t0 + tile) * VD_TILE + lane * PER;  // eight tokens a lane, in order
+    double v[PER], sum = 0.0, from, all_;
+    shares(first, 1, rest, v);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum += v[e];
+    const int at = pick(sum, from, all_), holder = at < 0 ? at + 32 : at;
+    if (lane == max(holder, 0)) {
+        int found = -1;
+        double acc = from;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const bool before_goal = !(acc > goal);
+            acc += v[e];
+            if (v[e] > 0.0 && (found < 0 || before_goal)) found = first + e;
+        }
+        p.out[row] = found;
+    }
 }
 
 template <typename T, bool GREEDY> cudaError_t launch(const VerifyArgs& a, bool draft, cudaStream_t s) {
@@ -391,7 +464,7 @@ template <typename T, bool GREEDY> cudaError_t launch(const VerifyArgs& a, bool 
     const int size = GREEDY ? 1 : VD_CLUSTER, tiles = (a.vocab + VD_TILE - 1) / VD_TILE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.nseq * size);
-    cfg.blockDim = dim3(VD_THREADS);
+    cfg.blockDim = dim3(VD_PICK_THREADS);
     cfg.dynamicSmemBytes = GREEDY ? 0 : (size_t)((tiles + size - 1) / size) * 8;
     cfg.stream = s;
     cudaLaunchAttribute at[2] = {};
