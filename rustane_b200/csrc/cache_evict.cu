@@ -371,9 +371,8 @@ extern "C" int cd_cache_evict(const cd_paged_cache* c, int keep, int sinks, int 
     DeviceGuard guard(c->device);
     if (guard.err != cudaSuccess) return cuda_status(guard.err, CALL);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int sms = 0;
+    cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return cuda_status(e, CALL);
     int size = 1;  // one CTA for every 8192 places, so that a pass over the keys stays short
     while (size < EV_CLUSTER && (long long)size * 8192 < a.c.cap) size *= 2;

@@ -53,9 +53,8 @@ int check_shape(const cd_paged_cache* c, int heads, int nrows, int max_rows, int
 }
 
 template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a, const Plan& plan, int collect, cudaStream_t s) {
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int sms = 0;
+    cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
     if constexpr (std::is_same<KT, float>::value) {
         attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);

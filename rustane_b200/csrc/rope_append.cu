@@ -76,40 +76,43 @@ template <typename T, int E> __device__ inline void store(T* p, const float (&x)
     }
 }
 
-// One item of a rotated head: E elements and, in halves, their partners; or E elements that pass.
-template <bool HALF, int E, typename TI, typename TO> __device__ inline void rotate_item(const TI* in, TO* out, int item, int rot, const float2* cs) {
-    const int turned = HALF ? rot / 2 / E : rot / E;
-    float a[E];
-    if (item >= turned) {
-        const int at = rot + (item - turned) * E;
+// One item: E elements of a rotated head and, in halves, their partners; or E elements that pass.  Loaded and stored apart, so that a thread
+// has the loads of several items under way.
+template <bool HALF, int E> struct Item {
+    float a[E], b[E];
+    int at = 0;
+    bool turns = false;
+    template <typename TI> __device__ inline void get(const TI* in, int item, int rot) {
+        const int turned = HALF ? rot / 2 / E : rot / E;
+        turns = item < turned;
+        at = turns ? item * E : rot + (item - turned) * E;
         load<TI, E>(in + at, a);
+        if (HALF && turns) load<TI, E>(in + rot / 2 + at, b);
+    }
+    template <typename TO> __device__ inline void put(TO* out, int rot, const float2* cs) {
+        if (turns) {
+            if constexpr (HALF) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float2 t = cs[at + e];
+                    const float x = a[e], y = b[e];
+                    a[e] = x * t.x - y * t.y;
+                    b[e] = x * t.y + y * t.x;
+                }
+                store<TO, E>(out + rot / 2 + at, b);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float2 t = cs[(at + e) / 2];
+                    const float x = a[e], y = a[e + 1];
+                    a[e] = x * t.x - y * t.y;
+                    a[e + 1] = x * t.y + y * t.x;
+                }
+            }
+        }
         store<TO, E>(out + at, a);
-        return;
     }
-    const int at = item * E;
-    load<TI, E>(in + at, a);
-    if constexpr (HALF) {
-        float b[E];
-        load<TI, E>(in + rot / 2 + at, b);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float2 t = cs[at + e];
-            const float x = a[e], y = b[e];
-            a[e] = x * t.x - y * t.y;
-            b[e] = x * t.y + y * t.x;
-        }
-        store<TO, E>(out + rot / 2 + at, b);
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const float2 t = cs[(at + e) / 2];
-            const float x = a[e], y = a[e + 1];
-            a[e] = x * t.x - y * t.y;
-            a[e + 1] = x * t.y + y * t.x;
-        }
-    }
-    store<TO, E>(out + at, a);
-}
+};
 
 template <typename QT, typename KT, int HD, bool HALF, int E> __global__ void __launch_bounds__(RA_THREADS) rope_append_kernel(const __grid_constant__ AppendArgs p) {
     __shared__ float2 cs[HD / 2];
@@ -140,20 +143,32 @@ template <typename QT, typename KT, int HD, bool HALF, int E> __global__ void __
     const QT *q = static_cast<const QT*>(p.q) + row * p.q_stride, *k = static_cast<const QT*>(p.k) + row * p.k_stride, *v = static_cast<const QT*>(p.v) + row * p.v_stride;
     QT* q_out = static_cast<QT*>(p.q_out) + (size_t)row * p.heads * HD;
     KT* pool = static_cast<KT*>(p.c.pool);
-#pragma unroll 2
-    for (int i = part * RA_THREADS + tid; i < all; i += p.parts * RA_THREADS) {
-        if (i < rotated) {
-            const int vec = i / per, item = i % per;
-            if (vec < p.heads) rotate_item<HALF, E>(q + (size_t)vec * HD, q_out + (size_t)vec * HD, item, p.rot, cs);
-            else if (page >= 0) {
-                const int h = vec - p.heads;
-                rotate_item<HALF, E>(k + (size_t)h * HD, pool + row_at(p.c, page, 0, h, entry, HD), item, p.rot, cs);
+    constexpr int DEEP = 2;
+    for (int i0 = part * RA_THREADS + tid; i0 < all; i0 += p.parts * RA_THREADS * DEEP) {
+        Item<HALF, E> x[DEEP];
+        int vec[DEEP];  // q heads, k heads, v heads; -1: nothing
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int i = i0 + d * p.parts * RA_THREADS;
+            vec[d] = -1;
+            if (i < rotated) {
+                vec[d] = i / per;
+                const QT* src = vec[d] < p.heads ? q + (size_t)vec[d] * HD : k + (size_t)(vec[d] - p.heads) * HD;
+                x[d].get(src, i - vec[d] * per, p.rot);
+            } else if (i < all) {
+                const int h = (i - rotated) / (HD / E);
+                vec[d] = p.heads + p.c.kv_heads + h;
+                x[d].get(v + (size_t)h * HD, i - rotated - h * (HD / E), 0);
             }
-        } else if (page >= 0) {
-            const int h = (i - rotated) / (HD / E), at = (i - rotated) % (HD / E) * E;
-            float x[E];
-            load<QT, E>(v + (size_t)h * HD + at, x);
-            store<KT, E>(pool + row_at(p.c, page, 1, h, entry, HD) + at, x);
+        }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int h = vec[d] - p.heads;
+            if (vec[d] >= 0 && h < 0) x[d].put(q_out + (size_t)vec[d] * HD, p.rot, cs);
+            else if (vec[d] >= 0 && page >= 0) {
+                const bool is_v = h >= p.c.kv_heads;
+                x[d].put(pool + row_at(p.c, page, is_v, is_v ? h - p.c.kv_heads : h, entry, HD), is_v ? 0 : p.rot, cs);
+            }
         }
     }
     if (p.c.weight && entry >= 0 && part == 0)

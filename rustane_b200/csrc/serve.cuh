@@ -3,6 +3,7 @@
 // Lengths, rows and page ids live on the device and a call never waits for them, so every kernel checks what it is about to use
 // as an address: batch_seq() leaves a sequence out whose rows or length do not fit, page_at() refuses a page outside the pool.
 #pragma once
+#include <atomic>
 #include <string>
 
 #include "model.h"
@@ -75,6 +76,17 @@ struct DeviceGuard {
         if (before >= 0) cudaSetDevice(before);
     }
 };
+// SMs of the current device (asked for once a device)
+inline cudaError_t sm_count(int* sms) {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess && dev < 64) known[dev].store(*sms, std::memory_order_relaxed);
+    return e;
+}
 inline size_t dtype_size(int dtype) { return dtype == CD_DTYPE_F32 ? 4 : 2; }
 inline bool aligned(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 inline int refuse(int code, const char* call, const char* what) { return fail(nullptr, code, std::string(call) + ": " + what); }

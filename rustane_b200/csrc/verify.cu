@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "serve.cuh"
 
@@ -19,7 +20,7 @@ using namespace cd;
 
 namespace {
 const char* CALL = "cd_verify_drafts";
-constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32, VD_PICK_THREADS = 512, VD_PICK_WARPS = VD_PICK_THREADS / 32, VD_CHUNKS = 32, VD_CLUSTER = 8, VD_TILE = 256, VD_VOCAB = 1 << 22;
+constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32, VD_PICK_THREADS = 512, VD_PICK_WARPS = VD_PICK_THREADS / 32, VD_CHUNKS = 32, VD_CLUSTER = 8, VD_TILE = 256, VD_KEEP = 16, VD_VOCAB = 1 << 22;
 
 struct Part {
     float m;   // NaN: the chunk holds NaN
@@ -120,7 +121,13 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
 #pragma unroll
         for (int d = 0; d < DEEP; ++d)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[d][e] = i + d * VD_THREADS < vecs ? wide(reinterpret_cast<const T*>(&w[d])[e]) : -INFINITY;
+            for (int e = 0; e < VEC; ++e) v[d][e] = wide(reinterpret_cast<const T*>(&w[d])[e]);
+        if (i + (DEEP - 1) * VD_THREADS >= vecs)
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d)
+                if (i + d * VD_THREADS >= vecs)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[d][e] = -INFINITY;
         if (i + VD_THREADS * DEEP < vecs) fetch(i + VD_THREADS * DEEP);
         if (GREEDY) {
 #pragma unroll
@@ -232,6 +239,7 @@ struct PickShared {
     double total[3];  // of this CTA: p's sum, q's sum, what is drawn from
     double red[2][VD_PICK_WARPS];
     float pm, qm;
+    RowStat rows[2][VD_KEEP];  // of the sequence's first rows, target and draft, as the tests found them
 };
 
 template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const __grid_constant__ VerifyArgs p) {
@@ -264,6 +272,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
         const bool in = (unsigned)x < (unsigned)p.vocab;
         const float tx = in && !GREEDY ? wide(target[(r0 + j) * p.target_stride + x]) : 0.f, qx_logit = in && draft ? wide(draft[(r0 + j) * p.draft_stride + x]) : 0.f;
         const RowStat t = row_stat<GREEDY>(p, tp, two_to);
+        if (lane == 0 && j < VD_KEEP) sh.rows[0][j] = t;
         bool stays = t.good() && in;
         if (GREEDY) stays = stays && t.at == x;
         else {
@@ -271,6 +280,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
             double qx = 1.0;
             if (draft) {
                 const RowStat q = row_stat<GREEDY>(p, qp, two_to);
+                if (lane == 0 && j < VD_KEEP) sh.rows[1][j] = q;
                 qx = q.good() ? exp_neg(((double)qx_logit - (double)q.m) * p.inv_t, two_to) / q.z : NAN;
             }
             stays = stays && (double)u * qx < px;
@@ -281,19 +291,21 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     const int end = sh.first_bad, row = r0 + end;
     const bool left = end < n - 1;  // a draft was turned down: draw from what p has over q
     if (warp == 0) {
-        const Part tp = load_part(p, row), qp = left && draft ? load_part(p, p.nrows + row) : Part{};
-        const RowStat t = row_stat<GREEDY>(p, tp, two_to);
-        bool good = t.good();
+        RowStat t, q;
+        if (left && end < VD_KEEP) {
+            t = sh.rows[0][end];
+            if (draft) q = sh.rows[1][end];
+        } else {
+            const Part tp = load_part(p, row), qp = left && draft ? load_part(p, p.nrows + row) : Part{};
+            t = row_stat<GREEDY>(p, tp, two_to);
+            if (left && draft) q = row_stat<GREEDY>(p, qp, two_to);
+        }
         if (lane == 0) {
             sh.pm = t.m;
             sh.at = t.at;
+            sh.qm = left && draft ? q.m : 0.f;
+            if (!t.good() || (!GREEDY && left && draft && !q.good())) sh.valid = 0;
         }
-        if (!GREEDY && left && draft) {
-            const RowStat q = row_stat<GREEDY>(p, qp, two_to);
-            good = good && q.good();
-            if (lane == 0) sh.qm = q.m;
-        }
-        if (lane == 0 && !good) sh.valid = 0;
     }
     __syncthreads();
     if (rank == 0) {
@@ -392,8 +404,8 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
             if (r < rank) before += totals[r];
             whole += totals[r];
         }
-        cluster.sync();
         if (whole > 0.0 || !rest) break;
+        cluster.sync();  // (rounding left nothing: once in a lifetime)
         rest = false;
     }
     // the first token whose running sum exceeds u * whole: the CTA, then the tile, then the token.  Sums of sums round, so where none
@@ -408,8 +420,12 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
         run += totals[r];
         open = open && !(run > goal);
     }
-    // (the barrier behind the totals: nobody reads this CTA's shared memory any more)
-    if (owner != rank || warp != 0) return;
+    // others may still read this CTA's totals: it stays until all have them, but does not wait for that with its own work
+    auto arrived = cluster.barrier_arrive();
+    if (owner != rank || warp != 0) {
+        cluster.barrier_wait(std::move(arrived));
+        return;
+    }
     // exclusive sums over the lanes' values in order; the first of them whose end exceeds the goal, or the last one with a share
     auto pick = [&](double v, double& before_it, double& all_) {
         double incl = v;
@@ -455,6 +471,8 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
         }
         p.out[row] = found;
     }
+    __syncwarp();
+    cluster.barrier_wait(std::move(arrived));
 }
 
 template <typename T, bool GREEDY> cudaError_t launch(const VerifyArgs& a, bool draft, cudaStream_t s) {

@@ -50,18 +50,21 @@ def flash_decode(q, k, v, heads, kv_heads, hd, dtype="bf16", nsplit=0):
 
 
 # ------------------------------------------------------------------------------------------------ operators of a serving step
-def _torch():
-    import torch
-    return torch
+torch = None   # loaded by the first cache, rope or verification: flash_decode does without
+_CODES = {}    # torch dtype -> CD_DTYPE_*
+_current = None  # a device's current stream as an address
 
 
-_CODES = {}  # torch dtype -> CD_DTYPE_*
+def _load_torch():
+    global torch, _current
+    if torch is None:
+        import torch as loaded
+        _CODES.update({loaded.float32: 0, loaded.float16: 1, loaded.bfloat16: 2})
+        _current = getattr(loaded._C, "_cuda_getCurrentRawStream", None) or (lambda i: loaded.cuda.current_stream(i).cuda_stream)
+        torch = loaded
 
 
 def _code(t, what):
-    if not _CODES:
-        torch = _torch()
-        _CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     code = _CODES.get(t.dtype)
     if code is None:
         raise ValueError("%s must be float32, float16 or bfloat16" % what)
@@ -90,16 +93,6 @@ def _row_stride(t, what, rows, hd, index):
     return row if rows > 1 else 0
 
 
-_STREAM = []  # torch's call for a device's current stream as an address
-
-
-def _stream(index):
-    if not _STREAM:
-        torch = _torch()
-        _STREAM.append(getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream))
-    return _STREAM[0](index)
-
-
 def _check(rc):
     if rc:
         raise CudaDecodeError(rc, lib.cd_last_error(None).decode())
@@ -112,7 +105,7 @@ class PagedCache:
     of one element that collects CD_STATUS_* bits of what a call had to leave out; made here if not given."""
 
     def __init__(self, pool, page_table, lens, weight=None, position=None, status=None):
-        torch = _torch()
+        _load_torch()
         if not pool.is_cuda:
             raise ValueError("the pool must be a CUDA tensor")
         if pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
@@ -137,7 +130,6 @@ class PagedCache:
 
     def replace(self, lens=None, weight=None, position=None):
         """Take other tensors for the lengths or the bookkeeping, as cache_evict returned them."""
-        torch = _torch()
         if lens is not None:
             self._c.lens = _tensor(lens, "lens", torch.int32, (self.nseq,), self._index)
             self.lens = lens
@@ -162,7 +154,6 @@ class PagedCache:
 
 
 def _workspace(given, need, device):
-    torch = _torch()
     if given is None:
         return torch.empty(need, dtype=torch.uint8, device=device)
     if given.dtype != torch.uint8 or given.device != device or not given.is_contiguous():
@@ -181,8 +172,8 @@ class Rope:
     def __init__(self, rot_dim, base=10000.0, layout="half", scaling=None, factor=1.0, original=4096, device="cuda"):
         if layout not in self.LAYOUTS or scaling not in self.SCALINGS:
             raise ValueError("layout is one of %s, scaling one of %s" % (sorted(self.LAYOUTS), sorted(k for k in self.SCALINGS if k)))
+        _load_torch()
         turns, magnitude = rope_frequencies(rot_dim, base, scaling, factor, original)
-        torch = _torch()
         self.turns = torch.from_numpy(turns.view(np.int64)).to(device)
         self.rot_dim, self.layout, self.magnitude = rot_dim, layout, magnitude
         self._c = _ffi.CdRope(rot_dim, self.LAYOUTS[layout], magnitude, 0, self.turns.data_ptr())
@@ -200,7 +191,7 @@ def rope_append(cache, rope, q, k, v, positions, row_start, out=None):
     """Rotate q [rows, heads, hd] and k [rows, kv_heads, hd] at `positions` [rows] int32, write k and v to their entries in the cache (with
     bookkeeping: weight 0, the position noted), return the rotated q.  q, k and v are f32 or of the pool's type; they may be
     slices of one fused projection.  out: a packed tensor for the result; q itself where q is packed."""
-    torch, index, hd = _torch(), cache._index, cache.hd
+    index, hd = cache._index, cache.hd
     rows, dtype = q.shape[0], q.dtype
     sq, sk, sv = _row_stride(q, "q", rows, hd, index), _row_stride(k, "k", rows, hd, index), _row_stride(v, "v", rows, hd, index)
     if k.shape[1] != cache.kv_heads or v.shape[1] != cache.kv_heads:
@@ -210,10 +201,10 @@ def rope_append(cache, rope, q, k, v, positions, row_start, out=None):
     if rope.turns.get_device() != index:
         raise ValueError("rope must be on cuda:%d" % index)
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=cache.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _check(lib.cd_rope_append(cache._ref, rope._ref, _code(q, "q"), q.shape[1], rows, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv,
                               _tensor(positions, "positions", torch.int32, (rows,), index), _tensor(row_start, "row_start", torch.int32, cache._starts, index),
-                              _tensor(out, "out", dtype, q.shape, index), _stream(index)))
+                              _tensor(out, "out", dtype, q.shape, index), _current(index)))
     return out
 
 
@@ -221,17 +212,17 @@ def paged_attention(cache, q, row_start, max_rows, scale=None, window=0, collect
     """Attention of the new rows q [rows, heads, hd] (f32 or of the pool's type) over the cache, each row up to its own entry, or over its last
     `window` entries.  max_rows: the most rows a sequence has.  collect: add the probabilities to cache.weight.  Returns out, or
     (out, lse [rows, heads] f32) with lse.  Rows from row_start[nseq] on are not written."""
-    torch, index = _torch(), cache._index
+    index = cache._index
     shape = q.shape
     rows, heads, collect = shape[0], shape[1], 1 if collect else 0
     stride = _row_stride(q, "q", rows, cache.hd, index)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=cache.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     norm = torch.empty((rows, heads), dtype=torch.float32, device=cache.device) if lse else None
     ws = cache._workspace(workspace, lib.cd_paged_attention_workspace, heads, rows, max_rows, collect)
     _check(lib.cd_paged_attention(cache._ref, _code(q, "q"), heads, rows, max_rows, q.data_ptr(), stride,
                                   _tensor(row_start, "row_start", torch.int32, cache._starts, index), 0.0 if scale is None else scale, window, collect,
-                                  _tensor(out, "out", q.dtype, shape, index), norm.data_ptr() if lse else None, ws.data_ptr(), ws.numel(), _stream(index)))
+                                  _tensor(out, "out", q.dtype, shape, index), norm.data_ptr() if lse else None, ws.data_ptr(), ws.numel(), _current(index)))
     return (out, norm) if lse else out
 
 
@@ -239,7 +230,7 @@ def cache_evict(cache, keep, sinks=0, recent=0, out=None, workspace=None):
     """Bring every sequence with more than `keep` entries down to `keep`, each kv head by its own weights; positions below `sinks` and the
     newest `recent` ones stay.  K and V move within the cache's pages.  Returns new (lens, weight, position), which the caller
     hands to cache.replace(); out: tensors for them (weight and position may be the cache's own, lens may not)."""
-    torch, index = _torch(), cache._index
+    index = cache._index
     if cache.weight is None:
         raise ValueError("the cache has no weight and position")
     lens, weight, position = out if out is not None else (torch.empty_like(cache.lens), torch.empty_like(cache.weight), torch.empty_like(cache.position))
@@ -247,7 +238,7 @@ def cache_evict(cache, keep, sinks=0, recent=0, out=None, workspace=None):
     shape = cache.weight.shape
     _check(lib.cd_cache_evict(cache._ref, keep, sinks, recent, _tensor(lens, "lens", torch.int32, cache.lens.shape, index),
                               _tensor(weight, "weight", torch.float32, shape, index), _tensor(position, "position", torch.int32, shape, index),
-                              ws.data_ptr(), ws.numel(), _stream(index)))
+                              ws.data_ptr(), ws.numel(), _current(index)))
     return lens, weight, position
 
 
@@ -256,7 +247,8 @@ def verify_drafts(target, tokens, row_start, max_rows, uniforms, draws, draft=No
     of each sequence, then its drafts; uniforms [rows] and draws [nseq] f32 in [0, 1) (not used at temperature 0, and None is fine there);
     draft [rows, vocab]: the logits the token behind each row was drawn from, None: drafts without a distribution.  Returns
     (accepted [nseq] int32, out_tokens [rows] int32: the drafts that stay, the drawn token, then -1)."""
-    torch, device, shape = _torch(), target.device, target.shape
+    _load_torch()
+    device, shape = target.device, target.shape
     index = device.index
     if not target.is_cuda or len(shape) != 2 or (shape[1] > 1 and target.stride(1) != 1):
         raise ValueError("target must be a CUDA tensor [rows, vocab] with packed rows")
@@ -281,7 +273,7 @@ def verify_drafts(target, tokens, row_start, max_rows, uniforms, draws, draft=No
                                 _tensor(uniforms, "uniforms", torch.float32, (rows,), index) if random else None,
                                 _tensor(draws, "draws", torch.float32, (nseq,), index) if random else None, temperature, accepted.data_ptr(),
                                 out.data_ptr(), None if status is None else _tensor(status, "status", torch.int32, (1,), index), ws.data_ptr(), ws.numel(),
-                                _stream(index)))
+                                _current(index)))
     return accepted, out
 
 
