@@ -49,21 +49,21 @@ __device__ inline float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// e^x in 64 bits for x <= 0: e^x = 2^(n / 32) e^r with |r| <= ln 2 / 64, e^r by its series up to r^6 / 720 (the next term is below
-// 4e-18), 2^(j / 32) from a table of 32.  Off by some 1e-16 (and x times 2e-17); half the 64-bit operations of exp().
+// e^x in 64 bits for x <= 0 (or a little above): e^x = 2^(n / 256) e^r with |r| <= ln 2 / 512, e^r by its series up to r^4 / 24 (the next
+// term is below 4e-17), 2^(j / 256) from a table.  Off by some 1e-16, and by x times 1e-16.  What the draw costs is the 64-bit pipe:
+// eight operations here against about twice that in exp().
+constexpr int EXP_TABLE = 256;
 __device__ inline double exp_neg(double x, const double* two_to) {
     constexpr double ROUND = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the integer
-    const double t = fma(x, 46.166241308446828384, ROUND);  // 32 / ln 2
+    const double t = fma(x, 369.32993046757462, ROUND);  // 256 / ln 2
     const int n = __double2loint(t);
-    const double r = fma(t - ROUND, -0.021660849392498290195, x);  // ln 2 / 32
-    double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
-    e = fma(e, r, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
+    const double r = fma(t - ROUND, -0.0027076061740622863, x);  // ln 2 / 256
+    double e = fma(r, 1.0 / 24.0, 1.0 / 6.0);
     e = fma(e, r, 0.5);
     e = fma(e, r, 1.0);
     e = fma(e, r, 1.0);
-    const double y = e * two_to[n & 31];
-    const double v = __hiloint2double(__double2hiint(y) + ((n >> 5) << 20), __double2loint(y));
+    const double y = e * two_to[n & (EXP_TABLE - 1)];
+    const double v = __hiloint2double(__double2hiint(y) + ((n >> 8) << 20), __double2loint(y));
     return x > -708.0 ? v : x != x ? x : 0.0;  // (no branch: a lane's terms go through the pipe together)
 }
 __device__ inline uint4 load_once(const void* p) {
@@ -257,8 +257,8 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
         }
         return;
     }
-    __shared__ double two_to[32];
-    if (tid < 32) two_to[tid] = exp2((double)tid / 32.0);
+    __shared__ double two_to[EXP_TABLE];
+    if (!GREEDY && tid < EXP_TABLE) two_to[tid] = exp2((double)tid / EXP_TABLE);
     if (tid == 0) {
         sh.first_bad = n - 1;
         sh.valid = 1;
@@ -323,7 +323,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     const T *pt = target + row * p.target_stride, *pd = left && draft ? draft + row * p.draft_stride : nullptr;
     const int gone = left && !draft ? p.tokens[row + 1] : -1;
     // e^((logit - largest) / temperature) as one multiplication and addition ahead of exp_neg (rounding may leave it above 0 by 1e-13)
-    const double pb = -(double)sh.pm * p.inv_t, qb = -(double)sh.qm * p.inv_t;
+    double pb = -(double)sh.pm * p.inv_t, qb = -(double)sh.qm * p.inv_t;
     auto ep = [&](float x) { return exp_neg(fma((double)x, p.inv_t, pb), two_to); };
     auto eq = [&](float x) { return exp_neg(fma((double)x, p.inv_t, qb), two_to); };
     constexpr int PER = VD_TILE / 32;  // tokens of a tile a lane has
@@ -333,7 +333,6 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     };
     const int all_tiles = (p.vocab + VD_TILE - 1) / VD_TILE, per = (all_tiles + size - 1) / size;
     const int t0 = min(all_tiles, rank * per), t1 = min(all_tiles, t0 + per);
-    double ip = 1.0, iq = 0.0;
     if (pd) {
         double sp = 0.0, sq = 0.0;
         for (int t = t0 + warp; t < t1; t += VD_PICK_WARPS) {
@@ -363,8 +362,8 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
             sp += o[0];
             sq += o[1];
         }
-        ip = 1.0 / sp;
-        iq = 1.0 / sq;
+        pb -= log(sp);  // from here on the terms are p and q themselves
+        qb -= log(sq);
     }
     auto shares = [&](int first, int step, bool rest, double (&v)[PER]) {  // of a lane's tokens in what is drawn from
         float a[PER], d[PER];
@@ -373,7 +372,10 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             v[e] = ep(a[e]);
-            if (rest && pd) v[e] = fmax(v[e] * ip - eq(d[e]) * iq, 0.0);
+            if (rest && pd) {
+                v[e] -= eq(d[e]);
+                if (__double2hiint(v[e]) < 0) v[e] = 0.0;  // (by its sign bit: no 64-bit comparison)
+            }
             if (rest && first + e * step == gone) v[e] = 0.0;
         }
     };
