@@ -93,11 +93,10 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
             if (i + d * VD_THREADS < vecs) w[d] = load_once(body + i + d * VD_THREADS);
     };
     fetch(tid);
-    // rows behind the last sequence, and draft rows with no draft behind them, are not looked at
-    bool skip = tid == 0 && r >= p.row_start[p.nseq];
-    if (is_draft)
-        for (int b = tid; b < p.nseq; b += VD_THREADS) skip |= p.row_start[b + 1] - 1 == r;
-    if (__syncthreads_or(skip)) return;
+    // rows of no sequence, and draft rows with no draft behind them, are not looked at
+    bool used = false;
+    for (int b = tid; b < p.nseq; b += VD_THREADS) used |= p.row_start[b] <= r && r < p.row_start[b + 1] - (is_draft ? 1 : 0);
+    if (!__syncthreads_or(used)) return;
     const float scale = (float)(p.inv_t * 1.4426950408889634074);
     float m = -INFINITY, s = 0.f;
     int at = 0x7fffffff;
@@ -250,7 +249,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r0 = p.row_start[b], r1 = p.row_start[b + 1], n = r1 - r0;
     pdl_wait();
-    if (r0 < 0 || n < 0 || r1 > p.nrows || n > p.max_rows || n == 0) {
+    if (r0 < 0 || r1 < r0 || r1 > p.nrows || n > p.max_rows || n == 0) {
         if (rank == 0 && tid == 0) {
             p.accepted[b] = 0;
             if (n != 0) report(p.status, CD_STATUS_BATCH);

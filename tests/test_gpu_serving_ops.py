@@ -505,3 +505,258 @@ def test_verify_strided_rows_unaligned_and_rows_behind_the_batch():
                                       draft=wide2[:, 5:1006])
     want_n, want = ref.verify(f64(x["target"]), f64(x["draft"]), x["tokens"].numpy(), f64(x["u"]), f64(x["d"]), x["starts"].numpy(), 1.0)
     assert accepted.tolist() == want_n.tolist() and out.tolist()[:6] == want.tolist()
+
+
+def test_verify_leaves_out_sequences_whose_rows_do_not_fit():
+    import torch
+
+    from rustane_b200 import ops
+    x = verify_inputs([3, 2, 4], 700, "bf16", 12)
+    want_n, want = ref.verify(f64(x["target"]), f64(x["draft"]), x["tokens"].numpy(), f64(x["u"]), f64(x["d"]), x["starts"].numpy(), 1.0)
+    for starts, fits in (([0, 3, -1, 9], [0]), ([0, 3, 5, 10], [0, 1]), ([0, 3, 2, 9], [0]), ([-2 ** 31, 3, 5, 9], [1, 2]), ([2 ** 31 - 1, 3, 5, 9], [1, 2])):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        accepted, out = ops.verify_drafts(x["target"].cuda(), x["tokens"].cuda(), torch.tensor(starts, dtype=torch.int32, device="cuda"), 4, x["u"].cuda(), x["d"].cuda(),
+                                          draft=x["draft"].cuda(), status=status)
+        assert int(status) & 1
+        for b in fits:
+            assert int(accepted[b]) == want_n[b]
+            r0, r1 = x["starts"][b], x["starts"][b + 1]
+            assert out[r0:r1].tolist() == want[r0:r1].tolist()
+
+
+# ------------------------------------------------------------------------------------------------ where calls meet
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("page", [16, 24, 48])
+def test_attention_many_units_a_cta_with_rows_of_every_size(q_type, kv_type, page):
+    """More units than CTAs, one to four row warps in turn: every unit's stages follow another's, of another width."""
+    rng = np.random.default_rng(page)
+    lens, counts = [int(n) for n in rng.integers(1, 400, 96)], [int(n) for n in rng.integers(0, 7, 96)]
+    check_attention(Batch(lens, counts, 2, 64, page, kv_type, seed=page), 16, q_type)
+    check_attention(Batch(lens[:40], counts[:40], 4, 128, page, kv_type, seed=page), 16, q_type)
+
+
+def test_offsets_past_32_bits():
+    """A pool of 2^31 elements and more, its last pages in use: attention, append and eviction."""
+    import torch
+
+    from rustane_b200 import ops
+    kv, hd, page = 8, 128, 64
+    per = 2 * kv * page * hd
+    pages = 2 ** 31 // per + 40
+    pool = torch.zeros(pages, 2, kv, page, hd, dtype=torch.bfloat16, device="cuda")
+    small = Batch([300, 130], [1, 1], kv, hd, page, "bf16", seed=3, book=True, spare_pages=0)
+    used = small.pool.shape[0]
+    pool[-used:] = small.pool
+    table = torch.where(small.table >= 0, small.table + (pages - used), small.table)
+    q = small.normal(2, 16, hd, dtype="bf16")
+    want = ops.paged_attention(small.cache(), q, small.row_start, 1)
+    cache = ops.PagedCache(pool, table, small.tlens, small.weight, small.position)
+    assert torch.equal(ops.paged_attention(cache, q, small.row_start, 1), want)
+    k, v, at = small.normal(2, kv, hd, dtype="bf16"), small.normal(2, kv, hd, dtype="bf16"), torch.tensor([299, 129], dtype=torch.int32, device="cuda")
+    rope = ops.Rope(hd)
+    for c in (small.cache(), cache):
+        ops.rope_append(c, rope, q, k, v, at, small.row_start)
+        ops.cache_evict(c, 100)
+    assert torch.equal(pool[-used:], small.pool) and not bool(pool[:-used].any())
+
+
+def test_long_score_rows_are_collected_past_32_bits():
+    """scores of rows times entries pass 2^31 elements in the workspace."""
+    batch = Batch([64] * 3, [1] * 3, 1, 64, 64, "bf16", seed=4, book=False)
+    import torch
+    rows, heads, entries = 3, 64, 12 * 2 ** 20
+    table = torch.zeros(3, entries // 64, dtype=torch.int32, device="cuda")
+    table[:, 0] = batch.table[:, 0]
+    batch.table = table
+    batch.cap = entries
+    batch.weight = torch.zeros(3, 1, entries, device="cuda")
+    batch.position = torch.zeros(3, 1, entries, dtype=torch.int32, device="cuda")
+    assert rows * heads * entries > 2 ** 31
+    check_attention(batch, heads, "bf16", collect=True)
+
+
+@pytest.mark.parametrize("kv_type", ["bf16", "f32"])
+def test_a_bounded_cache_over_many_steps(kv_type):
+    """append, attend with weights, evict, step after step, each against a plain cache that is carried along; then the same
+    steps from a captured graph."""
+    import torch
+
+    from rustane_b200 import ops
+    nseq, heads, kv, hd, page, keep, steps = 3, 4, 2, 64, 16, 40, 60
+    lens0 = [30, 5, 38]
+    batch = Batch([48] * nseq, [1] * nseq, kv, hd, page, kv_type, seed=21, book=True)
+    batch.lens = lens0
+    batch.tlens = torch.tensor(lens0, dtype=torch.int32, device="cuda")
+    g = torch.Generator("cpu").manual_seed(5)
+    inputs = [torch.randn(nseq, heads + 2 * kv, hd, generator=g).to(batch.pool.dtype).cuda() for _ in range(steps)]
+    rope = ops.Rope(hd, layout="half")
+    start = (batch.pool.clone(), batch.weight.clone(), batch.position.clone())
+
+    def reset():
+        for mine, was in zip((batch.pool, batch.weight, batch.position), start):
+            mine.copy_(was)
+
+    def one_step(cache, x, at, lens, spare):
+        lens.add_(1)
+        q = ops.rope_append(cache, rope, x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:], at, batch.row_start)
+        out = ops.paged_attention(cache, q, batch.row_start, 1, collect=True)
+        ops.cache_evict(cache, keep, sinks=2, recent=8, out=(spare, batch.weight, batch.position))
+        lens.copy_(spare)
+        return out
+
+    # step by step, each against the plain form of what the cache holds at that moment
+    lens, spare = batch.tlens, torch.empty_like(batch.tlens)
+    cache, outs = batch.cache(), []
+    at = torch.tensor([500, 9, 38], dtype=torch.int32, device="cuda")
+    for x in inputs:
+        lens.add_(1)
+        q = ops.rope_append(cache, rope, x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:], at, batch.row_start)
+        batch.lens = lens.tolist()
+        before = f64(batch.weight)
+        out = ops.paged_attention(cache, q, batch.row_start, 1, collect=True)
+        want, _, mass, got, worst = ref.attention(batch, q)
+        assert (np.abs(f64(out) - want) <= attention_tolerance(want, mass, kv_type, kv_type, hd, worst)).all()
+        weight, position, pool = f64(batch.weight), batch.position.cpu().numpy(), batch.pool.clone()
+        for b, n in enumerate(batch.lens):
+            np.testing.assert_allclose(weight[b][:, :n], before[b][:, :n] + got[b], rtol=1e-4, atol=1e-6)
+        ops.cache_evict(cache, keep, sinks=2, recent=8, out=(spare, batch.weight, batch.position))
+        for b, n in enumerate(batch.lens):
+            for h in range(kv):
+                for to, of in ref.evict(weight[b, h], position[b, h], n, keep, 2, 8):
+                    t = batch.table[b]
+                    pool[t[to // page], :, h, to % page] = pool[t[of // page], :, h, of % page]
+        assert torch.equal(batch.pool, pool)
+        lens.copy_(spare)
+        assert lens.tolist() == [min(n, keep) for n in batch.lens]
+        outs.append(out)
+        at.add_(1)
+    end = (batch.pool.clone(), batch.weight.clone(), batch.position.clone(), lens.clone())
+    assert lens.tolist() == [keep] * nseq and int(cache.status) == 0
+
+    # the same from one captured step
+    reset()
+    lens.copy_(torch.tensor(lens0, dtype=torch.int32))
+    at.copy_(torch.tensor([500, 9, 38], dtype=torch.int32))
+    x = inputs[0].clone()
+    warm = torch.cuda.Stream()
+    with torch.cuda.stream(warm):
+        one_step(cache, x, at, lens, spare)
+    torch.cuda.synchronize()
+    reset()
+    lens.copy_(torch.tensor(lens0, dtype=torch.int32))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = one_step(cache, x, at, lens, spare)
+        at.add_(1)
+    at.copy_(torch.tensor([500, 9, 38], dtype=torch.int32))
+    for i, more in enumerate(inputs):
+        x.copy_(more)
+        graph.replay()
+        assert torch.equal(out, outs[i])
+    for mine, was in zip((batch.pool, batch.weight, batch.position, lens), end):
+        assert torch.equal(mine, was)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_a_drafting_step(temperature):
+    """Pending token and drafts appended and attended together, verified, the cache cut back to what stays: the next step's rows see what a
+    cache that never held the refused drafts gives."""
+    import torch
+
+    from rustane_b200 import ops
+    kv, heads, hd, page, vocab = 2, 4, 64, 16, 900
+    lens, counts = [40, 17, 90], [4, 1, 6]
+    batch = Batch([n + c for n, c in zip(lens, counts)], counts, kv, hd, page, "f16", seed=31)
+    x = verify_inputs(counts, vocab, "f32", 7, near=0.3, heat=max(temperature, 0.5))
+    rope, cache = ops.Rope(hd), batch.cache()
+    fresh = batch.normal(batch.rows, heads + 2 * kv, hd, dtype="f16")
+    at = torch.cat([torch.arange(n, n + c) for n, c in zip(lens, counts)]).to(torch.int32).cuda()
+    q = ops.rope_append(cache, rope, fresh[:, :heads], fresh[:, heads:heads + kv], fresh[:, heads + kv:], at, batch.row_start)
+    ops.paged_attention(cache, q, batch.row_start, max(counts))
+    accepted, out = ops.verify_drafts(x["target"].cuda(), x["tokens"].cuda(), batch.row_start, max(counts), x["u"].cuda(), x["d"].cuda(), draft=x["draft"].cuda() if temperature else None,
+                                      temperature=temperature)
+    want_n, want = ref.verify(f64(x["target"]), f64(x["draft"]) if temperature else None, x["tokens"].numpy(), f64(x["u"]), f64(x["d"]), batch.starts, temperature)
+    assert accepted.tolist() == want_n.tolist() and out.tolist() == want.tolist()
+    # one more token each on what stays: pending token and accepted drafts
+    kept = [n + 1 + a for n, a in zip(lens, want_n)]
+    batch.tlens.copy_(torch.tensor([n + 1 for n in kept], dtype=torch.int32))
+    one = torch.arange(4, dtype=torch.int32, device="cuda")
+    more = batch.normal(3, heads + 2 * kv, hd, dtype="f16")
+    q = ops.rope_append(cache, rope, more[:, :heads], more[:, heads:heads + kv], more[:, heads + kv:], torch.tensor(kept, dtype=torch.int32, device="cuda"), one)
+    batch.lens, batch.counts, batch.starts, batch.row_start, batch.rows = [n + 1 for n in kept], [1, 1, 1], np.arange(4), one, 3
+    check_attention(batch, heads, "f16", q=q)
+
+
+def test_two_streams_at_once():
+    import torch
+
+    from rustane_b200 import ops
+    jobs = []
+    for i in range(2):
+        batch = Batch([4000 + i, 900], [1, 2], 2, 128, 64, "bf16", seed=40 + i, book=True)
+        jobs.append((batch.cache(), batch.normal(3, 8, 128, dtype="bf16"), batch.row_start, verify_inputs([4, 3], 20000, "bf16", i)))
+    moved = [{k: v.cuda() if hasattr(v, "cuda") else v for k, v in x.items()} for *_, x in jobs]
+
+    def work(i):
+        cache, q, starts, _ = jobs[i]
+        x = moved[i]
+        return (ops.paged_attention(cache, q, starts, 2), *ops.cache_evict(cache, 700, recent=50),
+                *ops.verify_drafts(x["target"], x["tokens"], x["starts"], x["most"], x["u"], x["d"], draft=x["draft"]))
+
+    pools = [j[0].pool.clone() for j in jobs]
+    alone = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for j, was in zip(jobs, pools):
+            j[0].pool.copy_(was)
+        torch.cuda.synchronize()
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(work(i))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_python_refusals():
+    import torch
+
+    from rustane_b200 import ops
+    batch = Batch([20, 30], [1, 1], 2, 64, 16, "f16", seed=1, book=True)
+    cache, q = batch.cache(), batch.normal(2, 4, 64, dtype="f16")
+    k = batch.normal(2, 2, 64, dtype="f16")
+    pos, rope = torch.zeros(2, dtype=torch.int32, device="cuda"), ops.Rope(64)
+    bad = [
+        lambda: ops.PagedCache(batch.pool.cpu(), batch.table, batch.tlens), lambda: ops.PagedCache(batch.pool[:, :1], batch.table, batch.tlens),
+        lambda: ops.PagedCache(batch.pool.double(), batch.table, batch.tlens), lambda: ops.PagedCache(batch.pool, batch.table.long(), batch.tlens),
+        lambda: ops.PagedCache(batch.pool, batch.table, batch.tlens[:1]), lambda: ops.PagedCache(batch.pool, batch.table, batch.tlens.cpu()),
+        lambda: ops.PagedCache(batch.pool, batch.table, batch.tlens, batch.weight), lambda: ops.PagedCache(batch.pool, batch.table, batch.tlens, batch.weight[:, :, 1:], batch.position),
+        lambda: ops.Rope(64, layout="other"), lambda: ops.Rope(64, scaling="other"),
+        lambda: ops.paged_attention(cache, q[0], batch.row_start, 1), lambda: ops.paged_attention(cache, q[:, :, :32], batch.row_start, 1),
+        lambda: ops.paged_attention(cache, q.transpose(0, 1), batch.row_start, 1), lambda: ops.paged_attention(cache, q.cpu(), batch.row_start, 1),
+        lambda: ops.paged_attention(cache, q, batch.row_start[:2], 1), lambda: ops.paged_attention(cache, q, batch.row_start.long(), 1),
+        lambda: ops.paged_attention(cache, q, batch.row_start, 1, out=torch.empty(2, 4, 64, device="cuda")), lambda: ops.paged_attention(cache, q.double(), batch.row_start, 1),
+        lambda: ops.paged_attention(cache, q, batch.row_start, 1, workspace=torch.empty(4, device="cuda")),
+        lambda: ops.rope_append(cache, rope, q, q, k, pos, batch.row_start), lambda: ops.rope_append(cache, rope, q, k, k.float(), pos, batch.row_start),
+        lambda: ops.rope_append(cache, rope, q, k, k, pos[:1], batch.row_start), lambda: ops.rope_append(cache, rope, q, k[:1], k, pos, batch.row_start),
+        lambda: ops.cache_evict(ops.PagedCache(batch.pool, batch.table, batch.tlens), 5), lambda: ops.cache_evict(cache, 5, out=(batch.tlens, batch.weight[:1], batch.position)),
+        lambda: ops.verify_drafts(q, pos, batch.row_start, 1, None, None), lambda: ops.verify_drafts(q[0], pos, batch.row_start, 1, None, None, temperature=0.0),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail("call %d was taken" % i)
+    worse = [
+        lambda: ops.paged_attention(cache, batch.normal(2, 3, 64, dtype="f16"), batch.row_start, 1), lambda: ops.paged_attention(cache, batch.normal(2, 4, 64, dtype="bf16"), batch.row_start, 1),
+        lambda: ops.paged_attention(cache, q, batch.row_start, 0), lambda: ops.paged_attention(cache, q, batch.row_start, 1, window=-1),
+        lambda: ops.paged_attention(cache, q, batch.row_start, 1, workspace=torch.empty(4, dtype=torch.uint8, device="cuda")),
+        lambda: ops.rope_append(cache, ops.Rope(66), q, k, k, pos, batch.row_start), lambda: ops.cache_evict(cache, 5, sinks=3, recent=3),
+        lambda: ops.cache_evict(cache, 5, out=(cache.lens, torch.empty_like(batch.weight), torch.empty_like(batch.position))),
+    ]
+    from rustane_b200 import CudaDecodeError
+    for i, call in enumerate(worse):
+        with pytest.raises(CudaDecodeError):
+            call()
+            pytest.fail("call %d was taken" % i)
