@@ -18,7 +18,7 @@ using namespace cd;
 namespace {
 const char* CALL = "cd_cache_evict";
 constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048, EV_CLUSTER = 8, EV_MOVE_THREADS = 256;
-constexpr int EV_RESIDENT = 45000;  // keys a CTA holds; beyond them they are made again from the weights at every use
+constexpr int EV_RESIDENT = 44000;  // keys a CTA holds; beyond them they are made again from the weights at every use
 
 struct EvictArgs {
     PagedView c;
@@ -37,7 +37,7 @@ __device__ inline uint32_t weight_key(float w) {
 }
 
 struct Shared {
-    alignas(16) uint32_t hist[EV_BINS];
+    alignas(16) uint32_t hist[EV_BINS], total[EV_BINS];  // this CTA's; the cluster's, this CTA's share of the bins
     alignas(16) int warp_sums[EV_WARPS], warp_sums2[EV_WARPS];
     int newest, ties, holes, sources;  // this CTA's, read by the cluster
     uint32_t bin, above;               // of the pass: the bin that holds the keep-th largest, keys above it
@@ -151,17 +151,22 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
             if (pass == 0 || k >> bits == prefix) atomicAdd(&sh.hist[k >> shift & (bins - 1)], 1u);
         }
         sync_all();
-        // from the top: thread t has the four bins below bins - 4 t
-        const int low = bins - 4 - 4 * tid;
-        uint4 sum4 = make_uint4(0, 0, 0, 0);
-        if (low >= 0) {
+        // every CTA adds up its share of the bins; then from the top: thread t has the four bins below bins - 4 t
+        if (tid * 4 < bins / size) {
+            const int at = rank * (bins / size) + tid * 4;
+            uint4 all4 = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < EV_CLUSTER; ++r)
                 if (r < size) {
-                    const uint4 h = *reinterpret_cast<const uint4*>(of_rank(sh.hist, r) + low);
-                    sum4.x += h.x; sum4.y += h.y; sum4.z += h.z; sum4.w += h.w;
+                    const uint4 h = *reinterpret_cast<const uint4*>(of_rank(sh.hist, r) + at);
+                    all4.x += h.x; all4.y += h.y; all4.z += h.z; all4.w += h.w;
                 }
+            *reinterpret_cast<uint4*>(sh.total + tid * 4) = all4;
         }
+        sync_all();
+        const int low = bins - 4 - 4 * tid;
+        uint4 sum4 = make_uint4(0, 0, 0, 0);
+        if (low >= 0) sum4 = *reinterpret_cast<const uint4*>(of_rank(sh.total, low / (bins / size)) + low % (bins / size));
         const uint32_t count[4] = {sum4.w, sum4.z, sum4.y, sum4.x}, sum = sum4.x + sum4.y + sum4.z + sum4.w;
         uint32_t before = sum;
 #pragma unroll
@@ -181,7 +186,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
             }
             before += count[j];
         }
-        sync_all();  // every CTA has read the histograms, too
+        __syncthreads();
         prefix = prefix << width | sh.bin;
         rest -= (int)sh.above;
         equal = sh.red[0];
@@ -374,8 +379,10 @@ extern "C" int cd_cache_evict(const cd_paged_cache* c, int keep, int sinks, int 
     int sms = 0;
     cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return cuda_status(e, CALL);
-    int size = 1;  // one CTA for every 8192 places, so that a pass over the keys stays short
-    while (size < EV_CLUSTER && (long long)size * 8192 < a.c.cap) size *= 2;
+    // CTAs a head: more of them while the GPU has room and each still has 8192 places, and as many as hold the keys.  (208 heads of 33000
+    // entries, one to go: 118 us with eight each, which wait for one another more than they work.)
+    int size = 1;
+    while (size < EV_CLUSTER && ((long long)size * EV_RESIDENT < a.c.cap || ((long long)plan.units * size < 2 * sms && (long long)size * 8192 < a.c.cap))) size *= 2;
     const int per = (a.c.cap + size - 1) / size;
     const bool resident = per <= EV_RESIDENT;
     const size_t shared = resident ? (size_t)per * 4 : 0;

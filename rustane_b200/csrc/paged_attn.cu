@@ -59,9 +59,12 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     if constexpr (std::is_same<KT, float>::value) {
         attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);
     } else {
-        if ((e = allow_shared_memory((const void*)attn_mma_kernel<KT, QT, HD>)) != cudaSuccess) return e;
+        void (*kernel)(AttnArgs) = attn_mma_kernel<KT, QT, HD, 12>;
+        if constexpr (std::is_same<QT, float>::value)
+            if (mma_slots<QT>(a.row_warps) == 8) kernel = attn_mma_kernel<KT, QT, HD, 8>;
+        if ((e = allow_shared_memory((const void*)kernel)) != cudaSuccess) return e;
         const size_t shared = mma_shared<KT, QT, HD>(a.c.nseq, a.row_warps);
-        attn_mma_kernel<KT, QT, HD><<<std::min((shared > 112 * 1024 ? 1 : MMA_CTAS) * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
+        kernel<<<std::min((shared > 112 * 1024 ? 1 : MMA_CTAS) * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const dim3 grid((unsigned)plan.units, (unsigned)std::min<long long>(a.ru, (long long)a.max_rows * a.group));

@@ -219,24 +219,41 @@ template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA
             }
         }
         const int first = w.start + tile * PA_TILE, end = min(w.s.len, first + tiles * PA_TILE);
-        for (int t0 = first + tg * 4 + side; __any_sync(0xffffffffu, t0 < end); t0 += groups * 4) {
-            const int page = t0 < end ? page_at(p.c, b, t0) : -1;
-            float k[NC * VEC], v[NC * VEC];
-            if (page >= 0) {
-                const KT *kr = pool + row_at(p.c, page, 0, kvh, t0, HD), *vr = pool + row_at(p.c, page, 1, kvh, t0, HD);
+        // the next entries' rows are on their way while these are worked on; their page is looked up a step before that
+        uint4 kn[NC], vn[NC];
+        int page_n = -1, word = 0;
+        auto look_up = [&](int t) { word = t < end ? page_word(p.c, b, t) : 0; };
+        auto fetch = [&](int t) {
+            page_n = t < end ? checked_page(p.c, word) : -1;
+            if (page_n >= 0) {
+                const KT *kr = pool + row_at(p.c, page_n, 0, kvh, t, HD), *vr = pool + row_at(p.c, page_n, 1, kvh, t, HD);
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
-                    const uint4 a = __ldg(reinterpret_cast<const uint4*>(kr) + i * 8 + l8), c = __ldg(reinterpret_cast<const uint4*>(vr) + i * 8 + l8);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        k[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&a)[e]);
-                        v[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&c)[e]);
-                    }
+                    kn[i] = __ldg(reinterpret_cast<const uint4*>(kr) + i * 8 + l8);
+                    vn[i] = __ldg(reinterpret_cast<const uint4*>(vr) + i * 8 + l8);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < NC * VEC; ++i) k[i] = v[i] = 0.f;
+                for (int i = 0; i < NC; ++i) kn[i] = vn[i] = make_uint4(0, 0, 0, 0);
             }
+        };
+        const int step = groups * 4;
+        int t0 = first + tg * 4 + side;
+        look_up(t0);
+        fetch(t0);
+        look_up(t0 + step);
+        for (; __any_sync(0xffffffffu, t0 < end); t0 += step) {
+            float k[NC * VEC], v[NC * VEC];
+            const int page = page_n;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    k[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&kn[i])[e]);
+                    v[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&vn[i])[e]);
+                }
+            fetch(t0 + step);
+            look_up(t0 + 2 * step);
 #pragma unroll
             for (int r = 0; r < RW; ++r) {
                 float s = 0.f;

@@ -88,9 +88,11 @@ template <typename KT, typename QT> struct MmaForm {
 };
 constexpr int MMA_STAGE = 8192;  // bytes of a stage: K, then V
 // CTAs an SM, stages of a CTA, which its groups share, and registers of a thread: they leave 8192 of an SM's to the joint's CTAs
-constexpr int MMA_CTAS = 2, MMA_SLOTS = 12, MMA_REGS = 224;
+constexpr int MMA_CTAS = 2, MMA_REGS = 224;
+// (the parts of 32-bit q for several row warps take the room of four stages: two CTAs then still fit an SM)
+template <typename QT> inline int mma_slots(int row_warps) { return std::is_same<QT, float>::value && row_warps > 1 ? 8 : 12; }
 template <typename KT, typename QT, int HD> inline size_t mma_shared(int nseq, int row_warps) {
-    const size_t q = (size_t)row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)MMA_SLOTS * MMA_STAGE;
+    const size_t q = (size_t)row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)mma_slots<QT>(row_warps) * MMA_STAGE;
     const size_t o = (size_t)PA_WARPS * 16 * (HD + 4) * 4;  // (in the ring's place once it is empty)
     return (ring > o ? ring : o) + q + (size_t)(nseq + 1) * 4 + 1024;  // (1024: the ring's own alignment)
 }
@@ -100,13 +102,13 @@ template <int HD> struct MmaShared {
 };
 
 // A run of one unit's tiles, its rows on ROW_WARPS warps.
-template <typename KT, typename QT, int HD, int ROW_WARPS>
+template <typename KT, typename QT, int HD, int ROW_WARPS, int SLOTS>
 __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint4* sq, MmaShared<HD>& sh, const SeqWork& w, int b, int kvh, int block, int tile, int tiles,
                                          bool whole, size_t slot) {
     using X = Mma16<KT>;
     using F = MmaForm<KT, QT>;
     constexpr int NQ = F::NQ, NP = F::NP, RW = 16, PAD = 4, TS = MMA_STAGE / 4 / HD, CH = HD / 8, KS = HD / 16, HALVES = TS / 16;  // TS: entries of a stage
-    constexpr int groups = PA_WARPS / ROW_WARPS, gsize = ROW_WARPS * 32, STAGES = MMA_SLOTS / groups < 4 ? MMA_SLOTS / groups : 4;
+    constexpr int groups = PA_WARPS / ROW_WARPS, gsize = ROW_WARPS * 32, STAGES = SLOTS / groups < 4 ? SLOTS / groups : 4;
     constexpr int PASS = gsize / CH, PASSES = TS / PASS, VOFF = MMA_STAGE / 2;  // PASS: rows that one copy of the whole group brings
     float* so = reinterpret_cast<float*>(ring_all);  // [warps][RW][HD + PAD]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -132,6 +134,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
         if (page16)
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) pages[h] = t0 + 16 * h < end ? page_word(p.c, b, t0 + 16 * h) : 0;
+        else pages[0] = lane < TS && t0 + lane < end ? page_word(p.c, b, t0 + lane) : 0;  // of row `lane`
     };
     uint32_t gaps = 0;                                           // bit s: stage s lacks a page
     const int row0 = gt / CH, ch = gt % CH;                      // this thread's place in a pass
@@ -181,8 +184,9 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
                 look_up(next + groups * TS);
             } else {  // lane r looks up row r (every warp of the group all of them: they agree on gaps)
                 const bool in = lane < TS && next + lane < end;
-                odd_page = in ? page_at(p.c, b, next + lane) : -1;
+                odd_page = in ? checked_page(p.c, pages[0]) : -1;
                 lacks = __any_sync(0xffffffffu, in && odd_page < 0);
+                look_up(next + groups * TS);
             }
             gaps = (gaps & ~(1u << put)) | (uint32_t)lacks << put;
             copy_half(0);
@@ -464,11 +468,11 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
     finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sh.ml}, RW, ROW_WARPS, w, kvh, block, whole, slot);
 }
 
-template <typename KT, typename QT, int HD> __global__ void __maxnreg__(MMA_REGS) attn_mma_kernel(const __grid_constant__ AttnArgs p) {
+template <typename KT, typename QT, int HD, int SLOTS> __global__ void __maxnreg__(MMA_REGS) attn_mma_kernel(const __grid_constant__ AttnArgs p) {
     extern __shared__ char dyn[];
     __shared__ int sums[2 * PA_WARPS];
     __shared__ MmaShared<HD> sh;
-    constexpr size_t RING = (size_t)MMA_SLOTS * MMA_STAGE, OUT = (size_t)PA_WARPS * 16 * (HD + 4) * 4;
+    constexpr size_t RING = (size_t)SLOTS * MMA_STAGE, OUT = (size_t)PA_WARPS * 16 * (HD + 4) * 4;
     char* ring = dyn + ((1024 - (smem_addr(dyn) & 1023)) & 1023);
     uint4* sq = reinterpret_cast<uint4*>(ring + (RING > OUT ? RING : OUT));  // [row warps][NQ][KS][32 lanes]
     int* pre = reinterpret_cast<int*>(sq + (size_t)p.row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32);
@@ -477,9 +481,9 @@ template <typename KT, typename QT, int HD> __global__ void __maxnreg__(MMA_REGS
     const int total = line_up(p, pre, sums, most);
     walk_line(p, pre, total, most, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
         const int rows = min(p.ru, w.s.n * p.group - block * p.ru);
-        if (rows <= 16) mma_unit<KT, QT, HD, 1>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
-        else if (rows <= 32) mma_unit<KT, QT, HD, 2>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
-        else mma_unit<KT, QT, HD, 4>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        if (rows <= 16) mma_unit<KT, QT, HD, 1, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        else if (rows <= 32) mma_unit<KT, QT, HD, 2, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        else mma_unit<KT, QT, HD, 4, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
     });
 }
 

@@ -116,37 +116,20 @@ template <bool HALF, int E> struct Item {
 
 template <typename QT, typename KT, int HD, bool HALF, int E> __global__ void __launch_bounds__(RA_THREADS) rope_append_kernel(const __grid_constant__ AppendArgs p) {
     __shared__ float2 cs[HD / 2];
-    __shared__ int found, s_entry, s_page;
+    __shared__ int found, s_entry[2];
     const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x;
     if (tid == 0) found = 0x7fffffff;
     const int position = p.positions[row];
-    if (tid < p.rot / 2) cs[tid] = cos_sin(p.turns[tid], position, p.magnitude);
-    __syncthreads();
-    for (int b = tid; b < p.c.nseq; b += RA_THREADS)
-        if (p.row_start[b] <= row && row < p.row_start[b + 1]) atomicMin(&found, b);
-    __syncthreads();
-    const int b = found;
-    if (b == 0x7fffffff) return;
-    if (tid == 0) {
-        const BatchSeq s = batch_seq(p.c, p.row_start, b, p.nrows, p.nrows);
-        const int entry = s.len - s.n + row - s.r0;
-        if (s.n > 0 && entry < 0) report(p.c.status, CD_STATUS_BATCH);
-        s_entry = s.n > 0 ? entry : -2;
-        s_page = s.n > 0 && entry >= 0 ? page_at(p.c, b, entry) : -1;
-        if (s_entry < 0) s_entry = s.n > 0 ? -1 : -2;
-    }
-    __syncthreads();
-    const int entry = s_entry, page = s_page;
-    if (entry == -2) return;  // the sequence is left out
     const int per = HALF ? p.rot / 2 / E + (HD - p.rot) / E : HD / E;  // items of a rotated head
     const int rotated = (p.heads + p.c.kv_heads) * per, all = rotated + p.c.kv_heads * (HD / E);
     const QT *q = static_cast<const QT*>(p.q) + row * p.q_stride, *k = static_cast<const QT*>(p.k) + row * p.k_stride, *v = static_cast<const QT*>(p.v) + row * p.v_stride;
     QT* q_out = static_cast<QT*>(p.q_out) + (size_t)row * p.heads * HD;
     KT* pool = static_cast<KT*>(p.c.pool);
+    // the first items are asked for before anything else is known of the row
     constexpr int DEEP = 2;
-    for (int i0 = part * RA_THREADS + tid; i0 < all; i0 += p.parts * RA_THREADS * DEEP) {
-        Item<HALF, E> x[DEEP];
-        int vec[DEEP];  // q heads, k heads, v heads; -1: nothing
+    Item<HALF, E> x[DEEP];
+    int vec[DEEP];  // q heads, k heads, v heads; -1: nothing
+    auto fetch = [&](int i0) {
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
             const int i = i0 + d * p.parts * RA_THREADS;
@@ -161,6 +144,31 @@ template <typename QT, typename KT, int HD, bool HALF, int E> __global__ void __
                 x[d].get(v + (size_t)h * HD, i - rotated - h * (HD / E), 0);
             }
         }
+    };
+    const int step = p.parts * RA_THREADS * DEEP;
+    int i0 = part * RA_THREADS + tid;
+    fetch(i0);
+    if (tid < p.rot / 2) cs[tid] = cos_sin(p.turns[tid], position, p.magnitude);
+    __syncthreads();
+    // the row's sequence (the first that claims it), its entry and page: by the thread that finds it
+    for (int b = tid; b < p.c.nseq; b += RA_THREADS) {
+        const int r0 = p.row_start[b], r1 = p.row_start[b + 1];
+        if (r0 <= row && row < r1) atomicMin(&found, b);
+    }
+    __syncthreads();
+    const int b = found;
+    if (b == 0x7fffffff) return;
+    if (tid == b % RA_THREADS) {
+        const BatchSeq s = batch_seq(p.c, p.row_start, b, p.nrows, p.nrows);
+        const int at = s.len - s.n + row - s.r0;
+        if (s.n > 0 && at < 0) report(p.c.status, CD_STATUS_BATCH);
+        s_entry[0] = s.n > 0 ? max(at, -1) : -2;
+        s_entry[1] = s.n > 0 && at >= 0 ? page_at(p.c, b, at) : -1;
+    }
+    __syncthreads();
+    const int entry = s_entry[0], page = s_entry[1];
+    if (entry == -2) return;  // the sequence is left out
+    while (true) {
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
             const int h = vec[d] - p.heads;
@@ -170,6 +178,9 @@ template <typename QT, typename KT, int HD, bool HALF, int E> __global__ void __
                 x[d].put(pool + row_at(p.c, page, is_v, is_v ? h - p.c.kv_heads : h, entry, HD), is_v ? 0 : p.rot, cs);
             }
         }
+        i0 += step;
+        if (i0 >= all) break;
+        fetch(i0);
     }
     if (p.c.weight && entry >= 0 && part == 0)
         for (int h = tid; h < p.c.kv_heads; h += RA_THREADS) {
