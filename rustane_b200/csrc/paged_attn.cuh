@@ -25,6 +25,7 @@ struct AttnArgs {
     int2* unit_info;  // [units] first CTA, CTAs
     float* lse2;      // [nrows][heads] log2; with scores only
     float* scores;    // [nrows][heads][score_stride] log2 domain, or nullptr
+    unsigned char* odd;  // [ctas][warps][16][hd]: what infinities and NaN that not all rows of a warp see do to those that do (written before it is read)
     long long q_stride, score_stride;
     int weights[3];  // what a tile of a unit of up to 16, 32 and more rows costs on the line; the first is the least
     float scale_log2;

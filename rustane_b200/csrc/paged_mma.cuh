@@ -96,6 +96,42 @@ template <typename KT, typename QT, int HD> inline size_t mma_shared(int nseq, i
     const size_t o = (size_t)PA_WARPS * 16 * (HD + 4) * 4;  // (in the ring's place once it is empty)
     return (ring > o ? ring : o) + q + (size_t)(nseq + 1) * 4 + 1024;  // (1024: the ring's own alignment)
 }
+// What entries with infinities and NaN in V do to rows that see them, where other rows of the unit do not: bits 1 (+inf), 2 (-inf) and 4 (NaN) of
+// the row's and column's sum, set aside (odd_sums, rare and therefore not inline) while the products take zeros for them.
+template <int TS> struct Probs {
+    float p[TS / 8][4];  // as the products have them: e^(score - maximum) of entries 8 n + 2 c + column, rows g and g + 8
+};
+template <typename KT, int HD, int TS>
+__device__ __noinline__ void odd_sums(const uint32_t* v, unsigned char* odd, Probs<TS> s, int t0, int end, int last0, int last1, int window, int lane) {
+    const int g = lane >> 2, c = lane & 3;
+    for (int at = 0; at < TS; ++at) {
+        const int t = t0 + at, from = (lane & ~3) | (at & 7) >> 1;
+        float e0 = 0.f, e1 = 0.f;
+#pragma unroll
+        for (int n = 0; n < TS / 8; ++n)
+            if (at >> 3 == n) {
+                e0 = at & 1 ? s.p[n][1] : s.p[n][0];
+                e1 = at & 1 ? s.p[n][3] : s.p[n][2];
+            }
+        e0 = __shfl_sync(0xffffffffu, e0, from);
+        e1 = __shfl_sync(0xffffffffu, e1, from);
+        if (t >= end) continue;
+        const bool see0 = t <= last0 && (window == 0 || t > last0 - window), see1 = t <= last1 && (window == 0 || t > last1 - window);
+        for (int n = 0; n < HD / 8; ++n) {
+            const uint32_t word = v[at * HD / 2 + ((n ^ (at & 7)) << 2) + c];
+            if (!not_finite<KT>(word)) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float x = as_float(reinterpret_cast<const KT*>(&word)[h]);
+                if (isfinite(x)) continue;
+                auto code = [&](float e) { const float y = e * x; return y != y ? 4 : y > 0.f ? 1 : 2; };
+                if (see0) odd[g * HD + n * 8 + 2 * c + h] |= code(e0);
+                if (see1) odd[(g + 8) * HD + n * 8 + 2 * c + h] |= code(e1);
+            }
+        }
+    }
+}
+
 template <int HD> struct MmaShared {
     float2 ml[PA_WARPS * 16];
     float qscale[4 * 16];
@@ -158,7 +194,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
                 copy16((to ^ ((k * PASS & 7) << 4)) + k * PASS * HD * 2, there ? from[k * PASS / 16] + off + k * PASS % 16 * HD : pool, there);
             }
         } else {
-#pragma unroll
+#pragma unroll 2
             for (int k = 0; k < PASSES; ++k) {
                 const int row = row0 + k * PASS, pg = __shfl_sync(0xffffffffu, odd_page, row);
                 copy16((to ^ ((k * PASS & 7) << 4)) + k * PASS * HD * 2, pg >= 0 ? pool + row_at(p.c, pg, 0, kvh, next + row, HD) + off + ch * 8 : pool, pg >= 0);
@@ -200,56 +236,15 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
         copies_close();
     };
     look_up(next);
-    // q is asked for ahead of the copies, which would otherwise be served first
+    // q comes ahead of the copies of K and V, which would otherwise be served first: as it is, into the place its parts will have
     constexpr int EL = HD / 32, QR = ROW_WARPS * RW / PA_WARPS;  // elements of a lane: EL lane .. EL lane + EL - 1; rows of a warp
-    struct alignas(EL * sizeof(QT)) QWord { QT e[EL]; } q_raw[QR];
-#pragma unroll
-    for (int k = 0; k < QR; ++k) {
-        const int r = warp + k * PA_WARPS;
-        if (r < valid_rows) {
-            const int rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
-            q_raw[k] = *reinterpret_cast<const QWord*>(static_cast<const QT*>(p.q) + (size_t)(w.s.r0 + j) * p.q_stride + (size_t)head * HD + lane * EL);
-        }
+    constexpr int QCH = HD * (int)sizeof(QT) / 16;
+    for (int i = tid; i < ROW_WARPS * RW * QCH; i += PA_THREADS) {
+        const int r = i / QCH, rho = block * p.ru + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
+        const bool there = r < valid_rows;
+        copy16(smem_addr(sq) + i * 16, static_cast<const QT*>(p.q) + (there ? (size_t)(w.s.r0 + j) * p.q_stride + (size_t)head * HD + i % QCH * (16 / sizeof(QT)) : 0), there);
     }
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        issue_k();
-        issue_v();
-    }
-    issue_k();
-    // ---- q, as the products' operand
-#pragma unroll
-    for (int qk = 0; qk < QR; ++qk) {
-        const int r = warp + qk * PA_WARPS;
-        float x[EL];
-#pragma unroll
-        for (int e = 0; e < EL; ++e) x[e] = r < valid_rows ? as_float(q_raw[qk].e[e]) : 0.f;
-        float back = 1.f;
-        if (F::F16 && F::WIDE) {
-            float most = 0.f;
-#pragma unroll
-            for (int e = 0; e < EL; ++e) most = fmaxf(most, fabsf(x[e]));
-            most = warp_max(most);
-            if (most > 0.f && most < INFINITY) {
-                const int ex = max(-100, ilogbf(most)) - 7;
-                back = __int_as_float((127 + ex) << 23);
-                const float by = __int_as_float((127 - ex) << 23);
-#pragma unroll
-                for (int e = 0; e < EL; ++e) x[e] *= by;
-            }
-        }
-        if (lane == 0) sh.qscale[r] = back * p.scale_log2;
-        // row r, column d: register (d % 16 / 8) * 2 + r % 16 / 8 of lane (r % 8) * 4 + d % 8 / 2, k-step d / 16
-#pragma unroll
-        for (int part = 0; part < NQ; ++part)
-#pragma unroll
-            for (int e = 0; e < EL; e += 2) {
-                const int d = lane * EL + e;
-                uint32_t* dst = reinterpret_cast<uint32_t*>(sq + ((size_t)(r / RW * NQ + part) * KS + d / 16) * 32 + (r % 8) * 4 + d % 8 / 2);
-                dst[d % 16 / 8 * 2 + r % RW / 8] = X::part(x[e], x[e + 1]);
-            }
-    }
-    __syncthreads();
+    copies_close();
     float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, scale[2];
     int last[2];
     float* srow[2];
@@ -257,7 +252,6 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
     for (int h = 0; h < 2; ++h) {
         const int r = rw * RW + g + 8 * h, rho = block * p.ru + r, j = rho / p.group;
         last[h] = r < valid_rows ? w.s.len - w.s.n + j : -1;
-        scale[h] = sh.qscale[r];
         srow[h] = p.scores && r < valid_rows ? p.scores + ((size_t)(w.s.r0 + j) * p.heads + kvh * p.group + rho % p.group) * p.score_stride : nullptr;
     }
 #pragma unroll
@@ -269,11 +263,64 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
     const bool mixed = w.s.n > 1 || p.window > 0;
     auto sees = [&](int t, int h) { return t <= last[h] && (p.window == 0 || t > last[h] - p.window); };
 
-    int get = 0;
-    for (int t0 = first + tg * TS; t0 < end; t0 += groups * TS) {
-        copies_wait<2 * STAGES - 2>();
-        group_sync();  // K is there, and V of the step before has been read
-        issue_v();
+    bool any_odd = false;
+    unsigned char* odd_at = p.odd + ((size_t)blockIdx.x * PA_WARPS + warp) * RW * HD;  // this warp's rows and columns
+    // Steps below 0 only issue copies: V of step it + STAGES - 1, K of step it + STAGES.  (One loop, so that the copies stand in the code
+    // once: at its start a kernel waits for its instructions more than for anything else.)
+    int get = 0, t0 = first + (tg - STAGES * groups) * TS;
+#pragma unroll 1
+    for (int it = -STAGES; it <= 0 || t0 < end; ++it, t0 += groups * TS) {
+        const bool work = it >= 0 && t0 < end;
+        if (it == 0) {  // ---- q, as the products' operand
+            copies_wait<2 * STAGES - 1>();
+            __syncthreads();
+            float x[QR][EL];
+#pragma unroll
+            for (int qk = 0; qk < QR; ++qk)
+#pragma unroll
+                for (int e = 0; e < EL; ++e) x[qk][e] = as_float(reinterpret_cast<const QT*>(sq)[(warp + qk * PA_WARPS) * HD + lane * EL + e]);
+            __syncthreads();
+#pragma unroll
+            for (int qk = 0; qk < QR; ++qk) {
+                const int r = warp + qk * PA_WARPS;
+                float back = 1.f;
+                if (F::F16 && F::WIDE) {
+                    float most = 0.f;
+#pragma unroll
+                    for (int e = 0; e < EL; ++e) most = fmaxf(most, fabsf(x[qk][e]));
+                    most = warp_max(most);
+                    if (most > 0.f && most < INFINITY) {
+                        const int ex = max(-100, ilogbf(most)) - 7;
+                        back = __int_as_float((127 + ex) << 23);
+                        const float by = __int_as_float((127 - ex) << 23);
+#pragma unroll
+                        for (int e = 0; e < EL; ++e) x[qk][e] *= by;
+                    }
+                }
+                if (lane == 0) sh.qscale[r] = back * p.scale_log2;
+                // row r, column d: register (d % 16 / 8) * 2 + r % 16 / 8 of lane (r % 8) * 4 + d % 8 / 2, k-step d / 16
+#pragma unroll
+                for (int part = 0; part < NQ; ++part)
+#pragma unroll
+                    for (int e = 0; e < EL; e += 2) {
+                        const int d = lane * EL + e;
+                        uint32_t* dst = reinterpret_cast<uint32_t*>(sq + ((size_t)(r / RW * NQ + part) * KS + d / 16) * 32 + (r % 8) * 4 + d % 8 / 2);
+                        dst[d % 16 / 8 * 2 + r % RW / 8] = X::part(x[qk][e], x[qk][e + 1]);
+                    }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) scale[h] = sh.qscale[rw * RW + g + 8 * h];
+        }
+        if (work) {
+            copies_wait<2 * STAGES - 2>();
+            group_sync();  // K is there, and V of the step before has been read
+        }
+        if (it > -STAGES) issue_v();
+        if (!work) {
+            issue_k();
+            continue;
+        }
         const bool lacks = gaps >> get & 1u;
         const uint32_t stage = ring + get * MMA_STAGE;
         // scores s[n][row half * 2 + column] of entries t0 + 8 n + 2 c + column; two k-steps' operands at a time, into two sets of sums in turn
@@ -373,36 +420,17 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
             const uint32_t* v = reinterpret_cast<const uint32_t*>(ring_all + (stage - ring_base) + VOFF);
             bool odd = false;
             for (int at = lane; at < TS * HD / 2; at += 32) odd |= not_finite<KT>(v[at]);
-            if (__any_sync(0xffffffffu, odd)) {  // rare: what is not finite goes, entry by entry, to the rows that see it
-#pragma unroll 1
-                for (int at = 0; at < TS; ++at) {
-                    const int t = t0 + at, lane_of = (lane & ~3) | (at & 7) >> 1;
-                    float e0 = 0.f, e1 = 0.f;
+            if (__any_sync(0xffffffffu, odd)) {
+                Probs<TS> probs;
 #pragma unroll
-                    for (int n = 0; n < TS / 8; ++n)
-                        if (at >> 3 == n) {
-                            e0 = at & 1 ? s[n][1] : s[n][0];
-                            e1 = at & 1 ? s[n][3] : s[n][2];
-                        }
-                    e0 = __shfl_sync(0xffffffffu, e0, lane_of);
-                    e1 = __shfl_sync(0xffffffffu, e1, lane_of);
-                    if (t >= end) continue;
-                    const bool see0 = sees(t, 0), see1 = sees(t, 1);
+                for (int n = 0; n < TS / 8; ++n)
 #pragma unroll
-                    for (int n = 0; n < CH; ++n) {
-                        const uint32_t word = v[at * HD / 2 + ((n ^ (at & 7)) << 2) + c];
-                        if (!not_finite<KT>(word)) continue;
-                        const float v0 = as_float(reinterpret_cast<const KT*>(&word)[0]), v1 = as_float(reinterpret_cast<const KT*>(&word)[1]);
-                        if (!isfinite(v0)) {
-                            if (see0) o[n][0] = fmaf(e0, v0, o[n][0]);
-                            if (see1) o[n][2] = fmaf(e1, v0, o[n][2]);
-                        }
-                        if (!isfinite(v1)) {
-                            if (see0) o[n][1] = fmaf(e0, v1, o[n][1]);
-                            if (see1) o[n][3] = fmaf(e1, v1, o[n][3]);
-                        }
-                    }
-                }
+                    for (int e = 0; e < 4; ++e) probs.p[n][e] = s[n][e];
+                if (!any_odd)
+                    for (int i = lane; i < RW * HD / 16; i += 32) reinterpret_cast<uint4*>(odd_at)[i] = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+                odd_sums<KT, HD, TS>(v, odd_at, probs, t0, end, last[0], last[1], p.window, lane);
+                any_odd = true;
                 group_sync();  // the group's warps have all read the stage: take what is not finite out of it
                 uint32_t* clean = const_cast<uint32_t*>(v);
                 for (int at = gt; at < TS * HD / 2; at += gsize) clean[at] = finite_part<KT>(clean[at]);
@@ -461,8 +489,15 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
         const int r = warp * RW + g + 8 * h;
         if (c == 0) sh.ml[r] = make_float2(m[h], l[h] * DOWN);
 #pragma unroll
-        for (int n = 0; n < CH; ++n)
+        for (int n = 0; n < CH; ++n) {
+            if (any_odd)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int code = odd_at[(g + 8 * h) * HD + n * 8 + 2 * c + e];
+                    if (code) o[n][2 * h + e] = code == 1 ? INFINITY : code == 2 ? -INFINITY : NAN;
+                }
             *reinterpret_cast<float2*>(so + (size_t)r * (HD + PAD) + n * 8 + 2 * c) = make_float2(o[n][2 * h] * DOWN, o[n][2 * h + 1] * DOWN);
+        }
     }
     __syncthreads();
     finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sh.ml}, RW, ROW_WARPS, w, kvh, block, whole, slot);
