@@ -1,11 +1,14 @@
 // cd_cache_evict: every sequence and kv head of a paged cache down to its `keep` heaviest entries.
 //
 // evict_select_kernel: a cluster of CTAs per (sequence, kv head) brings the entries' weights into shared memory as ordered 32-bit keys
-// and finds the keep-th largest by three histograms (11, 11 and 10 bits), joined over the cluster through distributed shared memory; equal keys
-// are counted off in order of place.  Survivors in places >= keep pair up with the holes below in order, so an entry moves
-// at most once, only as many move as have to (one, for a cache that grows by one a step), sources and targets never
-// overlap, and nothing but the two lists of places goes through memory.
-// evict_move_kernel: the pairs of all heads, spread over the GPU, 16 bytes a thread at a time.
+// and finds the keep-th largest by up to three histograms (11, 11 and 10 bits; none more than needed), joined over the cluster through
+// distributed shared memory, every CTA adding up its share of the bins; equal keys are counted off in order of place.  Survivors in
+// places >= keep pair up with the holes below in order, so an entry moves at most once, only as many move as have to (one, for a cache
+// that grows by one a step), sources and targets never overlap, and nothing but the two lists of places goes through memory.
+// Bound by its chain of barriers and memory latencies: 36 us for 32 heads of 60001 entries in clusters of eight, 11 us for 128 heads
+// of 2049.  (One loop of loads after the other, and histograms read word by word from every CTA of the cluster: 95 and 20 us.)
+// evict_move_kernel: the pairs of all heads, spread over the GPU, 16 bytes a thread, four pairs under way.  Bound by rows of 256 bytes
+// from all over the pool: 360000 pairs, 368 MB, 88 us, 4.2 TB/s (109 us with one pair at a time).
 #include <cooperative_groups.h>
 
 #include <algorithm>

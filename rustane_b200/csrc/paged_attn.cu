@@ -14,7 +14,8 @@ struct Plan {
     size_t units, part_o, part_ml, unit_info, odd, lse2, scores, bytes;  // offsets in the workspace
     long long score_stride;
 };
-// What a tile costs by its unit's rows: up to 16, 32, more (tensor-core form).
+// What a tile costs by its unit's rows: up to 16, 32, more (tensor-core form).  A CTA's four warps work on four places at once, on two, on
+// one; HBM evens out part of it.  24 sequences of one to six drafted rows, eight heads a kv head: 126 us with equal costs, 109 with these.
 constexpr int PA_WEIGHTS[3] = {2, 3, 6};
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 

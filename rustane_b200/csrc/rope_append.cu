@@ -1,9 +1,10 @@
 // cd_rope_append: rotary positions of a batch's new rows, K and V into their pages, in one pass over q, k and v.
 //
-// A CTA has one row (or a part of its heads, where there are few rows): it finds the row's sequence and entry, puts the row's
-// cosines and sines into shared memory once for all heads, and then moves eight elements a thread at a time: every element is
-// read once and written once.  Bound by those bytes on a long prompt, by the launch and three dependent loads
-// (row_start, lens and the page table, then the row) on a token.
+// A CTA has one row (or a part of its heads, where there are few rows): it asks for its first elements, finds the row's sequence and entry
+// meanwhile, puts the row's cosines and sines into shared memory once for all heads, and moves eight elements a thread at a time,
+// two such items under way: every element is read once and written once.  Bound by those bytes on a long prompt (8184 rows of 64
+// heads, 469 MB, 74 us: 6.3 TB/s, 98 % of the copy rate; 99 us with one item at a time), by the launch and the chain of row_start,
+// lens, page table and store on a token (four tokens 4.1 us).
 //
 // Angles: position * turns modulo 2^64 is the exact fraction of a turn; its upper half, brought into an eighth of a turn either
 // way, is exact in 30 bits and rounds once to fp32 (off by at most 2^-24 of the reduced angle), at any position.
