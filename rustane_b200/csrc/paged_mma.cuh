@@ -300,7 +300,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
                         for (int e = 0; e < EL; ++e) x[qk][e] *= by;
                     }
                 }
-                if (lane == 0) sh.qscale[r] = back * p.scale_log2;
+                if (lane == 0) sh.qscale[r] = fmaxf(back * p.scale_log2, 1e-37f);  // (0 times a masked score would be NaN)
                 // row r, column d: register (d % 16 / 8) * 2 + r % 16 / 8 of lane (r % 8) * 4 + d % 8 / 2, k-step d / 16
 #pragma unroll
                 for (int part = 0; part < NQ; ++part)
