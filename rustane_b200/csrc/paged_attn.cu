@@ -15,8 +15,8 @@ struct Plan {
     long long score_stride;
 };
 // What a tile costs by its unit's rows: up to 16, 32, more (tensor-core form).  A CTA's four warps work on four places at once, on two, on
-// one; HBM evens out part of it.  24 sequences of one to six drafted rows, eight heads a kv head: 126 us with equal costs, 109 with these.
-constexpr int PA_WEIGHTS[3] = {2, 3, 6};
+// one; HBM evens out part of it.  24 sequences of one to six drafted rows, eight heads a kv head: 93 us with costs of 1, 1 and 2, 87 with these.
+constexpr int PA_WEIGHTS[3] = {2, 4, 7};
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // A warp has 4 rows of a unit with an fp32 pool (FMAs), 16 with a 16-bit one (tensor cores); a unit as many of its warps as its rows need.
@@ -61,12 +61,18 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     if constexpr (std::is_same<KT, float>::value) {
         attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);
     } else {
-        void (*kernel)(AttnArgs) = attn_mma_kernel<KT, QT, HD, 12>;
-        if constexpr (std::is_same<QT, float>::value)
-            if (mma_slots<QT>(a.row_warps) == 8) kernel = attn_mma_kernel<KT, QT, HD, 8>;
+        using Size = MmaSize<QT, HD>;
+        const bool few = Size::slots(a.row_warps) == 8;
+        void (*kernel)(AttnArgs) = attn_mma_kernel<KT, QT, HD, 12, 224>;
+        if constexpr (Size::WIDE) {
+            if (few) kernel = attn_mma_kernel<KT, QT, HD, 8, 224>;
+        } else if constexpr (HD == 64) {
+            if (few) kernel = attn_mma_kernel<KT, QT, HD, 8, 160>;
+        }
         if ((e = allow_shared_memory((const void*)kernel)) != cudaSuccess) return e;
         const size_t shared = mma_shared<KT, QT, HD>(a.c.nseq, a.row_warps);
-        kernel<<<std::min((shared > 112 * 1024 ? 1 : MMA_CTAS) * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
+        const int fit = (int)(226 * 1024 / (shared + 2560));  // (and what the kernel has of its own and the system takes a CTA)
+        kernel<<<std::min(std::max(1, std::min(fit, Size::three(a.row_warps) ? 3 : 2)) * sms, PA_MAX_CTAS), PA_THREADS, shared, s>>>(a);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const dim3 grid((unsigned)plan.units, (unsigned)std::min<long long>(a.ru, (long long)a.max_rows * a.group));

@@ -6,9 +6,9 @@
 // bits of its place (chunk ^ place & 7), so that ldmatrix meets every bank once and an address is one XOR.  A group of one warp meets no
 // barrier inside the loop.
 //
-// What bounds it: HBM where one warp has a unit's rows (5.5 TB/s on a ragged batch of 48 over 1.6 GB; 130001 entries of four heads, 266 MB, 56 us
+// What bounds it: HBM where one warp has a unit's rows (5.5 TB/s on a ragged batch of 48 over 1.6 GB; 130001 entries of four heads, 266 MB, 55 us
 // with their joint: 4.7 TB/s, the rest is the launch, the line and the ends of two kernels), the chain of a step's instructions, 5 to 9
-// cycles each, where four do (48 rows over 167 MB 93 us), and the way to the first instruction of everything on a token of a few
+// cycles each, where four do (48 rows over 167 MB 88 us), and the way to the first instruction of everything on a token of a few
 // chats (11 us): a kernel's first pass waits for its code more than for data, so copies and rare cases stand in the code once.
 //
 // Forms measured on the way (the kernel alone, 130001 entries): K and V straight to registers, no ring, 70 us; boxes by TMA, issued by a
@@ -90,12 +90,17 @@ template <typename KT, typename QT> struct MmaForm {
     static constexpr int SHIFT = F16 ? (NP == 2 ? 12 : 8) : 0;  // P is times 2^SHIFT: fp16 parts of small ones keep their digits
 };
 constexpr int MMA_STAGE = 8192;  // bytes of a stage: K, then V
-// CTAs an SM, stages of a CTA, which its groups share, and registers of a thread: they leave 8192 of an SM's to the joint's CTAs
-constexpr int MMA_CTAS = 2, MMA_REGS = 224;
-// (the parts of 32-bit q for several row warps take the room of four stages: two CTAs then still fit an SM)
-template <typename QT> inline int mma_slots(int row_warps) { return std::is_same<QT, float>::value && row_warps > 1 ? 8 : 12; }
+// CTAs an SM, and stages of a CTA, which its groups share: two of twelve, at 224 registers a thread (they leave room for the joint's CTAs).
+// Half the columns need half the sums: at hd 64, with units of one row warp, three CTAs of eight stages at 160 registers (48 sequences of up to
+// 822 entries, 16 kv heads: 65 us for 69; but 106 for 88 on drafted rows, whose groups of four warps want the deeper ring).  The parts
+// of 32-bit q for several row warps take the room of four stages.
+template <typename QT, int HD> struct MmaSize {
+    static constexpr bool WIDE = std::is_same<QT, float>::value;
+    static bool three(int row_warps) { return HD == 64 && !WIDE && row_warps == 1; }
+    static int slots(int row_warps) { return three(row_warps) || (WIDE && row_warps > 1) ? 8 : 12; }
+};
 template <typename KT, typename QT, int HD> inline size_t mma_shared(int nseq, int row_warps) {
-    const size_t q = (size_t)row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)mma_slots<QT>(row_warps) * MMA_STAGE;
+    const size_t q = (size_t)row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)MmaSize<QT, HD>::slots(row_warps) * MMA_STAGE;
     const size_t o = (size_t)PA_WARPS * 16 * (HD + 4) * 4;  // (in the ring's place once it is empty)
     return (ring > o ? ring : o) + q + (size_t)(nseq + 1) * 4 + 1024;  // (1024: the ring's own alignment)
 }
@@ -506,7 +511,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
     finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sh.ml}, RW, ROW_WARPS, w, kvh, block, whole, slot);
 }
 
-template <typename KT, typename QT, int HD, int SLOTS> __global__ void __maxnreg__(MMA_REGS) attn_mma_kernel(const __grid_constant__ AttnArgs p) {
+template <typename KT, typename QT, int HD, int SLOTS, int REGS> __global__ void __maxnreg__(REGS) attn_mma_kernel(const __grid_constant__ AttnArgs p) {
     extern __shared__ char dyn[];
     __shared__ int sums[2 * PA_WARPS];
     __shared__ MmaShared<HD> sh;
