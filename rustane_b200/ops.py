@@ -90,7 +90,16 @@ def _row_stride(t, what, rows, hd, index):
     row, head, one = t.stride()
     if one != 1 or (head != hd and shape[1] != 1):
         raise ValueError("%s: the heads of a row must lie next to each other" % what)
-    return row if rows > 1 else 0
+    return _distance(row, what, rows)
+
+
+def _distance(stride, what, rows):
+    """A stride of rows for the library, where 0 is packed: rows broadcast from one are refused."""
+    if rows <= 1:
+        return 0
+    if stride == 0:
+        raise ValueError("%s: broadcast rows have to be made contiguous first" % what)
+    return stride
 
 
 def _check(rc):
@@ -267,8 +276,8 @@ def verify_drafts(target, tokens, row_start, max_rows, uniforms, draws, draft=No
         need = _VERIFY[(rows, nseq, vocab)] = n.value
     ws = _workspace(workspace, need, device)
     random = temperature != 0
-    _check(lib.cd_verify_drafts(index, _code(target, "target"), nseq, rows, max_rows, vocab, target.data_ptr(), target.stride(0) if rows > 1 else 0,
-                                None if draft is None else draft.data_ptr(), 0 if draft is None or rows < 2 else draft.stride(0),
+    _check(lib.cd_verify_drafts(index, _code(target, "target"), nseq, rows, max_rows, vocab, target.data_ptr(), _distance(target.stride(0), "target", rows),
+                                None if draft is None else draft.data_ptr(), 0 if draft is None else _distance(draft.stride(0), "draft", rows),
                                 _tensor(tokens, "tokens", torch.int32, (rows,), index), starts,
                                 _tensor(uniforms, "uniforms", torch.float32, (rows,), index) if random else None,
                                 _tensor(draws, "draws", torch.float32, (nseq,), index) if random else None, temperature, accepted.data_ptr(),

@@ -507,6 +507,19 @@ def test_verify_strided_rows_unaligned_and_rows_behind_the_batch():
     assert accepted.tolist() == want_n.tolist() and out.tolist()[:6] == want.tolist()
 
 
+def test_verify_refuses_broadcast_logits():
+    import torch
+
+    from rustane_b200 import ops
+    x = verify_inputs([4, 2], 1001, "f16", 10)
+    tokens, starts, u, d = (x[k].cuda() for k in ("tokens", "starts", "u", "d"))
+    target, draft = x["target"].cuda(), x["draft"].cuda()
+    with pytest.raises(ValueError, match="target: broadcast"):
+        ops.verify_drafts(target[:1].expand(6, 1001), tokens, starts, 4, u, d)
+    with pytest.raises(ValueError, match="draft: broadcast"):
+        ops.verify_drafts(target, tokens, starts, 4, u, d, draft=draft[:1].expand(6, 1001))
+
+
 def test_verify_leaves_out_sequences_whose_rows_do_not_fit():
     import torch
 

@@ -142,3 +142,18 @@ def test_rope_frequencies_refuses(R, args):
     from rustane_b200 import ops
     with pytest.raises(R.CudaDecodeError):
         ops.rope_frequencies(*args)
+
+
+def test_broadcast_rows_are_refused():
+    # the library reads a stride of 0 as packed rows, which a tensor broadcast from one row does not have
+    import torch
+
+    from rustane_b200 import ops
+    one = torch.zeros(1, 2, 64)
+    with pytest.raises(ValueError, match="q: broadcast"):
+        ops._row_stride(one.expand(3, 2, 64), "q", 3, 64, -1)
+    with pytest.raises(ValueError, match="next to each other"):
+        ops._row_stride(torch.zeros(3, 1, 64).expand(3, 2, 64), "q", 3, 64, -1)
+    assert ops._row_stride(one, "q", 1, 64, -1) == 0
+    assert ops._row_stride(one.expand(1, 2, 64), "q", 1, 64, -1) == 0
+    assert ops._row_stride(torch.zeros(3, 6, 64)[:, 2:4], "q", 3, 64, -1) == 384
