@@ -102,6 +102,13 @@ def _distance(stride, what, rows):
     return stride
 
 
+def _counts(*counts):
+    """Counts for the library's 32-bit integers, which would keep the low bits of larger ones."""
+    for n in counts:
+        if not -0x80000000 <= n <= 0x7fffffff:
+            raise ValueError("a count must fit 32 bits, got %d" % n)
+
+
 def _check(rc):
     if rc:
         raise CudaDecodeError(rc, lib.cd_last_error(None).decode())
@@ -221,6 +228,7 @@ def paged_attention(cache, q, row_start, max_rows, scale=None, window=0, collect
     """Attention of the new rows q [rows, heads, hd] (f32 or of the pool's type) over the cache, each row up to its own entry, or over its last
     `window` entries.  max_rows: the most rows a sequence has.  collect: add the probabilities to cache.weight.  Returns out, or
     (out, lse [rows, heads] f32) with lse.  Rows from row_start[nseq] on are not written."""
+    _counts(max_rows, window)
     index = cache._index
     shape = q.shape
     rows, heads, collect = shape[0], shape[1], 1 if collect else 0
@@ -239,6 +247,7 @@ def cache_evict(cache, keep, sinks=0, recent=0, out=None, workspace=None):
     """Bring every sequence with more than `keep` entries down to `keep`, each kv head by its own weights; positions below `sinks` and the
     newest `recent` ones stay.  K and V move within the cache's pages.  Returns new (lens, weight, position), which the caller
     hands to cache.replace(); out: tensors for them (weight and position may be the cache's own, lens may not)."""
+    _counts(keep, sinks, recent)
     index = cache._index
     if cache.weight is None:
         raise ValueError("the cache has no weight and position")
@@ -257,6 +266,7 @@ def verify_drafts(target, tokens, row_start, max_rows, uniforms, draws, draft=No
     draft [rows, vocab]: the logits the token behind each row was drawn from, None: drafts without a distribution.  Returns
     (accepted [nseq] int32, out_tokens [rows] int32: the drafts that stay, the drawn token, then -1)."""
     _load_torch()
+    _counts(max_rows)
     device, shape = target.device, target.shape
     index = device.index
     if not target.is_cuda or len(shape) != 2 or (shape[1] > 1 and target.stride(1) != 1):

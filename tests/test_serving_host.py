@@ -157,3 +157,16 @@ def test_broadcast_rows_are_refused():
     assert ops._row_stride(one, "q", 1, 64, -1) == 0
     assert ops._row_stride(one.expand(1, 2, 64), "q", 1, 64, -1) == 0
     assert ops._row_stride(torch.zeros(3, 6, 64)[:, 2:4], "q", 3, 64, -1) == 384
+
+
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1])
+def test_counts_past_32_bits_are_refused(R, n):
+    # (ahead of everything else: no cache is looked at)
+    import torch
+
+    from rustane_b200 import ops
+    for call in (lambda: ops.paged_attention(None, None, None, 1, window=n), lambda: ops.paged_attention(None, None, None, n),
+                 lambda: ops.cache_evict(None, n), lambda: ops.cache_evict(None, 5, sinks=n), lambda: ops.cache_evict(None, 5, recent=n),
+                 lambda: ops.verify_drafts(torch.zeros(1, 2), None, None, n, None, None)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
