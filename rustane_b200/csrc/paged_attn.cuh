@@ -8,11 +8,12 @@
 // and join_kernel puts them together in the line's order.  Inside a CTA four warps share a unit: `row_warps` of them have different rows of
 // the same entries, the rest other entries.  Statistics are fp32 in the log2 domain.
 #pragma once
+#include "paged_span.h"
 #include "serve.cuh"
 
 namespace cd {
 
-constexpr int PA_THREADS = 128, PA_WARPS = 4, PA_TILE = 64, PA_MAX_CTAS = 640;
+constexpr int PA_THREADS = 128, PA_WARPS = 4, PA_MAX_CTAS = 640;
 
 struct AttnArgs {
     PagedView c;
@@ -39,12 +40,9 @@ struct SeqWork {
 __device__ inline SeqWork seq_work(const AttnArgs& p, int b) {
     SeqWork w;
     w.s = batch_seq(p.c, p.row_start, b, p.nrows, p.max_rows);
-    w.start = 0;
-    if (p.window > 0) {
-        const int first = w.s.len - w.s.n + 1 - p.window;  // of the first row
-        w.start = first > 0 ? first & ~(PA_TILE - 1) : 0;
-    }
-    w.tiles = w.s.n > 0 && w.s.len > 0 ? (w.s.len - w.start + PA_TILE - 1) / PA_TILE : 0;
+    const PaSpan span = pa_span(w.s.len, w.s.n, p.window);
+    w.start = span.start;
+    w.tiles = span.tiles;
     const int rows = w.s.n * p.group;
     w.blocks = (rows + p.ru - 1) / p.ru;
     w.weight = p.weights[rows <= 16 ? 0 : rows <= 32 ? 1 : 2];
@@ -264,7 +262,7 @@ template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA
                 for (int i = 0; i < NC * VEC; ++i) s = fmaf(q[r][i], k[i], s);
 #pragma unroll
                 for (int x = 1; x < 8; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-                const bool seen = page >= 0 && t0 <= last[r] && (p.window == 0 || t0 > last[r] - p.window);
+                const bool seen = page >= 0 && pa_sees(t0, last[r], p.window);
                 if (!seen) s = -INFINITY;
                 if (srow[r] && l8 == r && t0 < end) srow[r][t0] = s;
                 if (!seen) continue;  // what is masked does not reach the sums, whatever its V holds

@@ -124,7 +124,7 @@ __device__ __noinline__ void odd_sums(const uint32_t* v, unsigned char* odd, Pro
         e0 = __shfl_sync(0xffffffffu, e0, from);
         e1 = __shfl_sync(0xffffffffu, e1, from);
         if (t >= end) continue;
-        const bool see0 = t <= last0 && (window == 0 || t > last0 - window), see1 = t <= last1 && (window == 0 || t > last1 - window);
+        const bool see0 = pa_sees(t, last0, window), see1 = pa_sees(t, last1, window);
         for (int n = 0; n < HD / 8; ++n) {
             const uint32_t word = v[at * HD / 2 + ((n ^ (at & 7)) << 2) + c];
             if (!not_finite<KT>(word)) continue;
@@ -269,7 +269,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
     const uint4* q4 = sq + (size_t)rw * NQ * KS * 32 + lane;
     const int all_see = w.s.len - w.s.n, none_out = p.window > 0 ? w.s.len - p.window : 0;  // every row sees entries none_out .. all_see
     const bool mixed = w.s.n > 1 || p.window > 0;
-    auto sees = [&](int t, int h) { return t <= last[h] && (p.window == 0 || t > last[h] - p.window); };
+    auto sees = [&](int t, int h) { return pa_sees(t, last[h], p.window); };
 
     bool any_odd = false;
     unsigned char* odd_at = p.odd + ((size_t)blockIdx.x * PA_WARPS + warp) * RW * HD;  // this warp's rows and columns
