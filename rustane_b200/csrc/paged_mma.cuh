@@ -17,10 +17,10 @@
 //
 // mma.sync and not tcgen05: a token's unit has 1 to 16 rows, of a 64-row minimum there, and the work is bound by the bytes of K and V.
 //
-// Exactness: q of 32 bits is two fp16 parts (scaled by a power of two per row) or three bf16 parts, P two or three parts with an fp32
-// result or a bf16 pool (a single bf16 P would cost 2^-9 a term, half the result's own rounding) and one with fp16 (2^-12).  Sums
-// stay in 32 bits; with an fp32 result every step's product goes to fresh accumulators and is added by the CUDA cores, which round
-// to nearest where the tensor cores cut off.
+// Exactness: q of 32 bits is two fp16 parts (scaled by a power of two per row) or three bf16 parts, P two parts or (bf16 pool, fp32 result)
+// three: in one part every term would be off by 2^-12 (fp16) or 2^-9 (bf16) of itself, which terms that cancel leave of a small
+// sum.  Sums stay in 32 bits; with an fp32 result every step's product goes to fresh accumulators and is added by the CUDA cores,
+// which round to nearest where the tensor cores cut off.
 #pragma once
 #include "paged_attn.cuh"
 
@@ -86,8 +86,8 @@ template <> __device__ inline void product<__nv_bfloat16>(float (&d)[4], const u
 
 template <typename KT, typename QT> struct MmaForm {
     static constexpr bool F16 = std::is_same<KT, __half>::value, WIDE = std::is_same<QT, float>::value;
-    static constexpr int NQ = WIDE ? (F16 ? 2 : 3) : 1, NP = WIDE ? (F16 ? 2 : 3) : F16 ? 1 : 2;
-    static constexpr int SHIFT = F16 ? (NP == 2 ? 12 : 8) : 0;  // P is times 2^SHIFT: fp16 parts of small ones keep their digits
+    static constexpr int NQ = WIDE ? (F16 ? 2 : 3) : 1, NP = WIDE && !F16 ? 3 : 2;
+    static constexpr int SHIFT = F16 ? 12 : 0;  // P is times 2^SHIFT: fp16 parts of small ones keep their digits
 };
 constexpr int MMA_STAGE = 8192;  // bytes of a stage: K, then V
 // CTAs an SM, and stages of a CTA, which its groups share: two of twelve, at 224 registers a thread (they leave room for the joint's CTAs).

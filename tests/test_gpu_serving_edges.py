@@ -26,3 +26,25 @@ def test_a_window_wider_than_every_sequence_is_none(q_type, kv_type, window):
     np.testing.assert_array_equal(f64(lse), f64(want_lse))
     assert np.isneginf(f64(lse[:3])).all() and (f64(out[:3]) == 0).all() and np.isfinite(f64(lse[3])).all()  # three of four rows ahead of the one entry
     assert int(cache.status) == 0
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("pairs", [1, 40])
+def test_probabilities_of_terms_that_cancel(q_type, kv_type, pairs):
+    """V is +1 and -1 in turn, and the scores (exact: one product each) differ by i / 1024 a sequence: what is left of the sum is small, so that a probability
+    rounded to 11 bits would show.  Allowed: the result's rounding, and of the terms' sum 2^-20 (fp32 sums of up to 80 terms and their
+    exponentials: 2^-22 each for 2^x and the score's scaling, 2^-24 a sum), with bf16 rows over bf16 2^-16 for P in two parts."""
+    from rustane_b200 import ops
+    n = 64
+    batch = Batch([2 * pairs] * n, [1] * n, 1, 64, 16, kv_type, seed=1, values=False)
+    for b in range(n):
+        for t in range(2 * pairs):
+            at = batch.pool[int(batch.table[b, t // 16]), :, 0, t % 16]
+            at[0, 0] = (t % 2) * (b + 1) / 1024.0
+            at[1] = 1.0 - 2.0 * (t % 2)
+    q = batch.normal(n, 1, 64, dtype=q_type).zero_()
+    q[:, :, 0] = 1.0
+    out = ops.paged_attention(batch.cache(), q, batch.row_start, 1, scale=1.0)
+    want, _, mass, _, _ = ref.attention(batch, q, 1.0)
+    part = 2.0 ** -16 if q_type == "bf16" else 2.0 ** -20
+    assert (np.abs(f64(out) - want) <= HALF_STEP[q_type] * np.abs(want) + part * mass).all(), np.abs(f64(out) - want).max()
