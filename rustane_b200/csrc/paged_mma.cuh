@@ -253,7 +253,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
         copy16(smem_addr(sq) + i * 16, static_cast<const QT*>(p.q) + (there ? (size_t)(w.s.r0 + j) * p.q_stride + (size_t)head * HD + i % QCH * (16 / sizeof(QT)) : 0), there);
     }
     copies_close();
-    float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, scale[2];
+    float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, scale[2];  // m: largest score before its scale, which is positive
     int last[2];
     float* srow[2];
 #pragma unroll
@@ -394,13 +394,13 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
             for (int n = 1; n < TS / 8; ++n) x = fmaxf(x, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-            top[h] = fmaxf(m[h], x * scale[h]);  // (scale is positive)
+            top[h] = fmaxf(m[h], x);
             raise |= top[h] > m[h];
         }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float f = top[h] == -INFINITY ? 1.f : ex2(m[h] - top[h]);
+                const float f = top[h] == -INFINITY ? 1.f : ex2((m[h] - top[h]) * scale[h]);
                 m[h] = top[h];
                 l[h] *= f;
 #pragma unroll
@@ -412,11 +412,12 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float base = (m[h] == -INFINITY ? 0.f : m[h]) - (float)F::SHIFT;
+            // (the difference first: past 2^24 a rounded product of the maximum and the scale would be off by more than a power of two)
+            const float base = m[h] == -INFINITY ? 0.f : m[h];
 #pragma unroll
             for (int n = 0; n < TS / 8; ++n) {
-                s[n][2 * h] = ex2(fmaf(s[n][2 * h], scale[h], -base));
-                s[n][2 * h + 1] = ex2(fmaf(s[n][2 * h + 1], scale[h], -base));
+                s[n][2 * h] = ex2(fmaf(s[n][2 * h] - base, scale[h], (float)F::SHIFT));
+                s[n][2 * h + 1] = ex2(fmaf(s[n][2 * h + 1] - base, scale[h], (float)F::SHIFT));
                 l[h] += s[n][2 * h] + s[n][2 * h + 1];
             }
         }
@@ -495,7 +496,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         const int r = warp * RW + g + 8 * h;
-        if (c == 0) sh.ml[r] = make_float2(m[h], l[h] * DOWN);
+        if (c == 0) sh.ml[r] = make_float2(m[h] * scale[h], l[h] * DOWN);
 #pragma unroll
         for (int n = 0; n < CH; ++n) {
             if (any_odd)

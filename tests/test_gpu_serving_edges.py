@@ -48,3 +48,30 @@ def test_probabilities_of_terms_that_cancel(q_type, kv_type, pairs):
     want, _, mass, _, _ = ref.attention(batch, q, 1.0)
     part = 2.0 ** -16 if q_type == "bf16" else 2.0 ** -20
     assert (np.abs(f64(out) - want) <= HALF_STEP[q_type] * np.abs(want) + part * mass).all(), np.abs(f64(out) - want).max()
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_past_the_digits_of_fp32(q_type, kv_type, hd):
+    """Finite scores of some 2^32 (one product each, a scale of 2^7), where a unit of the last place is hundreds: the largest takes all, two equal ones half each.
+    The result is an entry of V or the mean of two, off by its rounding and that of P's parts (2^-16 and less)."""
+    import torch
+
+    from rustane_b200 import ops
+    lens = [300, 64, 33, 5000]
+    batch = Batch(lens, [1, 2, 1, 1], 2, hd, 16, kv_type, seed=3)
+    heads, rng = 8, np.random.default_rng(hd)
+    for b, n in enumerate(lens):
+        pages = batch.table[b, :-(-n // 16)].long()
+        k = torch.zeros(len(pages), 16, hd, device="cuda").flatten(0, 1)
+        k[:n, 0] = torch.from_numpy(rng.uniform(1000, 2000, n).round().astype(np.float32)).cuda()  # (bf16 keeps fewer of them apart)
+        at = int(k[:n - 3, 0].argmax())
+        k[(at + n // 2) % (n - 3), 0] = k[at, 0]
+        batch.pool[pages, 0] = k.view(len(pages), 1, 16, hd).to(batch.pool.dtype).expand(-1, 2, -1, -1)
+    q = batch.normal(batch.rows, heads, hd, dtype=q_type).zero_()
+    q[:, :, 0] = 2.0 ** 14 * (1.0 + torch.arange(heads, device="cuda") / 64.0)  # exact in every type
+    out, lse = ops.paged_attention(batch.cache(), q, batch.row_start, 2, scale=128.0, lse=True)
+    want, want_lse, mass, _, _ = ref.attention(batch, q, 128.0)
+    assert want_lse.min() > 2.0 ** 30
+    assert (np.abs(f64(out) - want) <= HALF_STEP[q_type] * np.abs(want) + (2.0 ** -16 + 2.0 ** -20) * mass).all(), np.abs(f64(out) - want).max()
+    np.testing.assert_allclose(f64(lse), want_lse, rtol=2.0 ** -21)
