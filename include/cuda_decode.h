@@ -411,8 +411,8 @@ int cd_rope_append(const cd_paged_cache* cache, const cd_rope* rope, int dtype, 
 /* Softmax attention of every new row over the entries up to its own (with window > 0: over the last `window` of them).
  * q, out [nrows][heads][hd] of `dtype` (F32, or the pool's type), q rows q_stride elements apart (0: packed), out packed; heads is
  * a multiple of kv_heads, q head h reads kv head h / (heads / kv_heads).  scale <= 0: 1/sqrt(hd).  lse [nrows][heads]: natural
- * log of the sum of exp(score), or NULL.  A row that sees nothing gets zeros and -inf.  What a row does not see cannot
- * reach it, NaN and infinities included.  collect != 0: the probabilities an entry got, summed over the rows and q heads of
+ * log of the sum of exp(score), or NULL.  A row that sees nothing, or scores of -inf only, gets zeros and -inf.  What a row does not
+ * see cannot reach it, NaN and infinities included; those that it sees do to it what the formula says, in fp32.  collect != 0: the probabilities an entry got, summed over the rows and q heads of
  * its kv head, are added to its weight.  Results do not depend on the run: nothing is summed by atomics. */
 int cd_paged_attention_workspace(const cd_paged_cache* cache, int heads, int nrows, int max_rows, int collect, size_t* bytes);
 int cd_paged_attention(const cd_paged_cache* cache, int dtype, int heads, int nrows, int max_rows, const void* q, int64_t q_stride,

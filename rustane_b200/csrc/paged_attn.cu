@@ -11,7 +11,7 @@ const char* CALL = "cd_paged_attention";
 
 struct Plan {
     int group, ru, row_warps, blocks;
-    size_t units, part_o, part_ml, unit_info, odd, lse2, scores, bytes;  // offsets in the workspace
+    size_t units, part_o, part_ml, unit_info, lse2, scores, bytes;  // offsets in the workspace
     long long score_stride;
 };
 // What a tile costs by its unit's rows: up to 16, 32, more (tensor-core form).  A CTA's four warps work on four places at once, on two, on
@@ -33,8 +33,7 @@ Plan plan_of(const cd_paged_cache* c, int heads, int nrows, int max_rows, int co
     p.part_o = 0;
     p.part_ml = up(slots * p.ru * c->hd * 4);
     p.unit_info = p.part_ml + up(slots * p.ru * 8);
-    p.odd = p.unit_info + up(p.units * 8);
-    p.lse2 = p.odd + (c->dtype == CD_DTYPE_F32 ? 0 : up((size_t)PA_MAX_CTAS * PA_WARPS * 16 * c->hd));
+    p.lse2 = p.unit_info + up(p.units * 8);
     p.score_stride = ((long long)c->max_pages * c->page_tokens + 3) & ~3ll;
     p.scores = p.lse2 + (collect ? up((size_t)nrows * heads * 4) : 0);
     p.bytes = p.scores + (collect ? up((size_t)nrows * heads * p.score_stride * 4) : 0);
@@ -59,7 +58,7 @@ template <typename KT, typename QT, int HD> cudaError_t launch(const AttnArgs& a
     cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
     if constexpr (std::is_same<KT, float>::value) {
-        attn_fma_kernel<KT, QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);
+        attn_fma_kernel<QT, HD><<<std::min(2 * sms, PA_MAX_CTAS), PA_THREADS, (size_t)(a.c.nseq + 1) * 4, s>>>(a);
     } else {
         using Size = MmaSize<QT, HD>;
         const bool few = Size::slots(a.row_warps) == 8;
@@ -122,7 +121,6 @@ extern "C" int cd_paged_attention(const cd_paged_cache* c, int dtype, int heads,
     a.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     a.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     a.unit_info = reinterpret_cast<int2*>(ws + plan.unit_info);
-    a.odd = reinterpret_cast<unsigned char*>(ws + plan.odd);
     a.lse2 = reinterpret_cast<float*>(ws + plan.lse2);
     a.scores = collect ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;
     a.q_stride = q_stride;

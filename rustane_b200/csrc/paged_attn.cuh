@@ -26,7 +26,6 @@ struct AttnArgs {
     int2* unit_info;  // [units] first CTA, CTAs
     float* lse2;      // [nrows][heads] log2; with scores only
     float* scores;    // [nrows][heads][score_stride] log2 domain, or nullptr
-    unsigned char* odd;  // [ctas][warps][16][hd]: what infinities and NaN that not all rows of a warp see do to those that do (written before it is read)
     long long q_stride, score_stride;
     int weights[3];  // what a tile of a unit of up to 16, 32 and more rows costs on the line; the first is the least
     float scale_log2;
@@ -183,124 +182,137 @@ template <typename F> __device__ inline void walk_line(const AttnArgs& p, const 
 }
 
 // ------------------------------------------------------------------------------------------------ fp32 FMAs
-// For fp32 pools, where rounding K and V to 16 bits would cost what the pool is kept for.  Eight lanes hold one entry's K (and V) row, a
-// warp four entries side by side; each eight lanes keep (m, l, o) of their entries for four rows.  Bound by the chain of an entry's
+// RW rows of a unit (rho0 .. of all its blocks' rows) by one warp: eight lanes hold one entry's K (and V) row, a warp four entries side by side; each eight lanes keep
+// (m, l, o) of their entries, here entries from + side, from + side + step .. of [first, end).
+template <typename KT, typename QT, int HD, int RW>
+__device__ __forceinline__ void fma_rows(const AttnArgs& p, const SeqWork& w, int b, int kvh, int rho0, int from, int end, int step, float (&m)[RW], float (&l)[RW], float (&o)[RW][HD / 8]) {
+    constexpr int VEC = 16 / sizeof(KT), NC = HD / 8 / VEC;  // elements of a load, loads of a lane and row
+    const int lane = threadIdx.x & 31, l8 = lane & 7, side = lane >> 3;
+    const KT* pool = static_cast<const KT*>(p.c.pool);
+    float q[RW][NC * VEC];
+    int last[RW];        // the last entry a row sees, -1: none
+    float* srow[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+        const int rho = rho0 + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
+        const bool valid = rho < w.s.n * p.group;
+        last[r] = valid ? w.s.len - w.s.n + j : -1;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        srow[r] = p.scores && valid ? p.scores + ((size_t)(w.s.r0 + j) * p.heads + head) * p.score_stride : nullptr;
+        const QT* src = static_cast<const QT*>(p.q) + (size_t)(valid ? w.s.r0 + j : 0) * p.q_stride + (size_t)(valid ? head : 0) * HD;
+#pragma unroll
+        for (int i = 0; i < NC * VEC; ++i) {
+            q[r][i] = valid ? as_float(src[(i / VEC * 8 + l8) * VEC + i % VEC]) * p.scale_log2 : 0.f;
+            o[r][i] = 0.f;
+        }
+    }
+    // the next entries' rows are on their way while these are worked on; their page is looked up a step before that
+    uint4 kn[NC], vn[NC];
+    int page_n = -1, word = 0;
+    auto look_up = [&](int t) { word = t < end ? page_word(p.c, b, t) : 0; };
+    auto fetch = [&](int t) {
+        page_n = t < end ? checked_page(p.c, word) : -1;
+        if (page_n >= 0) {
+            const KT *kr = pool + row_at(p.c, page_n, 0, kvh, t, HD), *vr = pool + row_at(p.c, page_n, 1, kvh, t, HD);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                kn[i] = __ldg(reinterpret_cast<const uint4*>(kr) + i * 8 + l8);
+                vn[i] = __ldg(reinterpret_cast<const uint4*>(vr) + i * 8 + l8);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) kn[i] = vn[i] = make_uint4(0, 0, 0, 0);
+        }
+    };
+    int t0 = from + side;
+    look_up(t0);
+    fetch(t0);
+    look_up(t0 + step);
+    for (; __any_sync(0xffffffffu, t0 < end); t0 += step) {
+        float k[NC * VEC], v[NC * VEC];
+        const int page = page_n;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                k[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&kn[i])[e]);
+                v[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&vn[i])[e]);
+            }
+        fetch(t0 + step);
+        look_up(t0 + 2 * step);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < NC * VEC; ++i) s = fmaf(q[r][i], k[i], s);
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            const bool seen = page >= 0 && pa_sees(t0, last[r], p.window);
+            if (!seen) s = -INFINITY;
+            if (srow[r] && l8 == r && t0 < end) srow[r][t0] = s;
+            if (!seen) continue;  // what is masked does not reach the sums, whatever its V holds
+            if (s > m[r] || s != s) {
+                const float f = exp2f(m[r] - s);
+                m[r] = s;
+                l[r] *= f;
+#pragma unroll
+                for (int i = 0; i < NC * VEC; ++i) o[r][i] *= f;
+            }
+            const float e = exp2f(s - (m[r] == -INFINITY ? 0.f : m[r]));
+            l[r] += e;
+#pragma unroll
+            for (int i = 0; i < NC * VEC; ++i) o[r][i] = fmaf(e, v[i], o[r][i]);
+        }
+    }
+}
+// Those rows' sums over the warp's four sides: (m, l) to ml[r], o to so[r * stride ..].
+template <typename KT, int HD, int RW> __device__ __forceinline__ void fma_store(const float (&m)[RW], const float (&l)[RW], const float (&o)[RW][HD / 8], float2* ml, float* so, int stride) {
+    constexpr int VEC = 16 / sizeof(KT);
+    const int lane = threadIdx.x & 31, l8 = lane & 7;
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int x = 8; x < 32; x <<= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, top, x);
+            top = other > top || other != other ? other : top;
+        }
+        const float f = exp2f(m[r] - (top == -INFINITY ? 0.f : top));
+        float sum = l[r] * f;
+#pragma unroll
+        for (int x = 8; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (lane == 0) ml[r] = make_float2(top, sum);
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+            float x = o[r][i] * f;
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            if (lane < 8) so[r * stride + (i / VEC * 8 + l8) * VEC + i % VEC] = x;
+        }
+    }
+}
+
+// For fp32 pools, where rounding K and V to 16 bits would cost what the pool is kept for.  Bound by the chain of an entry's
 // instructions (hd / 8 FMAs, three shuffles and an exponential a row): 53 sequences of up to 953 entries, four heads, two rows,
 // 140 MB, 82 us; 105 us with the rows asked for when they are needed.
-template <typename KT, typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS, 2) attn_fma_kernel(const __grid_constant__ AttnArgs p) {
-    constexpr int VEC = 16 / sizeof(KT), NC = HD / 8 / VEC, RW = 4, PAD = 4;  // elements of a load, loads of a lane and row
+template <typename QT, int HD> __global__ void __launch_bounds__(PA_THREADS, 2) attn_fma_kernel(const __grid_constant__ AttnArgs p) {
+    constexpr int RW = 4, PAD = 4;
     extern __shared__ int pre[];
     __shared__ int sums[2 * PA_WARPS];
     __shared__ __align__(16) float so[PA_WARPS * RW * (HD + PAD)];
     __shared__ float2 sml[PA_WARPS * RW];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l8 = lane & 7, side = lane >> 3;
-    const int rw = warp % p.row_warps, tg = warp / p.row_warps, groups = PA_WARPS / p.row_warps;
-    const KT* pool = static_cast<const KT*>(p.c.pool);
+    const int warp = threadIdx.x >> 5, rw = warp % p.row_warps, tg = warp / p.row_warps, groups = PA_WARPS / p.row_warps;
 
     pdl_launch_dependents();
     int most;
     const int total = line_up(p, pre, sums, most);
     walk_line(p, pre, total, most, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
-        float q[RW][NC * VEC], o[RW][NC * VEC], m[RW], l[RW];
-        int last[RW];        // the last entry a row sees, -1: none
-        float* srow[RW];
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            const int rho = block * p.ru + rw * RW + r, j = rho / p.group, head = kvh * p.group + rho % p.group;
-            const bool valid = rho < w.s.n * p.group;
-            last[r] = valid ? w.s.len - w.s.n + j : -1;
-            m[r] = -INFINITY;
-            l[r] = 0.f;
-            srow[r] = p.scores && valid ? p.scores + ((size_t)(w.s.r0 + j) * p.heads + head) * p.score_stride : nullptr;
-            const QT* src = static_cast<const QT*>(p.q) + (size_t)(valid ? w.s.r0 + j : 0) * p.q_stride + (size_t)(valid ? head : 0) * HD;
-#pragma unroll
-            for (int i = 0; i < NC * VEC; ++i) {
-                q[r][i] = valid ? as_float(src[(i / VEC * 8 + l8) * VEC + i % VEC]) * p.scale_log2 : 0.f;
-                o[r][i] = 0.f;
-            }
-        }
         const int first = w.start + tile * PA_TILE, end = min(w.s.len, first + tiles * PA_TILE);
-        // the next entries' rows are on their way while these are worked on; their page is looked up a step before that
-        uint4 kn[NC], vn[NC];
-        int page_n = -1, word = 0;
-        auto look_up = [&](int t) { word = t < end ? page_word(p.c, b, t) : 0; };
-        auto fetch = [&](int t) {
-            page_n = t < end ? checked_page(p.c, word) : -1;
-            if (page_n >= 0) {
-                const KT *kr = pool + row_at(p.c, page_n, 0, kvh, t, HD), *vr = pool + row_at(p.c, page_n, 1, kvh, t, HD);
-#pragma unroll
-                for (int i = 0; i < NC; ++i) {
-                    kn[i] = __ldg(reinterpret_cast<const uint4*>(kr) + i * 8 + l8);
-                    vn[i] = __ldg(reinterpret_cast<const uint4*>(vr) + i * 8 + l8);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < NC; ++i) kn[i] = vn[i] = make_uint4(0, 0, 0, 0);
-            }
-        };
-        const int step = groups * 4;
-        int t0 = first + tg * 4 + side;
-        look_up(t0);
-        fetch(t0);
-        look_up(t0 + step);
-        for (; __any_sync(0xffffffffu, t0 < end); t0 += step) {
-            float k[NC * VEC], v[NC * VEC];
-            const int page = page_n;
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    k[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&kn[i])[e]);
-                    v[i * VEC + e] = as_float(reinterpret_cast<const KT*>(&vn[i])[e]);
-                }
-            fetch(t0 + step);
-            look_up(t0 + 2 * step);
-#pragma unroll
-            for (int r = 0; r < RW; ++r) {
-                float s = 0.f;
-#pragma unroll
-                for (int i = 0; i < NC * VEC; ++i) s = fmaf(q[r][i], k[i], s);
-#pragma unroll
-                for (int x = 1; x < 8; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-                const bool seen = page >= 0 && pa_sees(t0, last[r], p.window);
-                if (!seen) s = -INFINITY;
-                if (srow[r] && l8 == r && t0 < end) srow[r][t0] = s;
-                if (!seen) continue;  // what is masked does not reach the sums, whatever its V holds
-                if (s > m[r] || s != s) {
-                    const float f = exp2f(m[r] - s);
-                    m[r] = s;
-                    l[r] *= f;
-#pragma unroll
-                    for (int i = 0; i < NC * VEC; ++i) o[r][i] *= f;
-                }
-                const float e = exp2f(s - (m[r] == -INFINITY ? 0.f : m[r]));
-                l[r] += e;
-#pragma unroll
-                for (int i = 0; i < NC * VEC; ++i) o[r][i] = fmaf(e, v[i], o[r][i]);
-            }
-        }
+        float o[RW][HD / 8], m[RW], l[RW];
+        fma_rows<float, QT, HD, RW>(p, w, b, kvh, block * p.ru + rw * RW, first + tg * 4, end, groups * 4, m, l, o);
         __syncthreads();  // the unit before has been read
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            float top = m[r];
-#pragma unroll
-            for (int x = 8; x < 32; x <<= 1) {
-                const float other = __shfl_xor_sync(0xffffffffu, top, x);
-                top = other > top || other != other ? other : top;
-            }
-            const float f = exp2f(m[r] - (top == -INFINITY ? 0.f : top));
-            float sum = l[r] * f;
-#pragma unroll
-            for (int x = 8; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            if (lane == 0) sml[warp * RW + r] = make_float2(top, sum);
-#pragma unroll
-            for (int i = 0; i < NC * VEC; ++i) {
-                float x = o[r][i] * f;
-                x += __shfl_xor_sync(0xffffffffu, x, 8);
-                x += __shfl_xor_sync(0xffffffffu, x, 16);
-                if (side == 0) so[(warp * RW + r) * (HD + PAD) + (i / VEC * 8 + l8) * VEC + i % VEC] = x;
-            }
-        }
+        fma_store<float, HD, RW>(m, l, o, sml + warp * RW, so + warp * RW * (HD + PAD), HD + PAD);
         __syncthreads();
         finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sml}, RW, p.row_warps, w, kvh, block, whole, slot);
     });

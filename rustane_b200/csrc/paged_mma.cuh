@@ -104,45 +104,47 @@ template <typename KT, typename QT, int HD> inline size_t mma_shared(int nseq, i
     const size_t o = (size_t)PA_WARPS * 16 * (HD + 4) * 4;  // (in the ring's place once it is empty)
     return (ring > o ? ring : o) + q + (size_t)(nseq + 1) * 4 + 1024;  // (1024: the ring's own alignment)
 }
-// What entries with infinities and NaN in V do to rows that see them, where other rows of the unit do not: bits 1 (+inf), 2 (-inf) and 4 (NaN) of
-// the row's and column's sum, set aside (odd_sums, rare and therefore not inline) while the products take zeros for them.
-template <int TS> struct Probs {
-    float p[TS / 8][4];  // as the products have them: e^(score - maximum) of entries 8 n + 2 c + column, rows g and g + 8
-};
-template <typename KT, int HD, int TS>
-__device__ __noinline__ void odd_sums(const uint32_t* v, unsigned char* odd, Probs<TS> s, int t0, int end, int last0, int last1, int window, int lane) {
-    const int g = lane >> 2, c = lane & 3;
+// Infinities and NaN.  A product in parts is not what the formula says of an infinity: q k with k infinite is NaN where a lower part of q is zero
+// or of the other sign, p v likewise, and 0 * inf reaches rows that do not see the entry.  So (1) in tiles that some rows see only
+// in part, what is not finite in V is taken out ahead of the products, and rows that see it are marked; (2) rows whose sums come out NaN
+// are marked; (3) marked rows are worked out again, in fp32 FMAs, over all of the CTA's entries of the unit.  Rare, and therefore out of line.
+//
+// (1): which of this lane's rows (bit h: g + 8 h) see such an entry of the stage
+template <typename KT, int HD, int TS> __device__ __noinline__ uint32_t odd_rows(const uint32_t* v, int t0, int end, int last0, int last1, int window) {
+    const int lane = threadIdx.x & 31;
+    uint32_t rows = 0;
     for (int at = 0; at < TS; ++at) {
-        const int t = t0 + at, from = (lane & ~3) | (at & 7) >> 1;
-        float e0 = 0.f, e1 = 0.f;
-#pragma unroll
-        for (int n = 0; n < TS / 8; ++n)
-            if (at >> 3 == n) {
-                e0 = at & 1 ? s.p[n][1] : s.p[n][0];
-                e1 = at & 1 ? s.p[n][3] : s.p[n][2];
-            }
-        e0 = __shfl_sync(0xffffffffu, e0, from);
-        e1 = __shfl_sync(0xffffffffu, e1, from);
-        if (t >= end) continue;
-        const bool see0 = pa_sees(t, last0, window), see1 = pa_sees(t, last1, window);
-        for (int n = 0; n < HD / 8; ++n) {
-            const uint32_t word = v[at * HD / 2 + ((n ^ (at & 7)) << 2) + c];
-            if (!not_finite<KT>(word)) continue;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float x = as_float(reinterpret_cast<const KT*>(&word)[h]);
-                if (isfinite(x)) continue;
-                auto code = [&](float e) { const float y = e * x; return y != y ? 4 : y > 0.f ? 1 : 2; };
-                if (see0) odd[g * HD + n * 8 + 2 * c + h] |= code(e0);
-                if (see1) odd[(g + 8) * HD + n * 8 + 2 * c + h] |= code(e1);
-            }
+        const int t = t0 + at;
+        bool odd = false;
+        for (int i = lane; i < HD / 2; i += 32) odd |= not_finite<KT>(v[at * HD / 2 + i]);
+        if (__any_sync(0xffffffffu, odd) && t < end) rows |= (uint32_t)pa_sees(t, last0, window) | (uint32_t)pa_sees(t, last1, window) << 1;
+    }
+    return rows;
+}
+// (3): row r is in lane 4 (r % 8)'s bit of its row warp's marks, .x below 8 and .y from 8 on, of any of the groups.  All threads; ends with a barrier.
+template <typename KT, typename QT, int HD, int PAD>
+__device__ __noinline__ void rows_again(const AttnArgs& p, const SeqWork& w, int b, int kvh, int block, int first, int end, const uint2* marks, int row_warps, float2* ml, float* so) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = min(p.ru, w.s.n * p.group - block * p.ru);
+    for (int r = warp; r < rows; r += PA_WARPS) {
+        const int rw = r / 16, rr = r % 16;
+        uint32_t marked = 0;
+        for (int at = rw; at < PA_WARPS; at += row_warps) marked |= (rr < 8 ? marks[at].x : marks[at].y) >> 4 * (rr % 8) & 1u;
+        if (!marked) continue;
+        float o[1][HD / 8], m[1], l[1];
+        fma_rows<KT, QT, HD, 1>(p, w, b, kvh, block * p.ru + r, first, end, 4, m, l, o);
+        fma_store<KT, HD, 1>(m, l, o, ml + rw * 16 + rr, so + (rw * 16 + rr) * (HD + PAD), HD + PAD);
+        for (int at = rw + row_warps; at < PA_WARPS; at += row_warps) {  // the first group has all of it now
+            if (lane == 0) ml[at * 16 + rr] = make_float2(-INFINITY, 0.f);
+            for (int d = lane; d < HD; d += 32) so[(at * 16 + rr) * (HD + PAD) + d] = 0.f;
         }
     }
+    __syncthreads();
 }
 
 template <int HD> struct MmaShared {
     float2 ml[PA_WARPS * 16];
     float qscale[4 * 16];
+    uint2 marks[PA_WARPS];
 };
 
 // A run of one unit's tiles, its rows on ROW_WARPS warps.
@@ -271,8 +273,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
     const bool mixed = w.s.n > 1 || p.window > 0;
     auto sees = [&](int t, int h) { return pa_sees(t, last[h], p.window); };
 
-    bool any_odd = false;
-    unsigned char* odd_at = p.odd + ((size_t)blockIdx.x * PA_WARPS + warp) * RW * HD;  // this warp's rows and columns
+    uint32_t again = 0;  // marks of this lane's rows
     // Steps below 0 only issue copies: V of step it + STAGES - 1, K of step it + STAGES.  (One loop, so that the copies stand in the code
     // once: at its start a kernel waits for its instructions more than for anything else.)
     int get = 0, t0 = first + (tg - STAGES * groups) * TS;
@@ -430,16 +431,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
             bool odd = false;
             for (int at = lane; at < TS * HD / 2; at += 32) odd |= not_finite<KT>(v[at]);
             if (__any_sync(0xffffffffu, odd)) {
-                Probs<TS> probs;
-#pragma unroll
-                for (int n = 0; n < TS / 8; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) probs.p[n][e] = s[n][e];
-                if (!any_odd)
-                    for (int i = lane; i < RW * HD / 16; i += 32) reinterpret_cast<uint4*>(odd_at)[i] = make_uint4(0, 0, 0, 0);
-                __syncwarp();
-                odd_sums<KT, HD, TS>(v, odd_at, probs, t0, end, last[0], last[1], p.window, lane);
-                any_odd = true;
+                again |= odd_rows<KT, HD, TS>(v, t0, end, last[0], last[1], p.window);
                 group_sync();  // the group's warps have all read the stage: take what is not finite out of it
                 uint32_t* clean = const_cast<uint32_t*>(v);
                 for (int at = gt; at < TS * HD / 2; at += gsize) clean[at] = finite_part<KT>(clean[at]);
@@ -496,19 +488,27 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         const int r = warp * RW + g + 8 * h;
+        bool nan = l[h] != l[h];
         if (c == 0) sh.ml[r] = make_float2(m[h] * scale[h], l[h] * DOWN);
 #pragma unroll
         for (int n = 0; n < CH; ++n) {
-            if (any_odd)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int code = odd_at[(g + 8 * h) * HD + n * 8 + 2 * c + e];
-                    if (code) o[n][2 * h + e] = code == 1 ? INFINITY : code == 2 ? -INFINITY : NAN;
-                }
+            nan |= o[n][2 * h] != o[n][2 * h] || o[n][2 * h + 1] != o[n][2 * h + 1];
             *reinterpret_cast<float2*>(so + (size_t)r * (HD + PAD) + n * 8 + 2 * c) = make_float2(o[n][2 * h] * DOWN, o[n][2 * h + 1] * DOWN);
         }
+        again |= (uint32_t)nan << h;
+    }
+    again |= __shfl_xor_sync(0xffffffffu, again, 1);
+    again |= __shfl_xor_sync(0xffffffffu, again, 2);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // (rows past the unit's, and those that see nothing, have no result to mend)
+        const uint32_t x = __ballot_sync(0xffffffffu, again >> h & 1u && last[h] >= 0);
+        if (lane == 0) (h ? sh.marks[warp].y : sh.marks[warp].x) = x;
     }
     __syncthreads();
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < PA_WARPS; ++i) any |= sh.marks[i].x | sh.marks[i].y;
+    if (any) rows_again<KT, QT, HD, PAD>(p, w, b, kvh, block, first, end, sh.marks, ROW_WARPS, sh.ml, so);
     finish_unit<QT, HD, PAD>(p, UnitParts<HD, PAD>{so, sh.ml}, RW, ROW_WARPS, w, kvh, block, whole, slot);
 }
 

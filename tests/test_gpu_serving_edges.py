@@ -75,3 +75,102 @@ def test_scores_past_the_digits_of_fp32(q_type, kv_type, hd):
     assert want_lse.min() > 2.0 ** 30
     assert (np.abs(f64(out) - want) <= HALF_STEP[q_type] * np.abs(want) + (2.0 ** -16 + 2.0 ** -20) * mass).all(), np.abs(f64(out) - want).max()
     np.testing.assert_allclose(f64(lse), want_lse, rtol=2.0 ** -21)
+
+
+def at_entry(batch, b, t):
+    return int(batch.table[b, t // batch.page]), t % batch.page
+
+
+def attend(batch, q, **more):
+    from rustane_b200 import ops
+    cache = batch.cache()
+    out, lse = ops.paged_attention(cache, q, batch.row_start, max(batch.counts), lse=True, **more)
+    assert int(cache.status) == 0
+    return f64(out), f64(lse)
+
+
+def near(out, want, mass, q_type, kv_type, hd, worst):
+    """The result's rounding, and what scores (hd fp32 terms of at most `worst` together, 2^-21 for q's parts) and P's parts are off by."""
+    part = 2.0 ** -16 if q_type == kv_type == "bf16" else 2.0 ** -20
+    return np.abs(out - want) <= HALF_STEP[q_type] * np.abs(want) + (part + 2 * (hd * 2.0 ** -24 + 2.0 ** -21) * worst + 2.0 ** -20) * mass
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("heads", [2, 8, 24])
+def test_infinities_and_nan_of_v_reach_the_rows_that_see_them(q_type, kv_type, hd, window, heads):
+    """In single columns of V, with K finite: such a column of a row that sees the entry is +inf, -inf or NaN (both signs, NaN) exactly, in tiles that all rows see and
+    in ones that only some do; its other columns are as ever, and rows that do not see the entry keep every bit."""
+    lens, counts, inf, nan = [75, 200, 1000, 9000, 1], [3, 1, 2, 4, 1], float("inf"), float("nan")
+    batch = Batch(lens, counts, 2, hd, 32, kv_type, seed=2)
+    q = batch.normal(batch.rows, heads, hd, dtype=q_type)
+    clean, clean_lse = attend(batch, q, window=window)
+    want, _, mass, _, worst = ref.attention(batch, q, window=window)
+    spoil = [(0, 74, 3, inf), (0, 10, 4, inf), (0, 33, 5, -inf), (0, 73, 5, inf), (0, 74, 6, nan), (1, 50, 1, -inf), (1, 170, 2, inf), (1, 199, 8, -inf), (1, 198, 8, -inf),
+             (2, 500, 7, inf), (2, 999, 9, -inf), (2, 961, 10, inf), (2, 960, 11, -inf), (2, 990, 11, inf), (3, 4000, 12, inf), (3, 8999, 13, inf), (3, 8965, 14, -inf), (4, 0, 0, inf)]
+    touched = np.zeros(batch.rows, dtype=bool)
+    for b, t, col, value in spoil:
+        page, off = at_entry(batch, b, t)
+        batch.pool[page, 1, :, off, col] = value
+        for j in range(counts[b]):
+            row, last = batch.starts[b] + j, lens[b] - counts[b] + j
+            if t <= last and (window == 0 or last - t < window):
+                touched[row] = True
+                was = want[row, :, col]
+                want[row, :, col] = np.where(np.isfinite(was) | (was == value), value, nan)
+    out, lse = attend(batch, q, window=window)
+    np.testing.assert_array_equal(out[~touched], clean[~touched])
+    odd = ~np.isfinite(want)
+    np.testing.assert_array_equal(out[odd], want[odd])
+    assert near(out[~odd], want[~odd], mass[~odd], q_type, kv_type, hd, worst).all()
+    np.testing.assert_allclose(lse, clean_lse, rtol=2.0 ** -20, atol=2 * (hd + 8) * 2.0 ** -24 * max(worst, 1) + 2.0 ** -19)
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,counts", [(2, [1, 1, 1]), (8, [1, 1, 1]), (8, [3, 4, 2])])
+def test_infinities_of_k(q_type, kv_type, hd, heads, counts):
+    """An infinity of K that makes every score of its entry -inf leaves the rows, their log-sum-exp and the weights they hand on as if the entry had no
+    part in them; one that makes a score +inf makes the rows that see it NaN, as inf - inf is."""
+    lens = [75, 400, 9000]
+    batch = Batch(lens, counts, 2, hd, 32, kv_type, seed=4, book=True)
+    q = batch.normal(batch.rows, heads, hd, dtype=q_type)
+    q[:, :, 11] = q[:, :, 11].abs() + 0.01  # (parts of either sign)
+    _, _, _, _, worst = ref.attention(batch, q)
+    for b, t in ((0, 5), (0, 74), (1, 200), (1, 396), (2, 0), (2, 5000)):
+        page, off = at_entry(batch, b, t)
+        batch.pool[page, 0, :, off, 11] = -float("inf")
+    before = f64(batch.weight)
+    out, lse = attend(batch, q, collect=True)
+    want, want_lse, mass, got, _ = ref.attention(batch, q)
+    assert np.isfinite(want).all() and np.isfinite(out).all() and near(out, want, mass, q_type, kv_type, hd, worst).all()
+    np.testing.assert_allclose(lse, want_lse, atol=(hd + 8) * 2.0 ** -24 * max(worst, 1) + 2.0 ** -20, rtol=2.0 ** -21)
+    moved = 2 * ((hd + 8) * 2.0 ** -24 + 2.0 ** -21) * max(worst, 1) + max(counts) * heads * 2.0 ** -24 + 2.0 ** -20
+    for b, n in enumerate(lens):
+        np.testing.assert_allclose(f64(batch.weight[b])[:, :n], before[b][:, :n] + got[b], rtol=moved, atol=1e-7)
+    page, off = at_entry(batch, 1, 399)  # the newest entry: the last row alone sees it
+    batch.pool[page, 0, :, off, 11] = float("inf")
+    again, again_lse = attend(batch, q)
+    last = batch.starts[2] - 1
+    assert np.isnan(again[last]).all() and np.isnan(again_lse[last]).all()
+    others = np.arange(batch.rows) != last
+    np.testing.assert_array_equal(again[others], out[others])
+    np.testing.assert_array_equal(again_lse[others], lse[others])
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("page", [7, 16])
+def test_rows_of_nothing_but_infinite_scores(q_type, kv_type, page):
+    """Every score of a row -inf: no entry has weight, the row is zeros and -inf, its neighbours are not touched."""
+    batch = Batch([40, 40], [2, 2], 1, 64, page, kv_type, seed=5)
+    q = batch.normal(4, 3, 64, dtype=q_type)
+    clean, clean_lse = attend(batch, q)
+    for t in range(40):
+        p, off = at_entry(batch, 0, t)
+        batch.pool[p, 0, :, off, 0] = -float("inf")
+    q[:2, :, 0] = q[:2, :, 0].abs() + 0.01
+    out, lse = attend(batch, q)
+    assert (out[:2] == 0).all() and np.isneginf(lse[:2]).all()
+    np.testing.assert_array_equal(out[2:], clean[2:])
+    np.testing.assert_array_equal(lse[2:], clean_lse[2:])
