@@ -73,17 +73,6 @@ __device__ inline void ldsm_t(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
-// (not volatile, unlike Mma16's: the compiler may mix products and other work)
-template <typename KT> __device__ inline void product(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <> __device__ inline void product<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <> __device__ inline void product<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 template <typename KT, typename QT> struct MmaForm {
     static constexpr bool F16 = std::is_same<KT, __half>::value, WIDE = std::is_same<QT, float>::value;
     static constexpr int NQ = WIDE ? (F16 ? 2 : 3) : 1, NP = WIDE && !F16 ? 3 : 2;
@@ -360,8 +349,8 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
                 for (int part = NQ - 1; part >= 0; --part)
 #pragma unroll
                     for (int h = 0; h < HALVES; ++h) {
-                        product<KT>(kb & 1 ? s2[2 * h] : s[2 * h], a[i][part], k[i][h][0], k[i][h][1]);
-                        product<KT>(kb & 1 ? s2[2 * h + 1] : s[2 * h + 1], a[i][part], k[i][h][2], k[i][h][3]);
+                        X::mma(kb & 1 ? s2[2 * h] : s[2 * h], a[i][part], k[i][h][0], k[i][h][1]);
+                        X::mma(kb & 1 ? s2[2 * h + 1] : s[2 * h + 1], a[i][part], k[i][h][2], k[i][h][3]);
                     }
         }
 #pragma unroll
@@ -465,7 +454,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
 #pragma unroll
                         for (int part = NP - 1; part >= 0; --part)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) product<KT>(f[i], pp[part], v[n + i / 2][i % 2 * 2], v[n + i / 2][i % 2 * 2 + 1]);
+                            for (int i = 0; i < 4; ++i) X::mma(f[i], pp[part], v[n + i / 2][i % 2 * 2], v[n + i / 2][i % 2 * 2 + 1]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -475,7 +464,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
 #pragma unroll
                     for (int part = NP - 1; part >= 0; --part)
 #pragma unroll
-                        for (int n = 0; n < 8; ++n) product<KT>(o[2 * nb + n], pp[part], v[n / 2][n % 2 * 2], v[n / 2][n % 2 * 2 + 1]);
+                        for (int n = 0; n < 8; ++n) X::mma(o[2 * nb + n], pp[part], v[n / 2][n % 2 * 2], v[n / 2][n % 2 * 2 + 1]);
                 }
             }
         }
