@@ -323,10 +323,12 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     }
     const T *pt = target + row * p.target_stride, *pd = left && draft ? draft + row * p.draft_stride : nullptr;
     const int gone = left && !draft ? p.tokens[row + 1] : -1;
-    // e^((logit - largest) / temperature) as one multiplication and addition ahead of exp_neg (rounding may leave it above 0 by 1e-13)
-    double pb = -(double)sh.pm * p.inv_t, qb = -(double)sh.qm * p.inv_t;
-    auto ep = [&](float x) { return exp_neg(fma((double)x, p.inv_t, pb), two_to); };
-    auto eq = [&](float x) { return exp_neg(fma((double)x, p.inv_t, qb), two_to); };
+    // e^((logit - largest) / temperature), the difference first: it is 0 for the largest whatever its size, where a rounded product of the
+    // largest and 1 / temperature would leave what exceeds 64 bits of it
+    const double pm = sh.pm, qm = sh.qm;
+    double pb = 0.0, qb = 0.0;
+    auto ep = [&](float x) { return exp_neg(fma((double)x - pm, p.inv_t, pb), two_to); };
+    auto eq = [&](float x) { return exp_neg(fma((double)x - qm, p.inv_t, qb), two_to); };
     constexpr int PER = VD_TILE / 32;  // tokens of a tile a lane has
     auto logits = [&](const T* row_, int first, int step, float (&x)[PER]) {  // all of them asked for before one is used
 #pragma unroll
@@ -363,8 +365,8 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
             sp += o[0];
             sq += o[1];
         }
-        pb -= log(sp);  // from here on the terms are p and q themselves
-        qb -= log(sq);
+        pb = -log(sp);  // from here on the terms are p and q themselves
+        qb = -log(sq);
     }
     auto shares = [&](int first, int step, bool rest, double (&v)[PER]) {  // of a lane's tokens in what is drawn from
         float a[PER], d[PER];
@@ -382,7 +384,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     };
     double whole = 0.0, before = 0.0, totals[VD_CLUSTER];
     bool rest = left;
-    for (int turn = 0; turn < 2; ++turn) {  // again from p alone where rounding leaves nothing of p - q
+    for (int turn = 0; turn < 2; ++turn) {  // again from p alone where nothing is left of p - q; p's largest has a share, so that `whole` is then above 0
         for (int t = t0 + warp; t < t1; t += VD_PICK_WARPS) {
             double x[PER], v = 0.0;
             shares(t * VD_TILE + lane, 32, rest, x);

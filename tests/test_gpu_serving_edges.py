@@ -174,3 +174,53 @@ def test_rows_of_nothing_but_infinite_scores(q_type, kv_type, page):
     assert (out[:2] == 0).all() and np.isneginf(lse[:2]).all()
     np.testing.assert_array_equal(out[2:], clean[2:])
     np.testing.assert_array_equal(lse[2:], clean_lse[2:])
+
+
+# ------------------------------------------------------------------------------------------------ verification
+def verify_inputs(counts, vocab, dtype, seed, near=0.7):
+    import torch
+    g = torch.Generator("cpu").manual_seed(seed)
+    rows = sum(counts)
+    target = torch.randn(rows, vocab, generator=g) * 2
+    draft = target + near * torch.randn(rows, vocab, generator=g)
+    tokens = torch.zeros(rows, dtype=torch.int32)
+    tokens[1:] = draft[:-1].argmax(1).int()
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32)
+    kind = ref.torch_dtype(dtype)
+    return dict(target=target.to(kind), draft=draft.to(kind), tokens=tokens, starts=starts, u=torch.rand(rows, generator=g), d=torch.rand(len(counts), generator=g), most=max(counts + [1]))
+
+
+def verify(x, temperature, with_draft=True, **more):
+    """(accepted, out, status) as lists and a number."""
+    import torch
+
+    from rustane_b200 import ops
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    accepted, out = ops.verify_drafts(x["target"].cuda(), x["tokens"].cuda(), x["starts"].cuda(), x["most"], x["u"].cuda(), x["d"].cuda(),
+                                      draft=x["draft"].cuda() if with_draft else None, temperature=temperature, status=status, **more)
+    return accepted.tolist(), out.tolist(), int(status)
+
+
+def verify64(x, temperature, with_draft=True):
+    accepted, out = ref.verify(f64(x["target"]), f64(x["draft"]) if with_draft else None, x["tokens"].numpy(), f64(x["u"]), f64(x["d"]), x["starts"].numpy(), temperature)
+    return accepted.tolist(), out.tolist()
+
+
+@pytest.mark.parametrize("dtype,level", [("f32", -3.4028234663852886e38), ("f32", -1e30), ("f32", 1e30), ("f32", -65536.0), ("bf16", -3.3895313892515355e38), ("bf16", 1e25), ("f16", -65504.0)])
+@pytest.mark.parametrize("temperature", [0.7, 0.9, 1.0, 1e-6, 1e6])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_rows_of_one_large_logit(dtype, level, temperature, with_draft):
+    """Rows masked altogether with their type's lowest value, or shifted far off: every token as likely as the next, whatever the
+    size of what they share.  Draws are 1/2 of a token's share off every border, 2^-15 of the whole, where 64-bit sums are off by 2^-45."""
+    import torch
+    vocab, counts = 8192, [3, 1, 4, 1]
+    x = verify_inputs(counts, vocab, dtype, 5)
+    x["target"][:] = level
+    x["target"][7] = verify_inputs(counts, vocab, dtype, 5)["target"][7]
+    x["draft"][:] = level / 2
+    g = torch.Generator("cpu").manual_seed(1)
+    x["d"] = ((torch.randint(0, vocab, (4,), generator=g) + 0.5) / vocab).float()
+    x["u"][:] = torch.tensor([0.5, 0.5, 0, 0, 0.5, 0.999, 0.5, 0, 0])
+    got, out, status = verify(x, temperature, with_draft)
+    want = verify64(x, temperature, with_draft)
+    assert (got, out) == want and status == 0
