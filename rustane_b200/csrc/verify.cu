@@ -94,11 +94,12 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
         for (int d = 0; d < DEEP; ++d)
             if (i + d * VD_THREADS < vecs) w[d] = load_once(body + i + d * VD_THREADS);
     };
-    fetch(tid);
-    // rows of no sequence, and draft rows with no draft behind them, are not looked at
+    // target rows are all there and asked for at once; a draft row only if a draft is behind it, as there need not be memory for others
+    if (!is_draft) fetch(tid);
     bool used = false;
-    for (int b = tid; b < p.nseq; b += VD_THREADS) used |= p.row_start[b] <= r && r < p.row_start[b + 1] - (is_draft ? 1 : 0);
+    for (int b = tid; b < p.nseq; b += VD_THREADS) used |= p.row_start[b] <= r && r + is_draft < p.row_start[b + 1];
     if (!__syncthreads_or(used)) return;
+    if (is_draft) fetch(tid);
     const float scale = (float)(p.inv_t * 1.4426950408889634074);
     float m = -INFINITY, s = 0.f;
     int at = 0x7fffffff;

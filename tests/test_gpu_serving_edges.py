@@ -224,3 +224,17 @@ def test_rows_of_one_large_logit(dtype, level, temperature, with_draft):
     got, out, status = verify(x, temperature, with_draft)
     want = verify64(x, temperature, with_draft)
     assert (got, out) == want and status == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_draft_rows_with_no_draft_behind_them_are_not_read(dtype):
+    """A sequence's last row of draft logits holds NaN, infinities or the largest values: nothing changes.  (That the last one of a batch may not even be
+    memory cannot be tested here; the kernel asks for a draft row only once it knows that a draft is behind it.)"""
+    counts = [4, 1, 3, 1, 6]
+    x = verify_inputs(counts, 5003, dtype, 3)
+    want = verify(x, 0.9)
+    assert want[:2] == verify64(x, 0.9)
+    for value in (float("nan"), float("inf"), -float("inf"), 6e4):
+        for end in x["starts"][1:].tolist():
+            x["draft"][end - 1] = value
+        assert verify(x, 0.9) == want
