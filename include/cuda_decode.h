@@ -437,7 +437,7 @@ int cd_cache_evict(const cd_paged_cache* cache, int keep, int sinks, int recent,
  * max(p - q, 0), or from the last row's p where all stay: the first one whose running sum exceeds draws[b] times the whole.
  * temperature (0, or 1e-6 .. 1e6) 0: a draft stays where it is the row's largest logit (of equals the lowest token), which is also what is drawn.
  * accepted [nseq]: drafts that stay; out_tokens [nrows]: per sequence those, the drawn one, then -1.  A sequence without rows
- * has accepted 0.  Where a row that is reached holds NaN or has no finite maximum the drawn token is -1 (CD_STATUS_LOGITS). */
+ * has accepted 0, one that is left out (CD_STATUS_BATCH) -1, and rows ahead of row_start[nseq] that no other sequence has are -1.  Where a row that is reached holds NaN or has no finite maximum the drawn token is -1 (CD_STATUS_LOGITS). */
 int cd_verify_drafts_workspace(int nrows, int nseq, int vocab, size_t* bytes);
 int cd_verify_drafts(int device, int dtype, int nseq, int nrows, int max_rows, int vocab, const void* target, int64_t target_stride,
                      const void* draft, int64_t draft_stride, const int32_t* tokens, const int32_t* row_start, const float* uniforms,

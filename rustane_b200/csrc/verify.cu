@@ -74,6 +74,8 @@ __device__ inline uint4 load_once(const void* p) {
     return v;
 }
 
+__device__ inline bool rows_fit(const VerifyArgs& p, int r0, int r1) { return r0 >= 0 && r1 >= r0 && r1 <= p.nrows && r1 - r0 <= p.max_rows; }
+
 // (m, at, s) of one chunk.  GREEDY: no sums.
 template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_constant__ VerifyArgs p) {
     constexpr int VEC = 16 / sizeof(T), DEEP = 4;
@@ -97,8 +99,14 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
     // target rows are all there and asked for at once; a draft row only if a draft is behind it, as there need not be memory for others
     if (!is_draft) fetch(tid);
     bool used = false;
-    for (int b = tid; b < p.nseq; b += VD_THREADS) used |= p.row_start[b] <= r && r + is_draft < p.row_start[b + 1];
-    if (!__syncthreads_or(used)) return;
+    for (int b = tid; b < p.nseq; b += VD_THREADS) {
+        const int r0 = p.row_start[b], r1 = p.row_start[b + 1];
+        used |= r0 <= r && r + is_draft < r1 && rows_fit(p, r0, r1);
+    }
+    if (!__syncthreads_or(used)) {
+        if (!is_draft && ch == 0 && tid == 0 && r < p.row_start[p.nseq]) p.out[r] = -1;  // a row that no sequence took
+        return;
+    }
     if (is_draft) fetch(tid);
     const float scale = (float)(p.inv_t * 1.4426950408889634074);
     float m = -INFINITY, s = 0.f;
@@ -250,12 +258,13 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     cg::cluster_group cluster = cg::this_cluster();
     const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / size;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int r0 = p.row_start[b], r1 = p.row_start[b + 1], n = r1 - r0;
+    const int r0 = p.row_start[b], r1 = p.row_start[b + 1], n = (int)((unsigned)r1 - (unsigned)r0);  // (looked at where the rows fit)
     pdl_wait();
-    if (r0 < 0 || r1 < r0 || r1 > p.nrows || n > p.max_rows || n == 0) {
+    const bool fits = rows_fit(p, r0, r1);
+    if (!fits || n == 0) {
         if (rank == 0 && tid == 0) {
-            p.accepted[b] = 0;
-            if (n != 0) report(p.status, CD_STATUS_BATCH);
+            p.accepted[b] = fits ? 0 : -1;
+            if (!fits) report(p.status, CD_STATUS_BATCH);
         }
         return;
     }

@@ -264,7 +264,10 @@ def verify_drafts(target, tokens, row_start, max_rows, uniforms, draws, draft=No
     """Which drafted tokens stay, by given random numbers.  target [rows, vocab]: logits behind each row; tokens [rows] int32: the pending token
     of each sequence, then its drafts; uniforms [rows] and draws [nseq] f32 in [0, 1) (not used at temperature 0, and None is fine there);
     draft [rows, vocab]: the logits the token behind each row was drawn from, None: drafts without a distribution.  Returns
-    (accepted [nseq] int32, out_tokens [rows] int32: the drafts that stay, the drawn token, then -1)."""
+    (accepted [nseq] int32, out_tokens [rows] int32: the drafts that stay, the drawn token, then -1).  A sequence whose rows do not fit (row_start not
+    ascending, past the rows or max_rows) is left out: accepted -1, its rows -1.  A row of logits that is needed and holds NaN or has no finite maximum:
+    the drawn token is -1.  status: an int32 tensor of one element, into which such things are OR-ed as CD_STATUS_* bits.  Rows from
+    row_start[nseq] on are not written."""
     _load_torch()
     _counts(max_rows)
     device, shape = target.device, target.shape

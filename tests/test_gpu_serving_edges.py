@@ -238,3 +238,34 @@ def test_draft_rows_with_no_draft_behind_them_are_not_read(dtype):
         for end in x["starts"][1:].tolist():
             x["draft"][end - 1] = value
         assert verify(x, 0.9) == want
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_sequences_that_are_left_out_say_so(temperature):
+    """accepted -1 and tokens -1, without a look at the status; rows behind the batch keep what they held."""
+    import torch
+
+    from rustane_b200 import _ffi, ops
+    x = verify_inputs([3, 2, 4, 3], 700, "bf16", 12)
+    draft = temperature > 0
+    want_n, want = verify64(x, temperature, draft)
+    target, drafts, tokens, u, d = (x[k].cuda() for k in ("target", "draft", "tokens", "u", "d"))
+    # row_start, the most rows, which sequences fit, the rows of the batch that none of them has
+    for starts, most, fits, free in (([0, 3, -1, 9, 12], 4, [0, 3], range(3, 9)), ([0, 3, 5, 13, 13], 4, [0, 1], range(5, 12)), ([0, 3, 5, 9, 12], 3, [0, 1, 3], range(5, 9)),
+                                     ([2 ** 31 - 1, 3, 5, 9, 9], 4, [1, 2, 3], range(0, 3)), ([-2 ** 31, 3, 5, 2 ** 31 - 1, 12], 4, [1], list(range(0, 3)) + list(range(5, 12)))):
+        row_start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        got_n, got = ops.verify_drafts(target, tokens, row_start, most, u, d, draft=drafts if draft else None, temperature=temperature)
+        end = min(starts[-1], 12)
+        for b in range(4):
+            if b in fits and starts[b] < starts[b + 1]:
+                r0, r1 = starts[b], starts[b + 1]
+                assert int(got_n[b]) == want_n[b] and got[r0:r1].tolist() == want[r0:r1], (starts, b)
+            else:
+                assert int(got_n[b]) == (0 if b in fits else -1), (starts, b)
+        assert all(int(got[r]) == -1 for r in free if r < end), starts
+        # the same through the library, into memory that holds something
+        out, accepted, status = torch.full_like(tokens, 77), torch.full_like(got_n, 77), torch.zeros(1, dtype=torch.int32, device="cuda")
+        ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+        assert _ffi.lib.cd_verify_drafts(0, 2, 4, 12, most, 700, target.data_ptr(), 0, drafts.data_ptr(), 0, tokens.data_ptr(), row_start.data_ptr(), u.data_ptr(), d.data_ptr(),
+                                         temperature, accepted.data_ptr(), out.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
+        assert int(status) == 1 and torch.equal(accepted, got_n) and torch.equal(out[:end], got[:end]) and bool((out[end:] == 77).all())
