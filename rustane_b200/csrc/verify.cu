@@ -6,9 +6,10 @@
 // again.  Bound by the 64-bit exponentials, four a token (44 us for 32 sequences; 92 us with exp() and every logit asked for when it
 // was needed), on one sequence by five barriers of the cluster and the loads between them (10 us).
 //
-// What is decided there are comparisons with given random numbers, so sums must not blur them: the test u q(x) < p(x) takes p(x) and q(x)
-// in 64 bits over row sums of fp32 terms added in 64 bits (off by a few 2^-24 divided by the number of terms that count), and the
-// draw, where every one of `vocab` running sums is a border, is in 64 bits throughout, its row sums included.
+// What is decided there are comparisons with given random numbers, so sums must not blur them.  The test u q(x) < p(x) goes by row sums of
+// fp32 terms (16-byte loads' worth at a time, then over a thread's loads, in fp32; over threads in 64 bits), and where u q(x) is nearer to p(x)
+// than those can tell (VerifyArgs::near, some 3e-5 of it) by sums in 64 bits over both rows, a few microseconds in one call out of a hundred.
+// The draw, where every one of `vocab` running sums is a border, is in 64 bits throughout, its row sums included.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -36,7 +37,7 @@ struct VerifyArgs {
     const float *uniforms, *draws;
     int *accepted, *out, *status;
     Part* parts;  // [2 nrows][VD_CHUNKS]: target rows, then draft rows
-    double inv_t;
+    double inv_t, near;  // near: what the row pass's sums may be off by, of themselves, p's and q's together
     int nseq, nrows, max_rows, vocab, chunks, chunk;  // chunk: elements, a multiple of 8
 };
 
@@ -158,10 +159,12 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
                 m = top;
             }
             const float base = (m == -INFINITY ? 0.f : m);
+            float some = 0.f;
 #pragma unroll
             for (int d = 0; d < DEEP; ++d)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) s += ex2((v[d][e] - base) * scale);
+                for (int e = 0; e < VEC; ++e) some += ex2((v[d][e] - base) * scale);
+            s += some;
         }
     }
     for (int i = v0 + vecs * VEC + tid; i < e1; i += VD_THREADS) one(i);
@@ -245,12 +248,49 @@ template <bool GREEDY> __device__ inline RowStat row_stat(const VerifyArgs& p, c
 }
 
 struct PickShared {
-    int first_bad, valid, at;
+    int first_bad, first_near, stays, valid, at;  // of a sequence's drafts: the first turned down, the first that the row pass's sums cannot decide
     double total[3];  // of this CTA: p's sum, q's sum, what is drawn from
     double red[2][VD_PICK_WARPS];
     float pm, qm;
     RowStat rows[2][VD_KEEP];  // of the sequence's first rows, target and draft, as the tests found them
 };
+
+// Whether the draft behind `row` stays, by sums in 64 bits (all threads of a CTA; the same in every CTA of a cluster).
+template <typename T> __device__ __noinline__ bool stays_by_64_bits(const VerifyArgs& p, int row, PickShared& sh, const double* two_to) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, x = p.tokens[row + 1];
+    const T *target = static_cast<const T*>(p.target) + row * p.target_stride, *draft = p.draft ? static_cast<const T*>(p.draft) + row * p.draft_stride : nullptr;
+    if (warp == 0) {
+        const RowStat t = row_stat<false>(p, load_part(p, row), two_to);
+        const RowStat q = draft ? row_stat<false>(p, load_part(p, p.nrows + row), two_to) : RowStat{0.f, 0, 1.0};
+        if (lane == 0) {
+            sh.pm = t.m;
+            sh.qm = q.m;
+        }
+    }
+    __syncthreads();
+    const double pm = sh.pm, qm = sh.qm;
+    double sp = 0.0, sq = 0.0;
+    for (int i = tid; i < p.vocab; i += VD_PICK_THREADS) {
+        sp += exp_neg(((double)wide(target[i]) - pm) * p.inv_t, two_to);
+        if (draft) sq += exp_neg(((double)wide(draft[i]) - qm) * p.inv_t, two_to);
+    }
+    sp = warp_sum_d(sp);
+    sq = warp_sum_d(sq);
+    if (lane == 0) { sh.red[0][warp] = sp; sh.red[1][warp] = sq; }
+    __syncthreads();
+    if (tid == 0) {
+        sp = sq = 0.0;
+        for (int i = 0; i < VD_PICK_WARPS; ++i) {
+            sp += sh.red[0][i];
+            sq += sh.red[1][i];
+        }
+        const double px = exp_neg(((double)wide(target[x]) - pm) * p.inv_t, two_to) / sp;
+        const double qx = draft ? exp_neg(((double)wide(draft[x]) - qm) * p.inv_t, two_to) / sq : 1.0;
+        sh.stays = (double)p.uniforms[row] * qx < px;
+    }
+    __syncthreads();
+    return sh.stays;
+}
 
 template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const __grid_constant__ VerifyArgs p) {
     extern __shared__ double tiles[];  // sums of this CTA's tiles
@@ -271,34 +311,54 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     __shared__ double two_to[EXP_TABLE];
     if (!GREEDY && tid < EXP_TABLE) two_to[tid] = exp2((double)tid / EXP_TABLE);
     if (tid == 0) {
-        sh.first_bad = n - 1;
+        sh.first_bad = sh.first_near = n - 1;
         sh.valid = 1;
     }
     __syncthreads();
     const T *target = static_cast<const T*>(p.target), *draft = static_cast<const T*>(p.draft);
-    for (int j = warp; j < n - 1; j += VD_PICK_WARPS) {  // (every load that does not hang on another is asked for at once)
-        const int x = p.tokens[r0 + j + 1];
-        const Part tp = load_part(p, r0 + j), qp = draft ? load_part(p, p.nrows + r0 + j) : Part{};
-        const float u = GREEDY ? 0.f : p.uniforms[r0 + j];
-        const bool in = (unsigned)x < (unsigned)p.vocab;
-        const float tx = in && !GREEDY ? wide(target[(r0 + j) * p.target_stride + x]) : 0.f, qx_logit = in && draft ? wide(draft[(r0 + j) * p.draft_stride + x]) : 0.f;
-        const RowStat t = row_stat<GREEDY>(p, tp, two_to);
-        if (lane == 0 && j < VD_KEEP) sh.rows[0][j] = t;
-        bool stays = t.good() && in;
-        if (GREEDY) stays = stays && t.at == x;
-        else {
-            const double px = exp_neg(((double)tx - (double)t.m) * p.inv_t, two_to) / t.z;
-            double qx = 1.0;
-            if (draft) {
-                const RowStat q = row_stat<GREEDY>(p, qp, two_to);
-                if (lane == 0 && j < VD_KEEP) sh.rows[1][j] = q;
-                qx = q.good() ? exp_neg(((double)qx_logit - (double)q.m) * p.inv_t, two_to) / q.z : NAN;
+    for (int from = 0;;) {
+        for (int j = from + warp; j < n - 1; j += VD_PICK_WARPS) {  // (every load that does not hang on another is asked for at once)
+            const int x = p.tokens[r0 + j + 1];
+            const Part tp = load_part(p, r0 + j), qp = draft ? load_part(p, p.nrows + r0 + j) : Part{};
+            const float u = GREEDY ? 0.f : p.uniforms[r0 + j];
+            const bool in = (unsigned)x < (unsigned)p.vocab;
+            const float tx = in && !GREEDY ? wide(target[(r0 + j) * p.target_stride + x]) : 0.f, qx_logit = in && draft ? wide(draft[(r0 + j) * p.draft_stride + x]) : 0.f;
+            const RowStat t = row_stat<GREEDY>(p, tp, two_to);
+            if (lane == 0 && j < VD_KEEP) sh.rows[0][j] = t;
+            bool stays = t.good() && in;
+            if (GREEDY) stays = stays && t.at == x;
+            else {
+                const double px = exp_neg(((double)tx - (double)t.m) * p.inv_t, two_to) / t.z;
+                double qx = 1.0;
+                if (draft) {
+                    const RowStat q = row_stat<GREEDY>(p, qp, two_to);
+                    if (lane == 0 && j < VD_KEEP) sh.rows[1][j] = q;
+                    qx = q.good() ? exp_neg(((double)qx_logit - (double)q.m) * p.inv_t, two_to) / q.z : NAN;
+                }
+                const double uq = (double)u * qx;
+                // (above 0 on both sides: 0 < 0 and NaN are decided)
+                if (stays && uq > 0.0 && fabs(uq - px) <= p.near * px && lane == 0) atomicMin(&sh.first_near, j);
+                stays = stays && uq < px;
             }
-            stays = stays && (double)u * qx < px;
+            if (!stays && lane == 0) atomicMin(&sh.first_bad, j);
         }
-        if (!stays && lane == 0) atomicMin(&sh.first_bad, j);
+        __syncthreads();
+        if (GREEDY) break;
+        // A draft turned down by fp32 sums alone is one of the near ones.  The first of them goes first: what is behind a refused one does not count.
+        const int near = sh.first_near;
+        if (near > sh.first_bad || near == n - 1) break;
+        const bool stays = stays_by_64_bits<T>(p, r0 + near, sh, two_to);
+        if (!stays || near + 1 >= n - 1) {
+            __syncthreads();
+            if (tid == 0) sh.first_bad = stays ? n - 1 : near;
+            __syncthreads();
+            break;
+        }
+        __syncthreads();
+        if (tid == 0) sh.first_bad = sh.first_near = n - 1;
+        __syncthreads();
+        from = near + 1;
     }
-    __syncthreads();
     const int end = sh.first_bad, row = r0 + end;
     const bool left = end < n - 1;  // a draft was turned down: draw from what p has over q
     if (warp == 0) {
@@ -577,6 +637,10 @@ extern "C" int cd_verify_drafts(int device, int dtype, int nseq, int nrows, int 
     const long long rows = (long long)nrows * (a.draft ? 2 : 1), want = std::max<long long>(1, (148 * 8 + rows - 1) / rows);
     a.chunks = (int)std::max<long long>(1, std::min<long long>({want, (vocab + 2047) / 2048, VD_CHUNKS}));
     a.chunk = ((vocab + a.chunks - 1) / a.chunks + 7) & ~7;
+    // What a row's sum may be off by, in units of 2^-24 of it: the exponentials 4; their arguments' three roundings, 3 ln 2 for each of the at most 22 powers
+    // of two that a term of 2^22 lies below the largest on average (weighted by the terms, an entropy); 32 terms summed at a time; a sum over
+    // the loads and a rescaling by another exponential, 8 a load; three joints' exponentials.  p's and q's together twice that.
+    a.near = (4 + 46 + 32 + 8.0 * (a.chunk / (VD_THREADS * 16) + 2) + 24) * 2.0 / (1 << 24);
     cudaError_t e;
     if (dtype == CD_DTYPE_F32) e = launch_mode<float>(a, greedy, a.draft != nullptr, s);
     else if (dtype == CD_DTYPE_F16) e = launch_mode<__half>(a, greedy, a.draft != nullptr, s);

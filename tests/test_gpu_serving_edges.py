@@ -269,3 +269,33 @@ def test_sequences_that_are_left_out_say_so(temperature):
         assert _ffi.lib.cd_verify_drafts(0, 2, 4, 12, most, 700, target.data_ptr(), 0, drafts.data_ptr(), 0, tokens.data_ptr(), row_start.data_ptr(), u.data_ptr(), d.data_ptr(),
                                          temperature, accepted.data_ptr(), out.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
         assert int(status) == 1 and torch.equal(accepted, got_n) and torch.equal(out[:end], got[:end]) and bool((out[end:] == 77).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab,temperature", [(40, 1.0), (5003, 0.7), (32000, 1.0), (128000, 1.3)])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_drafts_on_the_border_of_acceptance(dtype, vocab, temperature, with_draft):
+    """Uniform numbers that are the fp32 neighbours of p(x) / q(x): one below stays, one not below does not.  They lie up to 2^-24 of themselves off the border,
+    which row sums in fp32 cannot tell.  (Those nearer than 2^-38, where the 64-bit forms themselves may differ, are moved a step away.)"""
+    import torch
+    counts = [1, 9, 25, 5, 2, 40]
+    x = verify_inputs(counts, vocab, dtype, 7, near=0.4)
+    p, q = (torch.log_softmax(x[k].double() / temperature, 1) for k in ("target", "draft"))
+    g = torch.Generator("cpu").manual_seed(2)
+    starts = x["starts"].tolist()
+    for b, n in enumerate(counts):
+        stop = int(torch.randint(0, n, (1,), generator=g))  # the draft of this sequence that does not stay (its last row has none)
+        for j in range(n - 1):
+            r = starts[b] + j
+            # a token that q gives more than p, so that the border is below 1 (any token will do without q)
+            x["tokens"][r + 1] = int((q[r] - p[r]).topk(3).indices[int(torch.randint(0, 3, (1,), generator=g))]) if with_draft else int(torch.randint(0, vocab, (1,), generator=g))
+            t = int(x["tokens"][r + 1])
+            border = float(torch.exp(p[r, t] - (q[r, t] if with_draft else 0.0)))
+            u = np.float32(border)
+            below = u if float(u) < border * (1 - 2.0 ** -38) else np.nextafter(u, np.float32(0))
+            above = u if float(u) > border * (1 + 2.0 ** -38) else np.nextafter(u, np.float32(2))
+            x["u"][r] = float(above if j == stop else below)
+    got, out, status = verify(x, temperature, with_draft)
+    want_n, want = verify64(x, temperature, with_draft)
+    assert got == want_n and out == want and status == 0
+    assert max(want_n) > 3  # (several borders in one sequence)
