@@ -299,3 +299,33 @@ def test_drafts_on_the_border_of_acceptance(dtype, vocab, temperature, with_draf
     want_n, want = verify64(x, temperature, with_draft)
     assert got == want_n and out == want and status == 0
     assert max(want_n) > 3  # (several borders in one sequence)
+
+
+# ------------------------------------------------------------------------------------------------ a step as the documents show it
+def test_the_step_in_the_readme():
+    """Its lines as they stand: they run, and the cache it leaves is the one that was brought down (lengths, and what the next step attends over)."""
+    import os
+    import re
+
+    import torch
+
+    from rustane_b200 import ops
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")).read()
+    block = next(b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "PagedCache(" in b)
+    lens0, counts, kv, heads, vocab = [3000, 5, 2049], [2, 1, 3], 2, 4, 900
+    batch = Batch(lens0, counts, kv, 128, 64, "bf16", seed=7, book=True)
+    x = verify_inputs(counts, vocab, "bf16", 7)
+    fused = batch.normal(batch.rows, heads + 2 * kv, 128, dtype="bf16")
+    at = torch.cat([torch.arange(n - c, n) for n, c in zip(lens0, counts)]).to(torch.int32).cuda()
+    names = dict(pool=batch.pool, page_table=batch.table, lens=batch.tlens, weight=batch.weight, position=batch.position, q=fused[:, :heads], k=fused[:, heads:heads + kv],
+                 v=fused[:, heads + kv:], positions=at, row_start=batch.row_start, max_rows=3, target_logits=x["target"].cuda(), draft_logits=x["draft"].cuda(), tokens=x["tokens"].cuda(),
+                 uniforms=x["u"].cuda(), draws=x["d"].cuda())
+    exec(block, names)
+    cache = names["cache"]
+    kept = [min(n, 2048) for n in lens0]
+    assert cache.lens.tolist() == kept and names["accepted"].tolist() == verify64(x, 1.0)[0]
+    q = batch.normal(3, heads, 128, dtype="bf16")
+    one = torch.arange(4, dtype=torch.int32, device="cuda")
+    batch.lens, batch.counts, batch.starts, batch.row_start, batch.rows = kept, [1, 1, 1], np.arange(4), one, 3
+    want, _, mass, _, worst = ref.attention(batch, q)  # (the pool as it is now)
+    assert near(f64(ops.paged_attention(cache, q, one, 1)), want, mass, "bf16", "bf16", 128, worst).all()
