@@ -145,17 +145,13 @@ class PagedCache:
         self.replace(lens, weight, position)
 
     def replace(self, lens=None, weight=None, position=None):
-        """Take other tensors for the lengths or the bookkeeping, as cache_evict returned them."""
-        if lens is not None:
-            self._c.lens = _tensor(lens, "lens", torch.int32, (self.nseq,), self._index)
-            self.lens = lens
+        """Take other tensors for the lengths or the bookkeeping, as cache_evict returned them (all of those given, or none where one does not fit)."""
         shape = (self.nseq, self.kv_heads, self.capacity)
-        if weight is not None:
-            self._c.weight = _tensor(weight, "weight", torch.float32, shape, self._index)
-            self.weight = weight
-        if position is not None:
-            self._c.position = _tensor(position, "position", torch.int32, shape, self._index)
-            self.position = position
+        given = [(name, t, _tensor(t, name, dtype, of, self._index)) for name, t, dtype, of in (
+            ("lens", lens, torch.int32, (self.nseq,)), ("weight", weight, torch.float32, shape), ("position", position, torch.int32, shape)) if t is not None]
+        for name, t, address in given:
+            setattr(self, name, t)
+            setattr(self._c, name, address)
 
     def _workspace(self, given, size, *key):
         """A workspace as `size` (one of the library's *_workspace calls) asks for it."""
