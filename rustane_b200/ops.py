@@ -222,9 +222,11 @@ def rope_append(cache, rope, q, k, v, positions, row_start, out=None):
 
 def paged_attention(cache, q, row_start, max_rows, scale=None, window=0, collect=False, lse=False, out=None, workspace=None):
     """Attention of the new rows q [rows, heads, hd] (f32 or of the pool's type) over the cache, each row up to its own entry, or over its last
-    `window` entries.  max_rows: the most rows a sequence has.  collect: add the probabilities to cache.weight.  Returns out, or
+    `window` entries.  scale: above 0; None: 1 / sqrt(hd).  max_rows: the most rows a sequence has.  collect: add the probabilities to cache.weight.  Returns out, or
     (out, lse [rows, heads] f32) with lse.  Rows from row_start[nseq] on are not written."""
     _counts(max_rows, window)
+    if scale is not None and not scale > 0:
+        raise ValueError("scale must be above 0, got %r" % scale)
     index = cache._index
     shape = q.shape
     rows, heads, collect = shape[0], shape[1], 1 if collect else 0

@@ -20,3 +20,11 @@ def test_a_cache_takes_all_that_replace_gives_or_nothing():
     more = lens.clone()
     cache.replace(more)
     assert cache.lens is more and cache._c.lens == more.data_ptr() and cache.weight is weight
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), 0])
+def test_a_scale_that_is_not_positive_is_refused(R, scale):
+    # (the library takes it for its default, which is not what was asked for; ahead of everything else: no cache is looked at)
+    from rustane_b200 import ops
+    with pytest.raises(ValueError, match="scale"):
+        ops.paged_attention(None, None, None, 1, scale=scale)
