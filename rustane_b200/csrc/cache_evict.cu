@@ -112,11 +112,13 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
     // One pass over weights and positions: the keys as if nothing were protected, the newest position, and a copy of the
     // bookkeeping (what a hole keeps of it the moves write over).
     int newest = INT_MIN;
+    bool low = false;  // an entry of this CTA at a position below `sinks` (with no sinks a negative one)
     for_batches(tid, mine, EV_THREADS, [&](int i) { return make_int2(__float_as_int(weight[s0 + i]), position[s0 + i]); }, [&](int i, int2 v) {
         if (RESIDENT) keys[i] = weight_key(__int_as_float(v.x));
         if (!same_w) weight_out[s0 + i] = __int_as_float(v.x);
         if (!same_p) position_out[s0 + i] = v.y;
         newest = max(newest, v.y);
+        low |= v.y < p.sinks;
     }, true);
     for_batches(len + rank * EV_THREADS + tid, p.c.cap, size * EV_THREADS, [&](int i) { return make_int2(__float_as_int(weight[i]), position[i]); }, [&](int i, int2 v) {
         if (!same_w) weight_out[i] = __int_as_float(v.x);
@@ -124,7 +126,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
     }, !same_w || !same_p);
     newest = __reduce_max_sync(0xffffffffu, newest);
     if (lane == 0) sh.red[warp] = newest;
-    __syncthreads();
+    low = __syncthreads_or(low);
     if (warp == 0) {
         newest = __reduce_max_sync(0xffffffffu, lane < EV_WARPS ? sh.red[lane] : INT_MIN);
         if (lane == 0) sh.newest = newest;
@@ -137,7 +139,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(EV_THREADS) evict_sel
     const long long recent_from = (long long)newest - p.recent;
     auto protects = [&](int pos) { return pos < p.sinks || pos > recent_from; };
     auto key = [&](int i) { return RESIDENT ? keys[i] : protects(position[s0 + i]) ? 0xffffffffu : weight_key(weight[s0 + i]); };
-    if (RESIDENT && (p.sinks > 0 || p.recent > 0))
+    if (RESIDENT && (low || p.recent > 0))
         for_batches(tid, mine, EV_THREADS, [&](int i) { return position[s0 + i]; }, [&](int i, int pos) {
             if (protects(pos)) keys[i] = 0xffffffffu;
         }, true);

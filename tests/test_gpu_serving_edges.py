@@ -301,6 +301,29 @@ def test_drafts_on_the_border_of_acceptance(dtype, vocab, temperature, with_draf
     assert max(want_n) > 3  # (several borders in one sequence)
 
 
+# ------------------------------------------------------------------------------------------------ eviction
+@pytest.mark.parametrize("length,resident", [(300, True), (9001, True), (360000, False)])
+@pytest.mark.parametrize("sinks,recent", [(0, 0), (3, 0), (0, 2), (3, 2)])
+def test_entries_at_positions_below_zero_are_below_any_sinks(length, resident, sinks, recent):
+    """A position below `sinks` stays, and a negative one is below 0: with no sinks and none recent too, however the keys are held."""
+    import torch
+
+    from rustane_b200 import ops
+    batch = Batch([length, length - 7], [0, 0], 1, 64, 64, "bf16", seed=length, book=True, values=length < 10 ** 5)
+    keep = length // 2
+    far = torch.randperm(length - 20, generator=batch.g)[:9]
+    batch.position[:, :, far.cuda()] = -1 - torch.arange(9, dtype=torch.int32, device="cuda")
+    batch.weight[:, :, far.cuda()] = 0.0  # the lightest: only their position keeps them
+    weight, position = f64(batch.weight), batch.position.cpu().numpy()
+    lens, _, new = ops.cache_evict(batch.cache(), keep, sinks=sinks, recent=recent)
+    assert lens.tolist() == [keep, keep]
+    for b, n in enumerate(batch.lens):
+        w, p, got = weight[b, 0, :n], position[b, 0, :n], new[b, 0, :keep].cpu().numpy()
+        safe = (p < sinks) | (p > int(p.max()) - recent)
+        order = np.lexsort((np.arange(n), np.where(safe, -np.inf, -w)))
+        np.testing.assert_array_equal(np.sort(got), np.sort(p[order[:keep]]))
+
+
 # ------------------------------------------------------------------------------------------------ a step as the documents show it
 def test_the_step_in_the_readme():
     """Its lines as they stand: they run, and the cache it leaves is the one that was brought down (lengths, and what the next step attends over)."""
