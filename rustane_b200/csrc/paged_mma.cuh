@@ -288,7 +288,7 @@ __device__ __forceinline__ void mma_unit(const AttnArgs& p, char* ring_all, uint
                     for (int e = 0; e < EL; ++e) most = fmaxf(most, fabsf(x[qk][e]));
                     most = warp_max(most);
                     if (most > 0.f && most < INFINITY) {
-                        const int ex = max(-100, ilogbf(most)) - 7;
+                        const int ex = max(-100, ilogbf(most)) - 14;  // the largest in [2^14, 2^15): two parts keep 2^-22 of elements down to 2^-18 of it
                         back = __int_as_float((127 + ex) << 23);
                         const float by = __int_as_float((127 - ex) << 23);
 #pragma unroll

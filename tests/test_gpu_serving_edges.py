@@ -77,6 +77,27 @@ def test_scores_past_the_digits_of_fp32(q_type, kv_type, hd):
     np.testing.assert_allclose(f64(lse), want_lse, rtol=2.0 ** -21)
 
 
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("down", [8, 16, 20])
+def test_small_elements_of_q_that_meet_large_ones_of_k(q_type, kv_type, hd, down):
+    """One element of q is 2^down times the others, and K holds zeros there and up to 2^14 elsewhere: the scores are sums of the small elements' products.
+    A score's terms are off by 2^-21 of themselves for q's parts and hd 2^-24 for their sum."""
+    from rustane_b200 import ops
+    batch = Batch([300, 64, 1], [1, 2, 1], 2, hd, 16, kv_type, seed=9)
+    batch.pool[:, 0] *= 2.0 ** 12
+    batch.pool[:, 0, :, :, 5] = 0.0
+    q = batch.normal(batch.rows, 6, hd, dtype=q_type) * 2.0 ** -down
+    q[:, :, 5] = 1.0
+    scale = 2.0 ** (down - 12) / 8
+    out, lse = ops.paged_attention(batch.cache(), q, batch.row_start, 2, scale=scale, lse=True)
+    want, want_lse, mass, _, worst = ref.attention(batch, q, scale)
+    part = 2.0 ** -16 if q_type == kv_type == "bf16" else 2.0 ** -20
+    moved = 2 * (hd * 2.0 ** -24 + 2.0 ** -21) * worst
+    assert (np.abs(f64(out) - want) <= HALF_STEP[q_type] * np.abs(want) + (part + moved + 2.0 ** -20) * mass).all()
+    np.testing.assert_allclose(f64(lse), want_lse, atol=(hd + 8) * 2.0 ** -24 * max(worst, 1) + 2.0 ** -20, rtol=2.0 ** -21)
+
+
 def at_entry(batch, b, t):
     return int(batch.table[b, t // batch.page]), t % batch.page
 
