@@ -408,12 +408,14 @@ int cd_rope_frequencies(int rot_dim, double base, int scaling, double factor, in
 int cd_rope_append(const cd_paged_cache* cache, const cd_rope* rope, int dtype, int heads, int nrows, const void* q, int64_t q_stride, const void* k,
                    int64_t k_stride, const void* v, int64_t v_stride, const int32_t* positions, const int32_t* row_start, void* q_out, void* stream);
 
-/* Softmax attention of every new row over the entries up to its own (with window > 0: over the last `window` of them).
- * q, out [nrows][heads][hd] of `dtype` (F32, or the pool's type), q rows q_stride elements apart (0: packed), out packed; heads is
- * a multiple of kv_heads, q head h reads kv head h / (heads / kv_heads).  scale <= 0: 1/sqrt(hd).  lse [nrows][heads]: natural
- * log of the sum of exp(score), or NULL.  A row that sees nothing, or scores of -inf only, gets zeros and -inf.  What a row does not
- * see cannot reach it, NaN and infinities included; those that it sees do to it what the formula says, in fp32.  collect != 0: the probabilities an entry got, summed over the rows and q heads of
- * its kv head, are added to its weight.  Results do not depend on the run: nothing is summed by atomics. */
+/* Softmax attention of every new row over the entries up to its own (with window > 0: over the last `window` of them, by place:
+ * after an eviction these are not the newest ones).  q, out [nrows][heads][hd] of `dtype` (F32, or the pool's type), q rows q_stride elements
+ * apart (0: packed), out packed (it may be q itself where q is packed); heads is a multiple of kv_heads, q head h reads kv head
+ * h / (heads / kv_heads).  scale <= 0: 1/sqrt(hd).  lse [nrows][heads]: natural log of the sum of exp(score), or NULL.  A row that sees
+ * nothing, or scores of -inf only, gets zeros and -inf.  What a row does not see cannot reach it, NaN and infinities included; those
+ * that it sees do to it what the formula says, in fp32.  collect != 0: the probabilities an entry got, summed over the rows and q
+ * heads of its kv head, are added to its weight; the workspace then has a float for every row, head and place of a page_table row.
+ * Results do not depend on the run: nothing is summed by atomics. */
 int cd_paged_attention_workspace(const cd_paged_cache* cache, int heads, int nrows, int max_rows, int collect, size_t* bytes);
 int cd_paged_attention(const cd_paged_cache* cache, int dtype, int heads, int nrows, int max_rows, const void* q, int64_t q_stride,
                        const int32_t* row_start, float scale, int window, int collect, void* out, float* lse, void* workspace,
@@ -422,7 +424,7 @@ int cd_paged_attention(const cd_paged_cache* cache, int dtype, int heads, int nr
 /* Bring every sequence with more than `keep` entries down to `keep`, for each kv head on its own.  Entries at positions below
  * `sinks` or above the head's newest position - `recent` come first (sinks + recent <= keep), then the heaviest; of equals
  * the one in the lower place; NaN counts as the lightest.  Kept entries that lie in places from `keep` on move into the places that
- * fell free below, in order; the others stay where they are.  K and V move in the pool, so its pages must not be shared between
+ * fell free below, in order; the others stay where they are (so places are not in order of position any more).  K and V move in the pool, so its pages must not be shared between
  * sequences; lens_out [nseq], weight_out and position_out (shaped as the cache's, and may be those) receive the bookkeeping, places
  * from the new length on as they were.  lens_out must not be lens.
  * max_pages * page_tokens <= 2^30, nseq * kv_heads <= 65535.  Entries of a page outside the pool do not move (CD_STATUS_PAGE). */

@@ -202,7 +202,8 @@ def rope_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, original=4
 def rope_append(cache, rope, q, k, v, positions, row_start, out=None):
     """Rotate q [rows, heads, hd] and k [rows, kv_heads, hd] at `positions` [rows] int32, write k and v to their entries in the cache (with
     bookkeeping: weight 0, the position noted), return the rotated q.  q, k and v are f32 or of the pool's type; they may be
-    slices of one fused projection.  out: a packed tensor for the result; q itself where q is packed."""
+    slices of one fused projection.  out: a packed tensor for the result; q itself where q is packed.  Rows of a sequence that does not
+    fit (cache.status says so) and rows from row_start[nseq] on are not written."""
     index, hd = cache._index, cache.hd
     rows, dtype = q.shape[0], q.dtype
     sq, sk, sv = _row_stride(q, "q", rows, hd, index), _row_stride(k, "k", rows, hd, index), _row_stride(v, "v", rows, hd, index)
@@ -223,7 +224,9 @@ def rope_append(cache, rope, q, k, v, positions, row_start, out=None):
 def paged_attention(cache, q, row_start, max_rows, scale=None, window=0, collect=False, lse=False, out=None, workspace=None):
     """Attention of the new rows q [rows, heads, hd] (f32 or of the pool's type) over the cache, each row up to its own entry, or over its last
     `window` entries.  scale: above 0; None: 1 / sqrt(hd).  max_rows: the most rows a sequence has.  collect: add the probabilities to cache.weight.  Returns out, or
-    (out, lse [rows, heads] f32) with lse.  Rows from row_start[nseq] on are not written."""
+    (out, lse [rows, heads] f32) with lse.  out: a packed tensor for the result; q itself where q is packed.  Rows of a sequence that does not fit
+    (cache.status says so) and rows from row_start[nseq] on are not written.  `window` counts entries: after an eviction the places are not in order of
+    position, and the last `window` of them are not the newest ones."""
     _counts(max_rows, window)
     if scale is not None and not scale > 0:
         raise ValueError("scale must be above 0, got %r" % scale)
@@ -243,7 +246,8 @@ def paged_attention(cache, q, row_start, max_rows, scale=None, window=0, collect
 
 def cache_evict(cache, keep, sinks=0, recent=0, out=None, workspace=None):
     """Bring every sequence with more than `keep` entries down to `keep`, each kv head by its own weights; positions below `sinks` and the
-    newest `recent` ones stay.  K and V move within the cache's pages.  Returns new (lens, weight, position), which the caller
+    newest `recent` ones stay.  K and V move within the cache's pages, which no two sequences may share (a common prefix has to be copied
+    first), and the entries that stay are not in order of position afterwards.  Returns new (lens, weight, position), which the caller
     hands to cache.replace(); out: tensors for them (weight and position may be the cache's own, lens may not)."""
     _counts(keep, sinks, recent)
     index = cache._index

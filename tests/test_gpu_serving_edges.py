@@ -373,3 +373,90 @@ def test_the_step_in_the_readme():
     batch.lens, batch.counts, batch.starts, batch.row_start, batch.rows = kept, [1, 1, 1], np.arange(4), one, 3
     want, _, mass, _, worst = ref.attention(batch, q)  # (the pool as it is now)
     assert near(f64(ops.paged_attention(cache, q, one, 1)), want, mass, "bf16", "bf16", 128, worst).all()
+
+
+# ------------------------------------------------------------------------------------------------ the most that calls take, and calls beside others
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+def test_as_many_sequences_as_there_may_be(q_type, kv_type):
+    """4096 sequences of 0 to 9 entries and 0 to 4 rows: attention, append and eviction."""
+    import torch
+
+    from rustane_b200 import ops
+    rng = np.random.default_rng(4)
+    lens, counts = [int(n) for n in rng.integers(0, 10, 4096)], [int(n) for n in rng.integers(0, 5, 4096)]
+    batch = Batch(lens, counts, 1, 64, 4, kv_type, seed=6, book=True)
+    q = batch.normal(batch.rows, 5, 64, dtype=q_type)
+    out, lse = attend(batch, q, collect=False)
+    want, want_lse, mass, _, worst = ref.attention(batch, q)
+    seen = np.isfinite(want_lse)
+    assert (np.isneginf(lse) == ~seen).all() and near(out, want, mass, q_type, kv_type, 64, worst).all()
+    k = batch.normal(batch.rows, 1, 64, dtype=q_type)
+    at, cache = torch.arange(batch.rows, dtype=torch.int32, device="cuda"), batch.cache()
+    before = batch.pool.clone()
+    turned = ops.rope_append(cache, ops.Rope(64), q, k, k, at, batch.row_start)
+    freq, magnitude = ref.frequencies(64, 10000.0, None, 1.0, 1)
+    angle = np.abs(f64(turned) - ref.rotate(f64(q), np.arange(batch.rows), freq, magnitude, "half"))
+    size = np.abs(f64(q)) + np.abs(np.roll(f64(q), 32, -1))
+    assert (angle <= HALF_STEP[q_type] * size * 1.5 + 10 * 2.0 ** -24 * size + 2.0 ** -25).all()
+    short = any(c > n for n, c in zip(lens, counts))
+    assert int(cache.status) == (1 if short else 0)  # rows that have no entry
+    for b in rng.integers(0, 4096, 200):
+        n, m = lens[b], counts[b]
+        r0, fit = int(batch.starts[b]), min(m, n)
+        assert np.array_equal(batch.entries(b, 1)[0, n - fit:], f64(k.to(batch.pool.dtype))[r0 + m - fit:r0 + m, 0])
+        assert np.array_equal(batch.entries(b, 1)[0, :n - fit], batch.entries(b, 1, before)[0, :n - fit])
+    weight, position = f64(batch.weight), batch.position.cpu().numpy()
+    lens1, _, new = ops.cache_evict(batch.cache(), 6, sinks=1, recent=2)
+    assert lens1.tolist() == [min(n, 6) for n in lens]
+    new = new.cpu().numpy()
+    for b in rng.integers(0, 4096, 300):
+        moved = position[b, 0].copy()
+        for to, of in ref.evict(weight[b, 0], position[b, 0], lens[b], 6, 1, 2):
+            moved[to] = position[b, 0, of]
+        assert np.array_equal(new[b, 0], moved)
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("page", [1000, 4096, 65536])
+def test_pages_longer_than_the_sequences(q_type, kv_type, page):
+    batch = Batch([page + 3, 70, page], [1, 3, 2], 2, 64, page, kv_type, seed=1)
+    q = batch.normal(batch.rows, 4, 64, dtype=q_type)
+    out, _ = attend(batch, q)
+    want, _, mass, _, worst = ref.attention(batch, q)
+    assert near(out, want, mass, q_type, kv_type, 64, worst).all()
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
+def test_the_same_bits_beside_other_work_and_in_place(q_type, kv_type):
+    """Units of one, two and four row warps, cut over several CTAs: call after call while another stream keeps the GPU busy, and into q itself."""
+    import torch
+
+    from rustane_b200 import ops
+    lens, counts = [9000, 5011, 64, 12000, 700, 1], [6, 2, 1, 8, 4, 1]
+    batch = Batch(lens, counts, 2, 64, 16, kv_type, seed=8, book=True)
+    q, cache = batch.normal(batch.rows, 16, 64, dtype=q_type), batch.cache()
+    first, lse = ops.paged_attention(cache, q, batch.row_start, 8, lse=True)
+    weight = batch.weight.clone()
+    collected, _ = ops.paged_attention(cache, q, batch.row_start, 8, lse=True, collect=True)
+    got = batch.weight.clone()
+    noise, side = torch.randn(1 << 26, device="cuda"), torch.cuda.Stream()
+    for i in range(40):
+        with torch.cuda.stream(side):
+            noise.mul_(1.0001)
+        batch.weight.copy_(weight)
+        again, again_lse = ops.paged_attention(cache, q, batch.row_start, 8, lse=True, collect=i % 2 == 1)
+        assert torch.equal(again, first) and torch.equal(again_lse, lse)
+        assert torch.equal(batch.weight, got if i % 2 else weight)
+    assert torch.equal(collected, first)
+    assert torch.equal(ops.paged_attention(cache, q, batch.row_start, 8), first)
+    mine = q.clone()
+    assert ops.paged_attention(cache, mine, batch.row_start, 8, out=mine) is mine and torch.equal(mine, first)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("temperature,with_draft", [(0.0, False), (0.8, True), (0.8, False)])
+def test_as_large_a_vocabulary_as_there_may_be(dtype, temperature, with_draft):
+    x = verify_inputs([2, 1], 1 << 22, dtype, 3)
+    got, out, status = verify(x, temperature, with_draft)
+    assert (got, out) == verify64(x, temperature, with_draft) and status == 0
