@@ -81,12 +81,15 @@ template <typename KT, typename QT> struct MmaForm {
 constexpr int MMA_STAGE = 8192;  // bytes of a stage: K, then V
 // CTAs an SM, and stages of a CTA, which its groups share: two of twelve, at 224 registers a thread (they leave room for the joint's CTAs).
 // Half the columns need half the sums: at hd 64, with units of one row warp, three CTAs of eight stages at 160 registers (48 sequences of up to
-// 822 entries, 16 kv heads: 65 us for 69; but 106 for 88 on drafted rows, whose groups of four warps want the deeper ring).  The parts
-// of 32-bit q for several row warps take the room of four stages.
+// 822 entries, 16 kv heads: 65 us for 69).  Drafted rows, whose units have several row warps, lose by it (106 us for 88; a group of four warps has
+// four stages either way, so it is not the ring: fewer registers or fewer turns a CTA).  The parts of 32-bit q for several row warps take
+// the room of four stages.
 template <typename QT, int HD> struct MmaSize {
     static constexpr bool WIDE = std::is_same<QT, float>::value;
     static bool three(int row_warps) { return HD == 64 && !WIDE && row_warps == 1; }
     static int slots(int row_warps) { return three(row_warps) || (WIDE && row_warps > 1) ? 8 : 12; }
+    // the most row warps that a build with so many stages meets
+    __device__ static constexpr int most(int slots) { return (slots == 8) != WIDE && (WIDE || HD == 64) ? 1 : 4; }
 };
 template <typename KT, typename QT, int HD> inline size_t mma_shared(int nseq, int row_warps) {
     const size_t q = (size_t)row_warps * MmaForm<KT, QT>::NQ * (HD / 16) * 32 * 16, ring = (size_t)MmaSize<QT, HD>::slots(row_warps) * MMA_STAGE;
@@ -514,7 +517,8 @@ template <typename KT, typename QT, int HD, int SLOTS, int REGS> __global__ void
     const int total = line_up(p, pre, sums, most);
     walk_line(p, pre, total, most, [&](const SeqWork& w, int b, int kvh, int block, int tile, int tiles, bool whole, size_t slot) {
         const int rows = min(p.ru, w.s.n * p.group - block * p.ru);
-        if (rows <= 16) mma_unit<KT, QT, HD, 1, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        if constexpr (MmaSize<QT, HD>::most(SLOTS) == 1) mma_unit<KT, QT, HD, 1, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
+        else if (rows <= 16) mma_unit<KT, QT, HD, 1, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
         else if (rows <= 32) mma_unit<KT, QT, HD, 2, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
         else mma_unit<KT, QT, HD, 4, SLOTS>(p, ring, sq, sh, w, b, kvh, block, tile, tiles, whole, slot);
     });
