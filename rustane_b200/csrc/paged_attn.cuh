@@ -87,15 +87,6 @@ __device__ inline int line_up(const AttnArgs& p, int* pre, int* sums, int& most)
     return carry;
 }
 
-template <typename T> __device__ inline T from_float(float v);
-template <> __device__ inline float from_float<float>(float v) { return v; }
-template <> __device__ inline __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <typename T> __device__ inline float as_float(T v);
-template <> __device__ inline float as_float<float>(float v) { return v; }
-template <> __device__ inline float as_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ inline float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-
 constexpr float LN2 = 0.69314718055994530942f;
 
 // One row's end: o relative to 2^m with sum l.  l is 0 where nothing was seen.

@@ -39,12 +39,6 @@ template <typename KT> __device__ inline uint32_t finite_part(uint32_t w) {
     const uint32_t e = w & Bits16<KT>::EXP;
     return w & (((e & 0xffffu) == (Bits16<KT>::EXP & 0xffffu) ? 0u : 0xffffu) | ((e >> 16) == (Bits16<KT>::EXP >> 16) ? 0u : 0xffff0000u));
 }
-// 2^x to 2^-22 of itself; 0 for -inf
-__device__ inline float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // (a, b) as a pair of 16-bit numbers; a and b become what is left
 template <typename KT> __device__ inline uint32_t take_part(float& a, float& b);
 template <> __device__ inline uint32_t take_part<__half>(float& a, float& b) {

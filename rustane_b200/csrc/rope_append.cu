@@ -40,14 +40,6 @@ __device__ inline float2 cos_sin(uint64_t turns, int position, float magnitude) 
     return make_float2(c * magnitude, s * magnitude);
 }
 
-template <typename T> __device__ inline float widen(T v);
-template <> __device__ inline float widen<float>(float v) { return v; }
-template <> __device__ inline float widen<__half>(__half v) { return __half2float(v); }
-template <> __device__ inline float widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ inline void narrow(float v, float& o) { o = v; }
-__device__ inline void narrow(float v, __half& o) { o = __float2half_rn(v); }
-__device__ inline void narrow(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
-
 // E elements; 16-byte accesses where they fill some
 template <typename T, int E> __device__ inline void load(const T* p, float (&x)[E]) {
     if constexpr (E * sizeof(T) % 16 == 0) {
@@ -55,11 +47,11 @@ template <typename T, int E> __device__ inline void load(const T* p, float (&x)[
         for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) {
             const uint4 w = *(reinterpret_cast<const uint4*>(p) + i);
 #pragma unroll
-            for (int e = 0; e < (int)(16 / sizeof(T)); ++e) x[i * (16 / sizeof(T)) + e] = widen(reinterpret_cast<const T*>(&w)[e]);
+            for (int e = 0; e < (int)(16 / sizeof(T)); ++e) x[i * (16 / sizeof(T)) + e] = as_float(reinterpret_cast<const T*>(&w)[e]);
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = widen(p[e]);
+        for (int e = 0; e < E; ++e) x[e] = as_float(p[e]);
     }
 }
 template <typename T, int E> __device__ inline void store(T* p, const float (&x)[E]) {
@@ -68,12 +60,12 @@ template <typename T, int E> __device__ inline void store(T* p, const float (&x)
         for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) {
             uint4 w;
 #pragma unroll
-            for (int e = 0; e < (int)(16 / sizeof(T)); ++e) narrow(x[i * (16 / sizeof(T)) + e], reinterpret_cast<T*>(&w)[e]);
+            for (int e = 0; e < (int)(16 / sizeof(T)); ++e) reinterpret_cast<T*>(&w)[e] = from_float<T>(x[i * (16 / sizeof(T)) + e]);
             *(reinterpret_cast<uint4*>(p) + i) = w;
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) narrow(x[e], p[e]);
+        for (int e = 0; e < E; ++e) p[e] = from_float<T>(x[e]);
     }
 }
 

@@ -59,6 +59,21 @@ __device__ inline size_t row_at(const PagedView& c, int page, int which, int hea
     return ((((size_t)page * 2 + which) * c.kv_heads + head) * c.page_tokens + off) * hd;
 }
 
+template <typename T> __device__ inline T from_float(float v);
+template <> __device__ inline float from_float<float>(float v) { return v; }
+template <> __device__ inline __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <typename T> __device__ inline float as_float(T v);
+template <> __device__ inline float as_float<float>(float v) { return v; }
+template <> __device__ inline float as_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ inline float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+// 2^x to 2^-22 of itself; 0 for -inf
+__device__ inline float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 // The caller's device for the length of a call.
 struct DeviceGuard {

@@ -41,17 +41,6 @@ struct VerifyArgs {
     int nseq, nrows, max_rows, vocab, chunks, chunk;  // chunk: elements, a multiple of 8
 };
 
-template <typename T> __device__ inline float wide(T v);
-template <> __device__ inline float wide<float>(float v) { return v; }
-template <> __device__ inline float wide<__half>(__half v) { return __half2float(v); }
-template <> __device__ inline float wide<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-// 2^x to 2^-22 of itself; 0 for -inf
-__device__ inline float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // e^x in 64 bits for x <= 0 (or a little above): e^x = 2^(n / 256) e^r with |r| <= ln 2 / 512, e^r by its series up to r^4 / 24 (the next
 // term is below 4e-17), 2^(j / 256) from a table.  Off by some 1e-16, and by x times 1e-16.  What the draw costs is the 64-bit pipe:
 // eight operations here against about twice that in exp().
@@ -114,7 +103,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
     int at = 0x7fffffff;
     bool nan = false;
     auto one = [&](int i) {  // a ragged end
-        const float v = wide(x[i]);
+        const float v = as_float(x[i]);
         if (GREEDY) {
             nan |= v != v;
             if (v > m || (v == m && i < at)) { m = v; at = i; }
@@ -132,7 +121,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_THREADS)
 #pragma unroll
         for (int d = 0; d < DEEP; ++d)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[d][e] = wide(reinterpret_cast<const T*>(&w[d])[e]);
+            for (int e = 0; e < VEC; ++e) v[d][e] = as_float(reinterpret_cast<const T*>(&w[d])[e]);
         if (i + (DEEP - 1) * VD_THREADS >= vecs)
 #pragma unroll
             for (int d = 0; d < DEEP; ++d)
@@ -271,8 +260,8 @@ template <typename T> __device__ __noinline__ bool stays_by_64_bits(const Verify
     const double pm = sh.pm, qm = sh.qm;
     double sp = 0.0, sq = 0.0;
     for (int i = tid; i < p.vocab; i += VD_PICK_THREADS) {
-        sp += exp_neg(((double)wide(target[i]) - pm) * p.inv_t, two_to);
-        if (draft) sq += exp_neg(((double)wide(draft[i]) - qm) * p.inv_t, two_to);
+        sp += exp_neg(((double)as_float(target[i]) - pm) * p.inv_t, two_to);
+        if (draft) sq += exp_neg(((double)as_float(draft[i]) - qm) * p.inv_t, two_to);
     }
     sp = warp_sum_d(sp);
     sq = warp_sum_d(sq);
@@ -284,8 +273,8 @@ template <typename T> __device__ __noinline__ bool stays_by_64_bits(const Verify
             sp += sh.red[0][i];
             sq += sh.red[1][i];
         }
-        const double px = exp_neg(((double)wide(target[x]) - pm) * p.inv_t, two_to) / sp;
-        const double qx = draft ? exp_neg(((double)wide(draft[x]) - qm) * p.inv_t, two_to) / sq : 1.0;
+        const double px = exp_neg(((double)as_float(target[x]) - pm) * p.inv_t, two_to) / sp;
+        const double qx = draft ? exp_neg(((double)as_float(draft[x]) - qm) * p.inv_t, two_to) / sq : 1.0;
         sh.stays = (double)p.uniforms[row] * qx < px;
     }
     __syncthreads();
@@ -322,7 +311,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
             const Part tp = load_part(p, r0 + j), qp = draft ? load_part(p, p.nrows + r0 + j) : Part{};
             const float u = GREEDY ? 0.f : p.uniforms[r0 + j];
             const bool in = (unsigned)x < (unsigned)p.vocab;
-            const float tx = in && !GREEDY ? wide(target[(r0 + j) * p.target_stride + x]) : 0.f, qx_logit = in && draft ? wide(draft[(r0 + j) * p.draft_stride + x]) : 0.f;
+            const float tx = in && !GREEDY ? as_float(target[(r0 + j) * p.target_stride + x]) : 0.f, qx_logit = in && draft ? as_float(draft[(r0 + j) * p.draft_stride + x]) : 0.f;
             const RowStat t = row_stat<GREEDY>(p, tp, two_to);
             if (lane == 0 && j < VD_KEEP) sh.rows[0][j] = t;
             bool stays = t.good() && in;
@@ -402,7 +391,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VD_PICK_THR
     constexpr int PER = VD_TILE / 32;  // tokens of a tile a lane has
     auto logits = [&](const T* row_, int first, int step, float (&x)[PER]) {  // all of them asked for before one is used
 #pragma unroll
-        for (int e = 0; e < PER; ++e) x[e] = first + e * step < p.vocab ? wide(row_[first + e * step]) : -INFINITY;
+        for (int e = 0; e < PER; ++e) x[e] = first + e * step < p.vocab ? as_float(row_[first + e * step]) : -INFINITY;
     };
     const int all_tiles = (p.vocab + VD_TILE - 1) / VD_TILE, per = (all_tiles + size - 1) / size;
     const int t0 = min(all_tiles, rank * per), t1 = min(all_tiles, t0 + per);
@@ -633,8 +622,10 @@ extern "C" int cd_verify_drafts(int device, int dtype, int nseq, int nrows, int 
     a.nrows = nrows;
     a.max_rows = max_rows;
     a.vocab = vocab;
-    // chunks of a row: enough CTAs for the GPU (148 SMs, eight each), none below 2048 elements
-    const long long rows = (long long)nrows * (a.draft ? 2 : 1), want = std::max<long long>(1, (148 * 8 + rows - 1) / rows);
+    // chunks of a row: enough CTAs for the GPU (eight an SM), none below 2048 elements
+    int sms = 0;
+    if (cudaError_t e = sm_count(&sms); e != cudaSuccess) return cuda_status(e, CALL);
+    const long long rows = (long long)nrows * (a.draft ? 2 : 1), want = std::max<long long>(1, (sms * 8 + rows - 1) / rows);
     a.chunks = (int)std::max<long long>(1, std::min<long long>({want, (vocab + 2047) / 2048, VD_CHUNKS}));
     a.chunk = ((vocab + a.chunks - 1) / a.chunks + 7) & ~7;
     // What a row's sum may be off by, in units of 2^-24 of it: the exponentials 4; their arguments' three roundings, 3 ln 2 for each of the at most 22 powers
