@@ -116,6 +116,12 @@ __device__ __noinline__ void rows_again(const AttnArgs& p, const SeqWork& w, int
         uint32_t marked = 0;
         for (int at = rw; at < PA_WARPS; at += row_warps) marked |= (rr < 8 ? marks[at].x : marks[at].y) >> 4 * (rr % 8) & 1u;
         if (!marked) continue;
+        // a row with NaN in q is NaN already (a batch padded with rows of anything is not to pay for them)
+        const int rho = block * p.ru + r;
+        const QT* q = static_cast<const QT*>(p.q) + (size_t)(w.s.r0 + rho / p.group) * p.q_stride + (size_t)(kvh * p.group + rho % p.group) * HD;
+        bool nan = false;
+        for (int d = lane; d < HD; d += 32) nan |= isnan(as_float(q[d]));
+        if (__any_sync(0xffffffffu, nan)) continue;
         float o[1][HD / 8], m[1], l[1];
         fma_rows<KT, QT, HD, 1>(p, w, b, kvh, block * p.ru + r, first, end, 4, m, l, o);
         fma_store<KT, HD, 1>(m, l, o, ml + rw * 16 + rr, so + (rw * 16 + rr) * (HD + PAD), HD + PAD);

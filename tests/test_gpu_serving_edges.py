@@ -181,6 +181,24 @@ def test_infinities_of_k(q_type, kv_type, hd, heads, counts):
 
 
 @pytest.mark.parametrize("q_type,kv_type", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_rows_of_q_that_are_not_finite(q_type, kv_type, value):
+    """One element of one head's row: its scores are NaN (or of both infinities), and so is the row and its log-sum-exp; no other row changes a bit."""
+    batch = Batch([70, 3000, 20], [3, 1, 20], 2, 64, 16, kv_type, seed=6)
+    q = batch.normal(batch.rows, 8, 64, dtype=q_type)
+    clean, clean_lse = attend(batch, q)
+    hit = [(1, 3), (3, 0), (3, 7), (23, 5)]
+    for row, head in hit:
+        q[row, head, 17] = value
+    out, lse = attend(batch, q)
+    mask = np.zeros(lse.shape, dtype=bool)
+    mask[tuple(zip(*hit))] = True
+    assert np.isnan(out[mask]).all() and np.isnan(lse[mask]).all()
+    np.testing.assert_array_equal(out[~mask], clean[~mask])
+    np.testing.assert_array_equal(lse[~mask], clean_lse[~mask])
+
+
+@pytest.mark.parametrize("q_type,kv_type", TYPES)
 @pytest.mark.parametrize("page", [7, 16])
 def test_rows_of_nothing_but_infinite_scores(q_type, kv_type, page):
     """Every score of a row -inf: no entry has weight, the row is zeros and -inf, its neighbours are not touched."""
