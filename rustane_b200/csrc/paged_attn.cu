@@ -15,7 +15,9 @@ struct Plan {
     long long score_stride;
 };
 // What a tile costs by its unit's rows: up to 16, 32, more (tensor-core form).  A CTA's four warps work on four places at once, on two, on
-// one; HBM evens out part of it.  24 sequences of one to six drafted rows, eight heads a kv head: 93 us with costs of 1, 1 and 2, 87 with these.
+// one; HBM evens out part of it.  24 sequences of one to six drafted rows, eight heads a kv head, with these costs, with 1, 2, 4 and with 1, 1, 2: fp16,
+// heads of 64, 96, 98 and 100 us; bf16, heads of 128, 126, 121 and 134; fp32 rows over bf16, heads of 64, 132, 139 and 132; over fp16, heads
+// of 128, 111, 108 and 114.  Four heads and one to eight rows, bf16, 128: 55, 55 and 63; sixteen heads and one to four rows 142, 142 and 148.
 constexpr int PA_WEIGHTS[3] = {2, 4, 7};
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 

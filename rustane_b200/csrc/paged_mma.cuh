@@ -6,14 +6,14 @@
 // bits of its place (chunk ^ place & 7), so that ldmatrix meets every bank once and an address is one XOR.  A group of one warp meets no
 // barrier inside the loop.
 //
-// What bounds it: HBM where one warp has a unit's rows (5.5 TB/s on a ragged batch of 48 over 1.6 GB; 130001 entries of four heads, 266 MB, 55 us
-// with their joint: 4.7 TB/s, the rest is the launch, the line and the ends of two kernels), the chain of a step's instructions, 5 to 9
-// cycles each, where four do (48 rows over 167 MB 88 us), and the way to the first instruction of everything on a token of a few
-// chats (11 us): a kernel's first pass waits for its code more than for data, so copies and rare cases stand in the code once.
+// What bounds it: HBM where one warp has a unit's rows (5.9 TB/s on a ragged batch of 48 over 1.6 GB, 272 us; 130001 entries of four heads, 266 MB,
+// 56 us with their joint: 4.7 TB/s, the rest is the launch, the line and the ends of two kernels), the chain of a step's instructions, 5 to 9
+// cycles each, where four do (48 rows over 167 MB 96 to 102 us), and the way to the first instruction of everything on a token of a few
+// chats (11 us): a kernel's first pass waits for its code as well as for data, so copies stand in the code once and rare cases out of line.
 //
-// Forms measured on the way (the kernel alone, 130001 entries): K and V straight to registers, no ring, 70 us; boxes by TMA, issued by a
-// group's first thread, 59 (and 317 for 290 on the ragged batch of fp32 rows); by producer warps of their own, with the registers
-// split, 64; three CTAs an SM with two stages and 168 registers 58, but the joint 6 us later, for which they leave no room.
+// Forms measured on the way (the kernel alone, 130001 entries, where this one took 53): K and V straight to registers, no ring, 70 us; boxes by TMA,
+// issued by a group's first thread, 59 (and 317 on the ragged batch of fp32 rows, then 290); by producer warps of their own, with the
+// registers split, 64; three CTAs an SM with two stages and 168 registers 58, but the joint 6 us later, for which they leave no room.
 //
 // mma.sync and not tcgen05: a token's unit has 1 to 16 rows, of a 64-row minimum there, and the work is bound by the bytes of K and V.
 //

@@ -4,7 +4,7 @@
 // and exponentials (0.6 instructions a cycle and scheduler; 254 rows of 128000 bf16 logits, 65 MB, 19 us).  verify_pick_kernel, a cluster
 // of CTAs per sequence, puts the chunks together, tests the drafts, and draws from the one row (pair of rows) it ended at, which it reads
 // again.  Bound by the 64-bit exponentials, four a token (44 us for 32 sequences; 92 us with exp() and every logit asked for when it
-// was needed), on one sequence by five barriers of the cluster and the loads between them (10 us).
+// was needed), on one sequence by five barriers of the cluster and the loads between them (11 us).
 //
 // What is decided there are comparisons with given random numbers, so sums must not blur them.  The test u q(x) < p(x) goes by row sums of
 // fp32 terms (16-byte loads' worth at a time, then over a thread's loads, in fp32; over threads in 64 bits), and where u q(x) is nearer to p(x)
